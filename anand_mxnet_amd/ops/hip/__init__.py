@@ -890,6 +890,65 @@ class _FlashMha(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+def _rows16(t):
+    """The tensor itself if the kernels can read its rows 16 bytes at a
+    time (any batch and row stride), else a packed copy."""
+    if (t.stride(2) == 1 and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0
+            and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class _ShapedMha(torch.autograd.Function):
+    """Attention with shaped scores (attn_mod_fwd.hip, attn_mod_bwd.hip):
+    the backward recomputes the scores from the saved log-sums; nothing is
+    summed through atomics, so it gives the same bits every time."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, conf, slopes, seg_q, seg_k, prefix, kv_len,
+                q_off, off0):
+        opts = (slopes, seg_q, seg_k, prefix, kv_len, q_off)
+        out, lse, *rng = _C.attn_mod_fwd(q, k, v, *conf, *opts, off0, True)
+        ctx.save_for_backward(q, k, v, out, lse, *opts, *rng)
+        ctx.conf = conf
+        ctx.off0 = off0
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, *rest = ctx.saved_tensors
+        opts, rng = rest[:6], (rest[6:] or [None, None])
+        need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        grads = _C.attn_mod_bwd(q, k, v, out, _rows16(dout), lse, *rng,
+                                *ctx.conf, *opts, ctx.off0, need_kv)
+        return tuple(grads) + (None,) * (11 - len(grads))
+
+
+# Up to this many rows (query tokens times heads of a group) the form that
+# splits the keys is taken; above, that of 128 queries a block.
+_DECODE_ROWS = 64
+
+
+@register_gpu("shaped_mha")
+def shaped_mha(q, k, v, num_heads, num_kv_heads, scale, cap, causal, slopes,
+               seg_q, seg_k, prefix, kv_len, q_off, off0):
+    if q.numel() == 0 or k.shape[1] == 0:
+        # nothing to see: zero rows that still belong to the graph
+        return q * 0 + (k.sum() + v.sum()) * 0
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    conf = (num_heads, num_kv_heads, scale, cap, causal)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                    or v.requires_grad):
+        return _ShapedMha.apply(q, k, v, conf, slopes, seg_q, seg_k, prefix,
+                                kv_len, q_off, off0)
+    if seg_q is None and q.shape[1] * (num_heads // num_kv_heads) \
+            <= _DECODE_ROWS:
+        return _C.attn_decode(q, k, v, *conf, slopes, prefix, kv_len, q_off,
+                              off0)
+    return _C.attn_mod_fwd(q, k, v, *conf, slopes, seg_q, seg_k, prefix,
+                           kv_len, q_off, off0, False)[0]
+
+
 import os as _os
 _USE_FLASH = _os.environ.get("MXA_FLASH", "1") != "0"
 

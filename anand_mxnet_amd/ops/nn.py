@@ -425,14 +425,184 @@ def embedding_impl(data, weight):
 
 # ---------------- attention (contrib/transformer parity) ----------------
 
+def _attn_ints(x, shape, what, q):
+    """An optional integer tensor of the given shape, as int32 on q's
+    device."""
+    from ..base import MXNetError
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor) or x.dtype.is_floating_point \
+            or x.dtype in (torch.bool, torch.complex64):
+        raise MXNetError(f"multi_head_attention: {what} must be an integer "
+                         f"array")
+    if tuple(x.shape) != shape:
+        raise MXNetError(f"multi_head_attention: {what} must have shape "
+                         f"{shape}, got {tuple(x.shape)}")
+    if x.device != q.device:
+        raise MXNetError(f"multi_head_attention: {what} is on {x.device}, "
+                         f"the queries are on {q.device}")
+    return x.to(torch.int32).contiguous()
+
+
+def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
+                causal, seg_q, seg_k, prefix, kv_len, q_off):
+    """Checks and dispatch of the shaped forms of multi_head_attention."""
+    from ..base import MXNetError
+
+    def need(ok, what):
+        if not ok:
+            raise MXNetError("multi_head_attention: " + what)
+
+    need(q.dim() == 3 and k.dim() == 3 and v.dim() == 3,
+         "query, key and value must be (batch, tokens, heads * size)")
+    B, Tq, HD = q.shape
+    Tk = k.shape[1]
+    H, Hkv = int(num_heads), int(num_kv_heads or num_heads)
+    need(H > 0 and HD % H == 0, f"{HD} columns do not divide into {H} heads")
+    need(Hkv > 0 and H % Hkv == 0,
+         f"{H} heads cannot share {Hkv} key heads")
+    D = HD // H
+    need(k.shape[0] == B and k.shape[2] == Hkv * D and v.shape == k.shape,
+         f"key and value must be ({B}, tokens, {Hkv * D}), got "
+         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    need(q.dtype == k.dtype == v.dtype and q.device == k.device == v.device,
+         "query, key and value must agree in type and device")
+    cap = 0.0
+    if logit_cap is not None:
+        cap = float(logit_cap)
+        need(0.0 < cap < float("inf"), "logit_cap must be positive")
+    if slopes is not None:
+        need(isinstance(slopes, torch.Tensor)
+             and slopes.dtype.is_floating_point
+             and tuple(slopes.shape) == (H,) and slopes.device == q.device,
+             f"distance_slopes must be {H} floats on the queries' device")
+        need(not slopes.requires_grad,
+             "distance_slopes are constants, they get no gradient")
+        slopes = slopes.float().contiguous()
+    if seg_q is None:
+        need(seg_k is None, "kv_segment_ids without segment_ids")
+    elif seg_k is None:
+        need(Tq == Tk, "segment_ids of other tokens than the keys': "
+                       "kv_segment_ids is needed too")
+        seg_k = seg_q
+    same = seg_k is seg_q
+    seg_q = _attn_ints(seg_q, (B, Tq), "segment_ids", q)
+    seg_k = seg_q if same else _attn_ints(seg_k, (B, Tk), "kv_segment_ids",
+                                          q)
+    need(prefix is None or causal, "prefix_length opens a causal mask; "
+                                   "without causal=True it has no meaning")
+    prefix = _attn_ints(prefix, (B,), "prefix_length", q)
+    kv_len = _attn_ints(kv_len, (B,), "kv_length", q)
+    off0 = 0
+    if q_off is not None and not isinstance(q_off, torch.Tensor):
+        off0, q_off = int(q_off), None
+        need(abs(off0) < 1 << 30, "query_offset is out of range")
+    q_off = _attn_ints(q_off, (B,), "query_offset", q)
+    args = (H, Hkv, float(scale if scale is not None else D ** -0.5), cap,
+            bool(causal), slopes, seg_q, seg_k, prefix, kv_len, q_off, off0)
+    if _use_hip(q, "shaped_mha", _BF16):
+        need(D % 8 == 0 and D <= 128, f"heads of {D} columns: the kernels "
+                                      "take multiples of 8 up to 128")
+        return gpu_impl("shaped_mha")(q, k, v, *args)
+    return _shaped_mha_oracle(q, k, v, *args)
+
+
+def _shaped_mha_oracle(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
+                       seg_k, prefix, kv_len, q_off, off0):
+    B, Tq, HD = q.shape
+    Tk, D, G = k.shape[1], HD // H, H // Hkv
+    ct = torch.float64 if q.dtype == torch.float64 else torch.float32
+    dev = q.device
+    j = torch.arange(Tk, device=dev)
+    pos = torch.arange(Tq, device=dev)[None, :] + off0
+    if q_off is not None:
+        pos = pos + q_off[:, None].long()
+    dist = pos[:, :, None] - j                       # [B or 1, Tq, Tk]
+    ok = torch.ones((B, Tq, Tk), dtype=torch.bool, device=dev)
+    live = torch.ones((B, Tk), dtype=torch.bool, device=dev)
+    if causal:
+        see = dist >= 0
+        if prefix is not None:
+            see = see | (j < prefix[:, None].long())[:, None, :]
+        ok = ok & see
+    if kv_len is not None:
+        live = j < kv_len[:, None].long()
+    if seg_q is not None:
+        ok = ok & (seg_q[:, :, None] == seg_k[:, None, :])
+        live = live & (seg_k >= 0)
+    ok = ok & live[:, None, :]
+    # keys and values that no query can see may hold anything
+    gone = ~live.reshape(B, Tk, 1)
+    k = k.masked_fill(gone, 0.0)
+    v = v.masked_fill(gone, 0.0)
+    if seg_q is not None:
+        q = q.masked_fill((seg_q < 0)[:, :, None], 0.0)
+    qh = q.reshape(B, Tq, Hkv, G, D).permute(0, 2, 3, 1, 4).to(ct)
+    kh = k.reshape(B, Tk, Hkv, 1, D).permute(0, 2, 3, 1, 4).to(ct)
+    vh = v.reshape(B, Tk, Hkv, 1, D).permute(0, 2, 3, 1, 4).to(ct)
+    s = torch.matmul(qh, kh.transpose(-1, -2)) * scale
+    if cap:
+        s = cap * torch.tanh(s / cap)
+    if slopes is not None:
+        s = s - slopes.to(ct).reshape(1, Hkv, G, 1, 1) \
+            * dist.abs()[:, None, None]
+    s = s.masked_fill(~ok[:, None, None], float("-inf"))
+    some = ok.any(-1)[:, None, None, :, None]
+    p = F.softmax(s.masked_fill(~some, 0.0), dim=-1).masked_fill(~some, 0.0)
+    out = torch.matmul(p, vh)
+    return out.permute(0, 3, 1, 2, 4).reshape(B, Tq, HD).to(q.dtype)
+
+
 @register("multi_head_attention")
 def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
-                         causal=False, softmax_scale=None):
+                         causal=False, softmax_scale=None, num_kv_heads=None,
+                         logit_cap=None, distance_slopes=None,
+                         segment_ids=None, kv_segment_ids=None,
+                         prefix_length=None, kv_length=None,
+                         query_offset=None):
     """Fused MHA.  q/k/v: (B, T, H*D).  GPU: flash-style CDNA4 kernel.
 
     Reference parity: the _contrib_interleaved_matmul_selfatt_* pair
     (src/operator/contrib/transformer.cu) composed into one op.
-    """
+
+    Shaped scores (any of the arguments after softmax_scale; kernels in
+    attn_mod_*.hip, head sizes that are multiples of 8 up to 128).  With
+    P = query_offset + i the position of query i:
+
+    num_kv_heads    heads of k and v, (B, Tk, num_kv_heads*D); each is shared
+                    by num_heads / num_kv_heads consecutive query heads
+    logit_cap       s -> cap * tanh(s / cap), on the scaled scores
+    distance_slopes (H,) floats: s -> s - slope_h * |P - j|, after the cap
+    segment_ids     (B, Tq) integers: a query sees the keys with its own id;
+                    negative ids are padding that sees and shows nothing
+    kv_segment_ids  (B, Tk), the keys' ids; segment_ids if not given
+    prefix_length   (B,) integers: with causal, keys below it are seen by all
+    kv_length       (B,) integers: keys from there on (a cache's unwritten
+                    part) are not seen and may hold anything
+    query_offset    integer or (B,) integers, 0 if not given: the position
+                    of the first query among the keys, kv_length - Tq for
+                    new tokens at the end of a cache
+
+    A query that sees no key gives a row of zeros and no gradient.  Few
+    queries outside autograd.record() take the form that splits the keys
+    over the chip.  Positions count exactly up to 2**24.  These forms take
+    neither a dense mask nor dropout."""
+    shaped = any(x is not None for x in (
+        logit_cap, distance_slopes, segment_ids, kv_segment_ids,
+        prefix_length, kv_length, query_offset)) or (
+        num_kv_heads is not None and int(num_kv_heads) != int(num_heads))
+    if shaped:
+        from ..base import MXNetError
+        if mask is not None:
+            raise MXNetError("multi_head_attention: a dense mask cannot be "
+                             "combined with shaped scores")
+        if dropout_p > 0 and _ag.is_training():
+            raise MXNetError("multi_head_attention: dropout cannot be "
+                             "combined with shaped scores")
+        return _shaped_mha(q, k, v, num_heads, num_kv_heads, softmax_scale,
+                           logit_cap, distance_slopes, causal, segment_ids,
+                           kv_segment_ids, prefix_length, kv_length,
+                           query_offset)
     B, Tq, HD = q.shape
     D = HD // num_heads
     scale = softmax_scale if softmax_scale is not None else D ** -0.5

@@ -11,7 +11,8 @@
 #include <unordered_map>
 #include <vector>
 
-#include "kernels/common.h"  // bf16 typedef, ZMap batch map
+#include "kernels/attn_mod.h"  // AttnArgs
+#include "kernels/common.h"    // bf16 typedef, ZMap batch map
 
 namespace mxa {
 // gemm_tn.hip
@@ -124,6 +125,13 @@ void attn_scores_bf16(const bf16*, const bf16*, bf16*, int, int, int, int,
                       int, const bf16*, hipStream_t);
 void attn_wg_bf16(const bf16*, const bf16*, bf16*, int, int, int, int,
                   int, const bf16*, hipStream_t);
+// attn_mod_{fwd,bwd,decode}.hip
+void attn_seg_ranges(const int*, int2*, int, int, hipStream_t);
+void attn_mod_fwd(const AttnArgs&, hipStream_t);
+void attn_mod_bwd(const AttnArgs&, bool, hipStream_t);
+int attn_decode_splits(int, int, int, int);
+long attn_decode_ws(int, int, int, int, int);
+void attn_decode(const AttnArgs&, hipStream_t);
 // flash.hip
 void flash_fwd_bf16(const bf16*, const bf16*, const bf16*, bf16*, float*,
                     float*, int, int, int, int, int, float, bool,
@@ -1083,6 +1091,209 @@ std::vector<at::Tensor> flash_bwd(const at::Tensor& q,
   return {dqacc.to(at::kBFloat16), dk, dv};
 }
 
+// ---- attention with shaped scores (attn_mod.h) ----
+using OptT = c10::optional<at::Tensor>;
+
+namespace {
+const int* attn_index(const OptT& t, const at::Tensor& like, long n,
+                      const char* what) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous() &&
+                  t->numel() == n && t->device() == like.device(),
+              "attention: ", what, " must be ", n,
+              " contiguous int32 values on the queries' device");
+  return t->data_ptr<int>();
+}
+
+void attn_operand(const at::Tensor& t, const at::Tensor& like,
+                  const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 3 &&
+                  t.device() == like.device() && t.is_cuda(),
+              "attention: ", what, " must be a 3-d bfloat16 GPU tensor");
+  // rows are read 16 bytes at a time
+  TORCH_CHECK((t.size(2) == 1 || t.stride(2) == 1) && t.stride(1) % 8 == 0 &&
+                  t.stride(0) % 8 == 0 && (size_t)t.data_ptr() % 16 == 0,
+              "attention: ", what, " must have contiguous, aligned rows");
+}
+
+mxa::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k,
+                        const at::Tensor& v, long H, long Hkv, double scale,
+                        double cap, bool causal, const OptT& slopes,
+                        const OptT& seg_q, const OptT& seg_k,
+                        const OptT& prefix, const OptT& kv_len,
+                        const OptT& q_off, long off0) {
+  attn_operand(q, q, "query");
+  attn_operand(k, q, "key");
+  attn_operand(v, q, "value");
+  mxa::AttnArgs a = {};
+  a.B = q.size(0);
+  a.Tq = q.size(1);
+  a.Tk = k.size(1);
+  a.H = H;
+  a.Hkv = Hkv;
+  TORCH_CHECK(H > 0 && Hkv > 0 && H % Hkv == 0 && q.size(2) % H == 0,
+              "attention: heads do not divide");
+  a.G = H / Hkv;
+  a.D = q.size(2) / H;
+  TORCH_CHECK(a.D % 8 == 0 && a.D > 0 && a.D <= 128,
+              "attention: head size must be a multiple of 8, at most 128");
+  TORCH_CHECK(k.size(0) == a.B && k.size(2) == Hkv * a.D &&
+                  v.sizes() == k.sizes(),
+              "attention: key and value must be [batch, keys, kv_heads * ",
+              a.D, "]");
+  TORCH_CHECK(q.size(1) < (1L << 30) && k.size(1) < (1L << 30) &&
+                  a.B * H * ((a.Tq + 127) / 128 + 1) < (1L << 30) &&
+                  (long)a.B * Hkv * ((a.Tk + 127) / 128 + 1) < (1L << 30),
+              "attention: too large");
+  a.TqP = (a.Tq + 63) / 64 * 64;
+  a.q = bfp(q);
+  a.k = bfp(k);
+  a.v = bfp(v);
+  a.qsb = q.stride(0);
+  a.qst = q.stride(1);
+  a.ksb = k.stride(0);
+  a.kst = k.stride(1);
+  a.vsb = v.stride(0);
+  a.vst = v.stride(1);
+  a.scale = (float)scale;
+  a.cap = (float)cap;
+  a.causal = causal;
+  if (slopes.has_value()) {
+    TORCH_CHECK(slopes->scalar_type() == at::kFloat &&
+                    slopes->is_contiguous() && slopes->numel() == H &&
+                    slopes->device() == q.device(),
+                "attention: slopes must be one float32 a head");
+    a.slopes = slopes->data_ptr<float>();
+  }
+  a.seg_q = attn_index(seg_q, q, (long)a.B * a.Tq, "segment_ids");
+  a.seg_k = attn_index(seg_k, q, (long)a.B * a.Tk, "kv_segment_ids");
+  TORCH_CHECK((a.seg_q == nullptr) == (a.seg_k == nullptr),
+              "attention: segment ids of one side are missing");
+  a.prefix = attn_index(prefix, q, a.B, "prefix_length");
+  a.kv_len = attn_index(kv_len, q, a.B, "kv_length");
+  a.q_off = attn_index(q_off, q, a.B, "query_offset");
+  a.off0 = (int)off0;
+  return a;
+}
+
+at::Tensor attn_ranges(const int* seg, long B, long T,
+                       const at::Tensor& like) {
+  auto r = at::empty({B, (T + 63) / 64, 2}, like.options().dtype(at::kInt));
+  mxa::attn_seg_ranges(seg, (int2*)r.data_ptr<int>(), (int)B, (int)T,
+                       cur_stream());
+  return r;
+}
+}  // namespace
+
+// Returns the output, and where with_stats is set the log2 sums and (with
+// ids) the id ranges of the query and key tiles, which the backward reuses.
+std::vector<at::Tensor> attn_mod_fwd(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, long H,
+    long Hkv, double scale, double cap, bool causal, const OptT& slopes,
+    const OptT& seg_q, const OptT& seg_k, const OptT& prefix,
+    const OptT& kv_len, const OptT& q_off, long off0, bool with_stats) {
+  c10::DeviceGuard guard(q.device());
+  auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
+                     seg_k, prefix, kv_len, q_off, off0);
+  TORCH_CHECK(a.B > 0 && a.Tq > 0 && a.Tk > 0, "attention: empty");
+  auto out = at::empty({a.B, a.Tq, q.size(2)}, q.options());
+  a.o = bfp_mut(out);
+  a.osb = out.stride(0);
+  a.ost = out.stride(1);
+  std::vector<at::Tensor> res = {out};
+  at::Tensor rq, rk;
+  if (a.seg_q) {
+    rk = attn_ranges(a.seg_k, a.B, a.Tk, q);
+    a.rng_k = (const int2*)rk.data_ptr<int>();
+    if (with_stats)
+      rq = a.seg_q == a.seg_k && a.Tq == a.Tk
+               ? rk
+               : attn_ranges(a.seg_q, a.B, a.Tq, q);
+  }
+  if (with_stats) {
+    auto lse = at::empty({a.B, H, a.TqP}, q.options().dtype(at::kFloat));
+    a.lse = lse.data_ptr<float>();
+    res.push_back(lse);
+    if (a.seg_q) {
+      res.push_back(rq);
+      res.push_back(rk);
+    }
+  }
+  mxa::attn_mod_fwd(a, cur_stream());
+  return res;
+}
+
+std::vector<at::Tensor> attn_mod_bwd(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& out, const at::Tensor& dout, const at::Tensor& lse,
+    const OptT& rng_q, const OptT& rng_k, long H, long Hkv, double scale,
+    double cap, bool causal, const OptT& slopes, const OptT& seg_q,
+    const OptT& seg_k, const OptT& prefix, const OptT& kv_len,
+    const OptT& q_off, long off0, bool need_kv) {
+  c10::DeviceGuard guard(q.device());
+  auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
+                     seg_k, prefix, kv_len, q_off, off0);
+  attn_operand(out, q, "output");
+  attn_operand(dout, q, "output gradient");
+  TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes() &&
+                  lse.numel() == (long)a.B * H * a.TqP &&
+                  (a.seg_q == nullptr) == !rng_q.has_value() &&
+                  rng_q.has_value() == rng_k.has_value(),
+              "attention: backward does not match its forward");
+  a.o = const_cast<bf16*>(bfp(out));
+  a.osb = out.stride(0);
+  a.ost = out.stride(1);
+  a.dout = bfp(dout);
+  a.gsb = dout.stride(0);
+  a.gst = dout.stride(1);
+  a.lse = lse.data_ptr<float>();
+  auto delta = at::empty_like(lse);
+  a.delta = delta.data_ptr<float>();
+  if (a.seg_q) {
+    a.rng_q = (const int2*)rng_q->data_ptr<int>();
+    a.rng_k = (const int2*)rng_k->data_ptr<int>();
+  }
+  auto dq = at::empty({a.B, a.Tq, q.size(2)}, q.options());
+  a.dq = bfp_mut(dq);
+  std::vector<at::Tensor> res = {dq};
+  if (need_kv) {
+    auto dk = at::empty({a.B, a.Tk, k.size(2)}, q.options());
+    auto dv = at::empty({a.B, a.Tk, k.size(2)}, q.options());
+    a.dk = bfp_mut(dk);
+    a.dv = bfp_mut(dv);
+    res.push_back(dk);
+    res.push_back(dv);
+  }
+  mxa::attn_mod_bwd(a, need_kv, cur_stream());
+  return res;
+}
+
+at::Tensor attn_decode(const at::Tensor& q, const at::Tensor& k,
+                       const at::Tensor& v, long H, long Hkv, double scale,
+                       double cap, bool causal, const OptT& slopes,
+                       const OptT& prefix, const OptT& kv_len,
+                       const OptT& q_off, long off0) {
+  c10::DeviceGuard guard(q.device());
+  auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, {}, {},
+                     prefix, kv_len, q_off, off0);
+  TORCH_CHECK(a.B > 0 && a.Tq > 0 && a.Tk > 0, "attention: empty");
+  auto out = at::empty({a.B, a.Tq, q.size(2)}, q.options());
+  a.o = bfp_mut(out);
+  a.osb = out.stride(0);
+  a.ost = out.stride(1);
+  const int R = a.Tq * a.G;
+  a.nsplit = mxa::attn_decode_splits(a.B, a.Hkv, R, a.Tk);
+  TORCH_CHECK((long)a.B * a.Hkv * ((R + 31) / 32) * a.nsplit < (1L << 31),
+              "attention: too large");
+  at::Tensor ws;
+  if (long n = mxa::attn_decode_ws(a.B, a.Hkv, R, a.D, a.nsplit)) {
+    ws = at::empty({n}, q.options().dtype(at::kFloat));
+    a.ws = ws.data_ptr<float>();
+  }
+  mxa::attn_decode(a, cur_stream());
+  return out;
+}
+
 at::Tensor attn_wg(const at::Tensor& p, const at::Tensor& q, long H) {
   // dK[b,tk,h*D+d] = sum_tq dS[b*H+h][tq][tk] q[b,tq,h*D+d] (WG form,
   // f32 out in [B,S,H*D] layout).  Also dV with (P, dO).
@@ -1644,6 +1855,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_scores", &attn_scores);
   m.def("attn_ctx", &attn_ctx);
   m.def("attn_wg", &attn_wg);
+  m.def("attn_mod_fwd", &attn_mod_fwd);
+  m.def("attn_mod_bwd", &attn_mod_bwd);
+  m.def("attn_decode", &attn_decode);
   m.def("flash_fwd", &flash_fwd);
   m.def("flash_bwd", &flash_bwd);
   m.def("dropout_fwd", &dropout_fwd);

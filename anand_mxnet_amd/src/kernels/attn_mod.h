@@ -1,0 +1,373 @@
+// Attention with shaped scores: what the forward, backward and few-token
+// kernels share (attn_mod_fwd.hip, attn_mod_bwd.hip, attn_mod_decode.hip).
+//
+// For a query i at position P = query_offset + i and a key j of one sequence
+//   s = scale * q.k
+//   s = cap * tanh(s / cap)              (CAP)
+//   s = s - slope_h * |P - j|            (BIAS)
+// and j is visible to i when all of these hold
+//   j < kv_length
+//   j <= P or j < prefix_length          (causal)
+//   seg_q[i] == seg_k[j] >= 0            (documents)
+// A query that sees nothing gives a zero row and zero gradients.
+//
+// Scores are held in units of log2 (x = s * log2 e), so that the softmax
+// needs exp2 alone.  tanh(y) = 1 - 2 / (1 + exp(2 y)) costs one exp2 and one
+// reciprocal and saturates by itself: exp2 -> inf gives 1, exp2 -> 0 gives
+// -1.  Its error is about 1e-7 of the cap, 1e-5 in a probability at most.
+//
+// Matrix operands (v_mfma_f32_32x32x16_bf16, wave of 64 lanes, l = lane):
+//   A row  l & 31,  k = 8 (l >> 5) + 0..7
+//   B col  l & 31,  k = 8 (l >> 5) + 0..7
+//   C col  l & 31,  row 8 (i >> 2) + 4 (l >> 5) + (i & 3), i = 0..15
+// Products are arranged so that the softmaxed axis lies along the rows of C:
+// then C of the first product, rounded to bf16, IS the B operand of the next
+// one (eight consecutive i are the k of one step, in the order 0-3, 8-11 for
+// the lower and 4-7, 12-15 for the upper half of the wave), and the A operand
+// is fetched in the same order by transposing LDS reads of four rows each.
+// Probabilities never leave the registers.
+#pragma once
+#include "common.h"
+
+namespace mxa {
+
+struct AttnArgs {
+  const bf16 *q, *k, *v;
+  bf16* o;
+  float* lse;  // [B, H, TqP] log2 of the softmax sum; +inf: row sees nothing
+  const bf16* dout;
+  float* delta;  // [B, H, TqP] sum_d dout * out
+  bf16 *dq, *dk, *dv;
+  float* ws;     // partial results of a split launch
+  long qsb, ksb, vsb, osb, gsb;  // batch strides, elements
+  long qst, kst, vst, ost, gst;  // row strides, elements (g: dout)
+  int B, H, Hkv, G, D, Tq, Tk, TqP;
+  float scale, cap;
+  int causal;
+  const int *seg_q, *seg_k, *prefix, *kv_len, *q_off;
+  const float* slopes;
+  int off0;  // added to every query_offset
+  const int2 *rng_q, *rng_k;  // smallest and largest id of each 64 rows
+  int nsplit;
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float M_INIT = -1.0e30f;  // running maximum before any score
+#define MXA_INF __builtin_inff()
+
+// Sixteen zero bytes that staging lanes read where a row or a chunk is out
+// of range: V rows behind a sequence must be zero (0 * NaN is NaN).
+static __device__ const uint4 attn_zero16[1] = {{0, 0, 0, 0}};
+
+DEVINL float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
+DEVINL float frcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// LDS image of [rows][D] bf16, D = 64 or 128, in chunks of 16 bytes; chunk c
+// of row r lies in slot c ^ attn_key(r).  The key is a bijection of 16 rows
+// (row fragments: 16 lanes, one chunk) and gives four aligned rows times
+// four aligned chunks 16 different slots (transposing reads), so both kinds
+// of read are free of bank conflicts.
+template <int D>
+DEVINL int attn_key(int r) {
+  return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3))
+                  : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
+}
+
+template <int D>
+DEVINL bf16x8 attn_row_frag(const bf16* img, int row, int chunk) {
+  return *(const bf16x8*)&img[row * D + ((chunk ^ attn_key<D>(row)) << 3)];
+}
+
+// A operand of img^T: rows of A are columns col0..col0+31 of the image, k
+// runs over image rows row0 + {0-3, 8-11} (lower half) or {4-7, 12-15}.
+template <int D>
+DEVINL bf16x8 attn_tr_frag(const bf16* img, int row0, int col0, int lane) {
+  int c = col0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  int r = row0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+  typedef __attribute__((address_space(3))) bf16x4 lds4;
+  auto at = [&](int row) {
+    return (lds4*)((__attribute__((address_space(3))) bf16*)img + row * D +
+                   (((c >> 3) ^ attn_key<D>(row)) << 3) + (c & 7));
+  };
+  bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at(r));
+  bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at(r + 8));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A direct copy into LDS: 16 bytes (or 4) a lane, from the lane's address to
+// dst + 16 (4) * lane.  Written as assembly because the compiler waits for
+// every copy in flight before any LDS read that follows a builtin one, which
+// would undo the double buffering; it names no register that a load fills.
+// Whoever reads the tile waits with attn_wait_copies and a barrier.
+DEVINL void copy_lds16(const void* g, unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+      :
+      : "v"(g), "s"(dst)
+      : "memory");
+}
+DEVINL void copy_lds4(const void* g, unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+      :
+      : "v"(g), "s"(dst)
+      : "memory");
+}
+// All but the last N copies have landed.
+template <int N>
+DEVINL void attn_wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+// Makes the compiler wait for x here, and not inside a later loop, where the
+// wait would catch the copies in flight too.
+DEVINL void attn_settle(bf16x8& x) { asm volatile("" : "+v"(x)); }
+
+DEVINL unsigned lds_addr(const void* p) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(
+      (const __attribute__((address_space(3))) char*)p));
+}
+
+// Copies NROW consecutive rows of a head (row0 on) into an image, by NW
+// waves.  Rows at or behind row_end, rows whose id in seg is negative (seg
+// may be null) and chunks at or behind Dact read as zero.
+template <int D, int NROW, int NW>
+DEVINL void attn_stage(const bf16* base, long stride, int row0, int row_end,
+                       int Dact, const int* seg, const bf16* img, int wave,
+                       int lane) {
+  constexpr int RPI = 512 / D;  // rows of one instruction
+  constexpr int CPR = D / 8;    // chunks of a row
+  constexpr int N = NROW / RPI / NW;
+  static_assert(N * RPI * NW == NROW, "rows divide among the waves");
+  const unsigned dst = lds_addr(img) + wave * (N * 1024);
+  const bool clean = row0 + NROW <= row_end && Dact == D && seg == nullptr;
+  const int r0 = wave * N * RPI + lane / CPR;
+  if (clean) {
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+      int r = r0 + p * RPI;
+      int ch = (lane % CPR) ^ attn_key<D>(r);
+      copy_lds16(base + (long)(row0 + r) * stride + ch * 8, dst + p * 1024);
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+      int r = r0 + p * RPI;
+      int ch = (lane % CPR) ^ attn_key<D>(r);
+      const bf16* g = base + (long)(row0 + r) * stride + ch * 8;
+      bool ok = row0 + r < row_end && ch * 8 < Dact;
+      if (ok && seg) ok = seg[row0 + r] >= 0;
+      if (!ok) g = (const bf16*)attn_zero16;
+      copy_lds16(g, dst + p * 1024);
+    }
+  }
+}
+
+// 64 words into LDS, one instruction of one wave; index clamped to [0, n).
+DEVINL void attn_stage64(const void* base, int first, int n, const void* dst,
+                         int lane) {
+  int j = min(first + lane, n - 1);
+  copy_lds4((const unsigned int*)base + j, lds_addr(dst));
+}
+
+DEVINL bf16x8 attn_load_row(const bf16* p, int chunk, int Dact, bool ok) {
+  bf16x8 z = {};
+  return ok && chunk * 8 < Dact ? *(const bf16x8*)(p + chunk * 8) : z;
+}
+
+DEVINL int wave_min(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+DEVINL int wave_max(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// Positions and document ids that a group of queries spans.
+struct RowSpan {
+  int pmin, pmax, smin, smax;
+};
+
+// One sequence's masks, uniform over a block.
+struct SeqMask {
+  int kv_len, prefix, off, causal, has_seg;
+};
+
+DEVINL SeqMask attn_seq_mask(const AttnArgs& a, int b) {
+  SeqMask m;
+  m.kv_len = a.kv_len ? min(max(a.kv_len[b], 0), a.Tk) : a.Tk;
+  m.prefix = a.prefix ? a.prefix[b] : 0;
+  m.off = a.off0 + (a.q_off ? a.q_off[b] : 0);
+  m.causal = a.causal;
+  m.has_seg = a.seg_q != nullptr;
+  return m;
+}
+
+// First key that a query at position p cannot see (documents aside).
+DEVINL int attn_limit(const SeqMask& m, int p) {
+  return m.causal ? min(m.kv_len, max(p + 1, m.prefix)) : m.kv_len;
+}
+
+// May any query of s see any key of the 64 from j0 on?
+DEVINL bool attn_tile_any(const SeqMask& m, const RowSpan& s, int j0,
+                          int2 r) {
+  bool ok = j0 < attn_limit(m, s.pmax);
+  if (m.has_seg) ok = ok && max(max(s.smin, r.x), 0) <= min(s.smax, r.y);
+  return ok;
+}
+
+// Does every query of s see every one of them?
+DEVINL bool attn_tile_all(const SeqMask& m, const RowSpan& s, int j0,
+                          int2 r) {
+  bool ok = j0 + 64 <= attn_limit(m, s.pmin);
+  if (m.has_seg)
+    ok = ok && s.smin >= 0 && s.smin == s.smax && r.x == s.smin &&
+         r.y == s.smin;
+  return ok;
+}
+
+struct Tile {
+  int t;      // index of 64 keys; negative: no more
+  bool work;  // this wave has pairs in it
+  bool full;  // all its pairs are visible
+  bool neg;   // some ids are negative: stage with care
+};
+
+// Walks the key tiles a block has work in: 64 tiles are judged at once, a
+// tile to a lane, and the verdicts are kept as bits.
+struct TileWalk {
+  int base, nt;
+  u64 act, wact, wful, neg;
+
+  DEVINL void start(int first, int ntiles) {
+    base = first - 64;
+    nt = ntiles;
+    act = wact = wful = neg = 0;
+  }
+  DEVINL Tile next(const SeqMask& m, const RowSpan& blk, const RowSpan& wav,
+                   const int2* rng, int lane) {
+    while (act == 0) {
+      base += 64;
+      if (base >= nt) return Tile{-1, false, false, false};
+      int t = base + lane;
+      int2 r = make_int2(0, 0);
+      bool in = t < nt;
+      if (in && m.has_seg) r = rng[t];
+      act = __ballot(in && attn_tile_any(m, blk, t * 64, r));
+      wact = __ballot(in && attn_tile_any(m, wav, t * 64, r));
+      wful = __ballot(in && attn_tile_all(m, wav, t * 64, r));
+      neg = __ballot(in && m.has_seg && r.x < 0);
+    }
+    int i = __builtin_ctzll(act);
+    act &= act - 1;
+    return Tile{base + i, (bool)((wact >> i) & 1), (bool)((wful >> i) & 1),
+                (bool)((neg >> i) & 1)};
+  }
+};
+
+// The spans of a wave's 32 queries (q0 on) and of its block of 128.
+DEVINL void attn_spans(const SeqMask& m, int q0, int Tq, bool qok, int sq,
+                       int4* shared, int wave, int lane, RowSpan& wav,
+                       RowSpan& blk) {
+  wav.pmin = q0 + m.off;
+  wav.pmax = min(q0 + 31, Tq - 1) + m.off;
+  wav.smin = wave_min(qok ? sq : 0x7fffffff);
+  wav.smax = wave_max(qok ? sq : -0x7fffffff - 1);
+  if (q0 >= Tq) {  // a wave without rows sees no tile
+    wav.pmin = wav.pmax = -0x7fffffff;
+    wav.smin = 0x7fffffff;
+    wav.smax = -0x7fffffff - 1;
+  }
+  if (lane == 0)
+    shared[wave] = make_int4(wav.pmin, wav.pmax, wav.smin, wav.smax);
+  __syncthreads();
+  blk = {q0 - wave * 32 + m.off, wav.pmax, wav.smin, wav.smax};
+  for (int w = 0; w < 4; ++w) {
+    int4 s = shared[w];
+    blk.pmax = max(blk.pmax, __builtin_amdgcn_readfirstlane(s.y));
+    blk.smin = min(blk.smin, __builtin_amdgcn_readfirstlane(s.z));
+    blk.smax = max(blk.smax, __builtin_amdgcn_readfirstlane(s.w));
+  }
+}
+
+// Masks 16 scores of one query (C order): ids at ksg, first `lim` keys seen.
+DEVINL void attn_mask_keys(float* x, int has_seg, const int* ksg, int sq,
+                           int lim) {
+  if (has_seg) {
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) {
+      const int4 k4 = *(const int4*)(ksg + 8 * ii);
+      x[ii * 4 + 0] = k4.x == sq ? x[ii * 4 + 0] : -MXA_INF;
+      x[ii * 4 + 1] = k4.y == sq ? x[ii * 4 + 1] : -MXA_INF;
+      x[ii * 4 + 2] = k4.z == sq ? x[ii * 4 + 2] : -MXA_INF;
+      x[ii * 4 + 3] = k4.w == sq ? x[ii * 4 + 3] : -MXA_INF;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    x[i] = 8 * (i >> 2) + (i & 3) < lim ? x[i] : -MXA_INF;
+}
+
+// Constants of the score function, in units of log2.
+struct ScoreFn {
+  float c1, A, slope;
+  template <bool CAP>
+  DEVINL void set(float scale, float cap, float slope_) {
+    if (CAP) {
+      c1 = scale / cap * 2.f * LOG2E;
+      A = cap * LOG2E;
+    } else {
+      c1 = scale * LOG2E;
+      A = 0.f;
+    }
+    slope = -slope_ * LOG2E;
+  }
+};
+
+// x of one raw product; u is 4 r (1 - r) = 1 - tanh^2 where CAP.
+template <bool CAP>
+DEVINL float attn_score(const ScoreFn& f, float s, float* u = nullptr) {
+  if (!CAP) return s * f.c1;
+  float r = frcp(1.f + fexp2(s * f.c1));
+  if (u) *u = 4.f * (r - r * r);
+  return f.A - (2.f * f.A) * r;
+}
+
+DEVINL bf16x8 pack8(const float* x) {
+  bf16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (bf16)x[i];
+  return y;
+}
+
+DEVINL f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+DEVINL f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Writes one row of a transposed accumulator: d = 8 ii + 4 half + 0..3 of
+// each 32.
+template <int DB>
+DEVINL void attn_store_t(bf16* p, const f32x16* acc, float mul, int Dact,
+                         int half) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) {
+      const int d = db * 32 + 8 * ii + 4 * half;
+      bf16x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = (bf16)(acc[db][ii * 4 + i] * mul);
+      if (d < Dact) *(bf16x4*)(p + d) = y;
+    }
+}
+
+}  // namespace mxa

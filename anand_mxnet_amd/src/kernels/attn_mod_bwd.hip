@@ -1,0 +1,414 @@
+// Backward pass of attention with shaped scores (see attn_mod.h).
+//
+// With t = tanh(s / cap), P the probabilities and dP = dO V^T:
+//   dS = scale * P * (dP - delta) * (1 - t^2),  delta_i = sum_d dO_i O_i
+//   dV = P^T dO,   dK = dS^T Q,   dQ = dS K
+// Two kernels, each of which recomputes the scores: one walks the keys for
+// 128 queries and keeps dQ in registers, the other walks the queries for 128
+// keys and keeps dK and dV.  That is 7 matrix products where one kernel would
+// need 5, but nothing is added through memory: no fp32 copy of dQ, no
+// atomics, and the same bits in every run.
+#include "attn_mod.h"
+
+namespace mxa {
+
+// ---------------------------------------------------------------------------
+// dQ (and delta): block = 128 queries of one head, wave = 32 queries along
+// the lanes, as in the forward pass.
+// ---------------------------------------------------------------------------
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
+  constexpr int KK = D / 16, DB = D / 32;
+  __shared__ __align__(16) bf16 kimg[2][64 * D];
+  __shared__ __align__(16) bf16 vimg[2][64 * D];
+  __shared__ __align__(16) int ksg[2][64];
+  __shared__ int4 spans[4];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int nqb = cdiv(a.Tq, 128);
+  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int qb = nqb - 1 - id % nqb;
+  const int h = (id / nqb) % a.H, b = id / nqb / a.H;
+  const int hk = h / a.G;
+  const SeqMask m = attn_seq_mask(a, b);
+
+  const int q0 = qb * 128 + wave * 32;
+  const int qi = q0 + col;
+  const bool qok = qi < a.Tq;
+  const int pos = qi + m.off;
+  int sq = 0;
+  if (m.has_seg) sq = qok ? a.seg_q[(long)b * a.Tq + qi] : -1;
+
+  RowSpan wav, blk;
+  attn_spans(m, q0, a.Tq, qok, sq, spans, wave, lane, wav, blk);
+  const int limit = m.has_seg && sq < 0 ? 0 : attn_limit(m, pos);
+  ScoreFn f;
+  f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
+
+  // queries, their output gradients and delta
+  bf16x8 qf[KK], gf[KK];
+  float lse = MXA_INF, delta = 0.f;
+  {
+    const bool ok = qok && sq >= 0;
+    const long row = ((long)b * a.H + h) * a.TqP + qi;
+    const bf16* qp = a.q + b * a.qsb + (long)qi * a.qst + (long)h * a.D;
+    const bf16* gp = a.dout + b * a.gsb + (long)qi * a.gst + (long)h * a.D;
+    const bf16* op = a.o + b * a.osb + (long)qi * a.ost + (long)h * a.D;
+    if (ok) lse = a.lse[row];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[kk] = attn_load_row(qp, kk * 2 + half, a.D, ok);
+      gf[kk] = attn_load_row(gp, kk * 2 + half, a.D, ok);
+      bf16x8 of = attn_load_row(op, kk * 2 + half, a.D, ok);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        delta = fmaf((float)gf[kk][i], (float)of[i], delta);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (half == 0 && qi < a.TqP) a.delta[row] = delta;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      attn_settle(qf[kk]);
+      attn_settle(gf[kk]);
+    }
+    asm volatile("" : "+v"(lse));
+  }
+
+  const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
+  const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
+  const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
+  const int2* rng = m.has_seg ? a.rng_k + (long)b * cdiv(a.Tk, 64) : nullptr;
+
+  auto stage = [&](int buf, const Tile& t) {
+    const int* sg = t.neg ? skb : nullptr;
+    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg, kimg[buf],
+                         wave, lane);
+    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg, vimg[buf],
+                         wave, lane);
+    if (m.has_seg && wave == 0)
+      attn_stage64(skb, t.t * 64, a.Tk, ksg[buf], lane);
+  };
+
+  f32x16 dq[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dq[db] = zero16();
+
+  TileWalk walk;
+  walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
+  Tile cur = walk.next(m, blk, wav, rng, lane);
+  if (cur.t >= 0) stage(0, cur);
+  int buf = 0;
+  while (cur.t >= 0) {
+    attn_wait_copies<0>();
+    __syncthreads();
+    Tile nxt = walk.next(m, blk, wav, rng, lane);
+    if (nxt.t >= 0) stage(buf ^ 1, nxt);
+    if (cur.work) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          s = mfma32(
+              attn_row_frag<D>(kimg[buf], nb * 32 + col, kk * 2 + half),
+              qf[kk], s);
+          dp = mfma32(
+              attn_row_frag<D>(vimg[buf], nb * 32 + col, kk * 2 + half),
+              gf[kk], dp);
+        }
+        const int j0 = cur.t * 64 + nb * 32 + 4 * half;
+        const float d0 = BIAS ? (float)(pos - j0) : 0.f;
+        float x[16], u[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int dj = 8 * (i >> 2) + (i & 3);
+          x[i] = attn_score<CAP>(f, s[i], &u[i]);
+          if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
+        }
+        if (!cur.full)
+          attn_mask_keys(x, m.has_seg, &ksg[buf][nb * 32 + 4 * half], sq,
+                         limit - j0);
+        bf16x8 df[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float ds[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            ds[i] = fexp2(x[8 * w + i] - lse) * (dp[8 * w + i] - delta);
+            if (CAP) ds[i] *= u[8 * w + i];
+          }
+          df[w] = pack8(ds);
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            dq[db] = mfma32(attn_tr_frag<D>(kimg[buf], nb * 32 + w * 16,
+                                            db * 32, lane),
+                            df[w], dq[db]);
+      }
+    }
+    cur = nxt;
+    buf ^= 1;
+  }
+
+  if (qok) {
+    bf16* op = a.dq + ((long)b * a.Tq + qi) * a.H * a.D + (long)h * a.D;
+    attn_store_t<DB>(op, dq, a.scale, a.D, half);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV: block = 128 keys of one key head, wave = 32 keys along the lanes;
+// the queries of every head that shares them pass by in tiles of 64.
+// ---------------------------------------------------------------------------
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
+    AttnArgs a) {
+  constexpr int KK = D / 16, DB = D / 32;
+  __shared__ __align__(16) bf16 qimg[2][64 * D];
+  __shared__ __align__(16) bf16 gimg[2][64 * D];
+  __shared__ __align__(16) float lses[2][64];
+  __shared__ __align__(16) float dels[2][64];
+  __shared__ __align__(16) int qsg[2][64];
+  __shared__ int2 spans[4];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int nkb = cdiv(a.Tk, 128);
+  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int kb = id % nkb;
+  const int hk = (id / nkb) % a.Hkv, b = id / nkb / a.Hkv;
+  const SeqMask m = attn_seq_mask(a, b);
+
+  const int k0 = kb * 128 + wave * 32;
+  const int kj = k0 + col;
+  int sk = 0;
+  if (m.has_seg) sk = kj < a.Tk ? a.seg_k[(long)b * a.Tk + kj] : -1;
+  const bool kok = kj < m.kv_len && sk >= 0;
+  // first position that sees this key (documents aside)
+  const int NEVER = 0x7fffffff;
+  const int first =
+      !kok ? NEVER
+           : (!m.causal || kj < m.prefix ? -0x7fffffff : kj);
+
+  // spans of the wave and the block: smallest `first`, largest, ids
+  int wlo = wave_min(first), whi = wave_max(first);
+  int slo = wave_min(sk), shi = wave_max(sk);
+  if (lane == 0) spans[wave] = make_int2(slo, shi);
+  __shared__ int firsts[4];
+  if (lane == 0) firsts[wave] = wlo;
+  __syncthreads();
+  int blo = wlo, bslo = slo, bshi = shi;
+  for (int w = 0; w < 4; ++w) {
+    blo = min(blo, __builtin_amdgcn_readfirstlane(firsts[w]));
+    bslo = min(bslo, __builtin_amdgcn_readfirstlane(spans[w].x));
+    bshi = max(bshi, __builtin_amdgcn_readfirstlane(spans[w].y));
+  }
+
+  bf16x8 kf[KK], vf[KK];
+  {
+    const bf16* kp = a.k + b * a.ksb + (long)kj * a.kst + (long)hk * a.D;
+    const bf16* vp = a.v + b * a.vsb + (long)kj * a.vst + (long)hk * a.D;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      kf[kk] = attn_load_row(kp, kk * 2 + half, a.D, kok);
+      vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      attn_settle(kf[kk]);
+      attn_settle(vf[kk]);
+    }
+  }
+
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
+
+  const int ntq = cdiv(a.Tq, 64);
+  const int2* rng = m.has_seg ? a.rng_q + (long)b * ntq : nullptr;
+  const int* sqb = m.has_seg ? a.seg_q + (long)b * a.Tq : nullptr;
+
+  // Verdict on query tile t: bit 0 block, bit 1 wave, bit 2 all pairs of the
+  // wave visible, bit 3 negative ids.
+  auto judge = [&](int t) {
+    int2 r = m.has_seg ? rng[t] : make_int2(0, 0);
+    const int p0 = t * 64 + m.off, p1 = min(t * 64 + 63, a.Tq - 1) + m.off;
+    bool any = p1 >= blo && blo != NEVER, wany = p1 >= wlo && wlo != NEVER;
+    bool all = p0 >= whi && whi != NEVER;
+    if (m.has_seg) {
+      any = any && max(max(bslo, r.x), 0) <= min(bshi, r.y);
+      wany = wany && max(max(slo, r.x), 0) <= min(shi, r.y);
+      all = all && slo == shi && r.x == slo && r.y == slo;
+    }
+    return (any ? 1 : 0) | (wany ? 2 : 0) | (all ? 4 : 0) |
+           (m.has_seg && r.x < 0 ? 8 : 0);
+  };
+
+  int cg = 0, base = -64;
+  u64 act = 0, wact = 0, wful = 0, neg = 0;
+  struct QTile {
+    int g, t;
+    bool work, full, neg;
+  };
+  auto next = [&]() -> QTile {
+    while (act == 0) {
+      base += 64;
+      if (base >= ntq) {
+        base = 0;
+        if (++cg >= a.G) return QTile{-1, 0, false, false, false};
+      }
+      int t = base + lane;
+      int v = t < ntq ? judge(t) : 0;
+      act = __ballot(v & 1);
+      wact = __ballot(v & 2);
+      wful = __ballot(v & 4);
+      neg = __ballot(v & 8);
+    }
+    int i = __builtin_ctzll(act);
+    act &= act - 1;
+    return QTile{cg, base + i, (bool)((wact >> i) & 1),
+                 (bool)((wful >> i) & 1), (bool)((neg >> i) & 1)};
+  };
+
+  auto stage = [&](int buf, const QTile& t) {
+    const int h = hk * a.G + t.g;
+    const int* sg = t.neg ? sqb : nullptr;
+    attn_stage<D, 64, 4>(a.q + b * a.qsb + (long)h * a.D, a.qst, t.t * 64,
+                         a.Tq, a.D, sg, qimg[buf], wave, lane);
+    attn_stage<D, 64, 4>(a.dout + b * a.gsb + (long)h * a.D, a.gst, t.t * 64,
+                         a.Tq, a.D, sg, gimg[buf], wave, lane);
+    const long row = ((long)b * a.H + h) * a.TqP;
+    if (wave == 0)
+      attn_stage64(a.lse + row, t.t * 64, a.TqP, lses[buf], lane);
+    if (wave == 1)
+      attn_stage64(a.delta + row, t.t * 64, a.TqP, dels[buf], lane);
+    if (wave == 2 && m.has_seg)
+      attn_stage64(sqb, t.t * 64, a.Tq, qsg[buf], lane);
+  };
+
+  ScoreFn f;
+  QTile cur = next();
+  if (cur.g >= 0) stage(0, cur);
+  int buf = 0;
+  while (cur.g >= 0) {
+    attn_wait_copies<0>();
+    __syncthreads();
+    QTile nxt = next();
+    if (nxt.g >= 0) stage(buf ^ 1, nxt);
+    if (cur.work) {
+      f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[hk * a.G + cur.g] : 0.f);
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          s = mfma32(
+              attn_row_frag<D>(qimg[buf], nb * 32 + col, kk * 2 + half),
+              kf[kk], s);
+          dp = mfma32(
+              attn_row_frag<D>(gimg[buf], nb * 32 + col, kk * 2 + half),
+              vf[kk], dp);
+        }
+        const int r0 = nb * 32 + 4 * half;  // this lane's first tile row
+        const int p0 = cur.t * 64 + r0 + m.off;
+        const float d0 = BIAS ? (float)(p0 - kj) : 0.f;
+        float x[16], u[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int dj = 8 * (i >> 2) + (i & 3);
+          x[i] = attn_score<CAP>(f, s[i], &u[i]);
+          if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 + (float)dj), x[i]);
+        }
+        if (!cur.full) {
+          if (m.has_seg) {
+#pragma unroll
+            for (int ii = 0; ii < 4; ++ii) {
+              const int4 q4 = *(const int4*)&qsg[buf][r0 + 8 * ii];
+              x[ii * 4 + 0] = q4.x == sk ? x[ii * 4 + 0] : -MXA_INF;
+              x[ii * 4 + 1] = q4.y == sk ? x[ii * 4 + 1] : -MXA_INF;
+              x[ii * 4 + 2] = q4.z == sk ? x[ii * 4 + 2] : -MXA_INF;
+              x[ii * 4 + 3] = q4.w == sk ? x[ii * 4 + 3] : -MXA_INF;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[i] = p0 + 8 * (i >> 2) + (i & 3) >= first ? x[i] : -MXA_INF;
+        }
+        bf16x8 pf[2], df[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float p[8], ds[8];
+#pragma unroll
+          for (int ii = 0; ii < 2; ++ii) {
+            const f32x4 l4 = *(const f32x4*)&lses[buf][r0 + 8 * (2 * w + ii)];
+            const f32x4 e4 = *(const f32x4*)&dels[buf][r0 + 8 * (2 * w + ii)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = 8 * w + 4 * ii + i;
+              p[4 * ii + i] = fexp2(x[k] - l4[i]);
+              ds[4 * ii + i] = p[4 * ii + i] * (dp[k] - e4[i]);
+              if (CAP) ds[4 * ii + i] *= u[k];
+            }
+          }
+          pf[w] = pack8(p);
+          df[w] = pack8(ds);
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            dv[db] = mfma32(attn_tr_frag<D>(gimg[buf], nb * 32 + w * 16,
+                                            db * 32, lane),
+                            pf[w], dv[db]);
+            dk[db] = mfma32(attn_tr_frag<D>(qimg[buf], nb * 32 + w * 16,
+                                            db * 32, lane),
+                            df[w], dk[db]);
+          }
+      }
+    }
+    cur = nxt;
+    buf ^= 1;
+  }
+
+  if (kj < a.Tk) {
+    const long off = ((long)b * a.Tk + kj) * a.Hkv * a.D + (long)hk * a.D;
+    attn_store_t<DB>(a.dk + off, dk, a.scale, a.D, half);
+    attn_store_t<DB>(a.dv + off, dv, 1.f, a.D, half);
+  }
+}
+
+void attn_mod_bwd(const AttnArgs& a, bool need_kv, hipStream_t s) {
+  dim3 gq((unsigned)((long)a.B * a.H * cdiv_h(a.Tq, 128)));
+  dim3 gk((unsigned)((long)a.B * a.Hkv * cdiv_h(a.Tk, 128)));
+  const bool c = a.cap != 0.f, w = a.slopes != nullptr;
+#define GO(D, C, W)                                 \
+  do {                                              \
+    attn_mod_dq_kernel<D, C, W><<<gq, 256, 0, s>>>(a);  \
+    if (need_kv)                                         \
+      attn_mod_dkv_kernel<D, C, W><<<gk, 256, 0, s>>>(a); \
+  } while (0)
+#define PICK(D)                       \
+  do {                                \
+    if (c && w)                       \
+      GO(D, true, true);              \
+    else if (c)                       \
+      GO(D, true, false);             \
+    else if (w)                       \
+      GO(D, false, true);             \
+    else                              \
+      GO(D, false, false);            \
+  } while (0)
+  if (a.D <= 64)
+    PICK(64);
+  else
+    PICK(128);
+#undef PICK
+#undef GO
+}
+
+}  // namespace mxa

@@ -1,0 +1,211 @@
+// Forward pass of attention with shaped scores (see attn_mod.h).
+//
+// One block: 128 queries of one head, four waves of 32 queries.  Keys and
+// values pass through LDS in tiles of 64, double buffered by direct copies;
+// tiles that no query of the block can see are never touched.  A wave
+// computes S^T = K Q^T (queries along the lanes), so the softmax statistics
+// of a query lie in one lane of each half of the wave, and feeds the rounded
+// P^T straight into O^T += V^T P^T.
+//
+// The running maximum moves only when some row's scores pass it by more
+// than 8 (a factor of 256, harmless in fp32 sums and bf16 probabilities), so
+// the rescaling of the accumulators is skipped for almost every tile.
+#include "attn_mod.h"
+
+namespace mxa {
+
+// Smallest and largest document id of every 64 rows: [B][nt].
+__global__ __launch_bounds__(256) void attn_seg_ranges_kernel(
+    const int* __restrict__ seg, int2* __restrict__ out, int T, int nt,
+    long total) {
+  long w = (long)blockIdx.x * 4 + threadIdx.x / 64;
+  int lane = threadIdx.x & 63;
+  if (w >= total) return;
+  long b = w / nt;
+  int t = (int)(w % nt) * 64 + lane;
+  int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+  if (t < T) lo = hi = seg[b * T + t];
+  lo = wave_min(lo);
+  hi = wave_max(hi);
+  if (lane == 0) out[w] = make_int2(lo, hi);
+}
+
+void attn_seg_ranges(const int* seg, int2* out, int B, int T,
+                     hipStream_t s) {
+  int nt = cdiv_h(T, 64);
+  long total = (long)B * nt;
+  attn_seg_ranges_kernel<<<(unsigned)((total + 3) / 4), 256, 0, s>>>(
+      seg, out, T, nt, total);
+}
+
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
+  constexpr int KK = D / 16, DB = D / 32;
+  __shared__ __align__(16) bf16 kimg[2][64 * D];
+  __shared__ __align__(16) bf16 vimg[2][64 * D];
+  __shared__ __align__(16) int ksg[2][64];
+  __shared__ int4 spans[4];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  // consecutive ids share a head, and so its keys, on one XCD; the last
+  // queries (the longest rows of a causal mask) start first
+  const int nqb = cdiv(a.Tq, 128);
+  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int qb = nqb - 1 - id % nqb;
+  const int h = (id / nqb) % a.H, b = id / nqb / a.H;
+  const int hk = h / a.G;
+  const SeqMask m = attn_seq_mask(a, b);
+
+  const int q0 = qb * 128 + wave * 32;
+  const int qi = q0 + col;
+  const bool qok = qi < a.Tq;
+  const int pos = qi + m.off;
+  int sq = 0;
+  if (m.has_seg) sq = qok ? a.seg_q[(long)b * a.Tq + qi] : -1;
+
+  RowSpan wav, blk;
+  attn_spans(m, q0, a.Tq, qok, sq, spans, wave, lane, wav, blk);
+  const int limit = m.has_seg && sq < 0 ? 0 : attn_limit(m, pos);
+  ScoreFn f;
+  f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
+
+  bf16x8 qf[KK];
+  {
+    const bf16* qp = a.q + b * a.qsb + (long)qi * a.qst + (long)h * a.D;
+    const bool ok = qok && sq >= 0;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[kk] = attn_load_row(qp, kk * 2 + half, a.D, ok);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
+  }
+
+  const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
+  const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
+  const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
+  const int ntk = cdiv(a.Tk, 64);
+  const int2* rng = m.has_seg ? a.rng_k + (long)b * ntk : nullptr;
+
+  auto stage = [&](int buf, const Tile& t) {
+    const int* sg = t.neg ? skb : nullptr;
+    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg, kimg[buf],
+                         wave, lane);
+    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg, vimg[buf],
+                         wave, lane);
+    if (m.has_seg && wave == 0)
+      attn_stage64(skb, t.t * 64, a.Tk, ksg[buf], lane);
+  };
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = zero16();
+  float mrow = M_INIT, lsum = 0.f;
+
+  TileWalk walk;
+  walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
+  Tile cur = walk.next(m, blk, wav, rng, lane);
+  if (cur.t >= 0) stage(0, cur);
+  int buf = 0;
+  while (cur.t >= 0) {
+    attn_wait_copies<0>();
+    __syncthreads();  // this tile has landed, the other buffer is free
+    Tile nxt = walk.next(m, blk, wav, rng, lane);
+    if (nxt.t >= 0) stage(buf ^ 1, nxt);
+    if (cur.work) {
+      f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+          s[nb] = mfma32(
+              attn_row_frag<D>(kimg[buf], nb * 32 + col, kk * 2 + half),
+              qf[kk], s[nb]);
+
+      const int j0 = cur.t * 64 + 4 * half;
+      const float d0 = BIAS ? (float)(pos - j0) : 0.f;
+      float x[32], mx = -MXA_INF;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int dj = 8 * (i >> 2) + (i & 3);
+        x[i] = attn_score<CAP>(f, s[i >> 4][i & 15]);
+        if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
+      }
+      if (!cur.full) {
+        attn_mask_keys(x, m.has_seg, &ksg[buf][4 * half], sq, limit - j0);
+        attn_mask_keys(x + 16, m.has_seg, &ksg[buf][32 + 4 * half], sq,
+                       limit - j0 - 32);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      if (__ballot(mx > mrow + 8.f)) {
+        float mnew = fmaxf(mrow, mx);
+        float al = fexp2(mrow - mnew);
+        mrow = mnew;
+        lsum *= al;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[db][i] *= al;
+      }
+      bf16x8 pf[4];
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = fexp2(x[8 * st + i] - mrow);
+          lsum += p[i];
+        }
+        pf[st] = pack8(p);
+      }
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          o[db] = mfma32(
+              attn_tr_frag<D>(vimg[buf], st * 16, db * 32, lane), pf[st],
+              o[db]);
+    }
+    cur = nxt;
+    buf ^= 1;
+  }
+
+  lsum += __shfl_xor(lsum, 32, 64);
+  // a sum of zero: nothing seen, the row is zero; a NaN stays one
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  if (qok) {
+    bf16* op = a.o + b * a.osb + (long)qi * a.ost + (long)h * a.D;
+    attn_store_t<DB>(op, o, inv, a.D, half);
+  }
+  if (a.lse && half == 0 && qi < a.TqP)
+    a.lse[((long)b * a.H + h) * a.TqP + qi] =
+        qok && lsum != 0.f ? mrow + __log2f(lsum) : MXA_INF;
+}
+
+void attn_mod_fwd(const AttnArgs& a, hipStream_t s) {
+  dim3 g((unsigned)((long)a.B * a.H * cdiv_h(a.Tq, 128)));
+  const bool c = a.cap != 0.f, w = a.slopes != nullptr;
+#define GO(D, C, W) attn_mod_fwd_kernel<D, C, W><<<g, 256, 0, s>>>(a)
+#define PICK(D)                       \
+  do {                                \
+    if (c && w)                       \
+      GO(D, true, true);              \
+    else if (c)                       \
+      GO(D, true, false);             \
+    else if (w)                       \
+      GO(D, false, true);             \
+    else                              \
+      GO(D, false, false);            \
+  } while (0)
+  if (a.D <= 64)
+    PICK(64);
+  else
+    PICK(128);
+#undef PICK
+#undef GO
+}
+
+}  // namespace mxa

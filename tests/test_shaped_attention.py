@@ -1,0 +1,159 @@
+"""Attention with shaped scores on the CPU: values and gradients against the
+definition in 64 bits, gradients against differences, refusals."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import anand_mxnet_amd as mx
+from anand_mxnet_amd import nd
+from anand_mxnet_amd.base import MXNetError
+
+sys.path.insert(0, os.path.dirname(__file__))
+from shaped_attention_ref import reference, visible  # noqa: E402
+
+SEG = np.array([[0, 0, 0, 1, 1, -1, 2, 2, 2], [4, 4, 4, 4, 4, 4, 4, -3, -3]],
+               np.int32)
+CASES = [
+    dict(logit_cap=3.0, causal=True),
+    dict(slopes=True),
+    dict(logit_cap=2.0, slopes=True, segment_ids=SEG, causal=True),
+    dict(prefix_length=np.array([4, 0]), causal=True, slopes=True),
+    dict(kv_length=np.array([0, 5]), query_offset=np.array([-1, 3]),
+         causal=True),
+    dict(query_offset=2, causal=True),
+]
+
+
+def _setup(i):
+    kw = dict(CASES[i])
+    rng = np.random.default_rng(i)
+    H, Hkv, D, T = 4, 2, 8, 9
+    q = torch.from_numpy(rng.standard_normal((2, T, H * D)))
+    k = torch.from_numpy(rng.standard_normal((2, T, Hkv * D)))
+    v = torch.from_numpy(rng.standard_normal((2, T, Hkv * D)))
+    g = torch.from_numpy(rng.standard_normal((2, T, H * D)))
+    sl = torch.tensor([0.5, 0.25, 0.125, 0.0625]) if kw.pop("slopes", False) \
+        else None
+    seg = kw.get("segment_ids")
+    ok, pos = visible(2, T, T, kw.get("causal", False), seg, seg,
+                      kw.get("prefix_length"), kw.get("kv_length"),
+                      kw.get("query_offset", 0))
+    ref = reference(q, k, v, g, H, Hkv, ok, pos, None, kw.get("logit_cap"),
+                    sl)
+    for key in ("segment_ids", "prefix_length", "kv_length", "query_offset"):
+        if isinstance(kw.get(key), np.ndarray):
+            kw[key] = nd.from_torch(torch.from_numpy(kw[key]))
+    if sl is not None:
+        kw["distance_slopes"] = nd.from_torch(sl)
+    return q, k, v, g, kw, ref
+
+
+def _run(q, k, v, g, kw):
+    a = [nd.from_torch(t.clone()) for t in (q, k, v)]
+    for x in a:
+        x.attach_grad()
+    with mx.autograd.record():
+        out = nd.multi_head_attention(*a, 4, num_kv_heads=2, **kw)
+    out.backward(nd.from_torch(g.to(out._t.dtype)))
+    return [out._t.detach()] + [x.grad._t for x in a]
+
+
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_matches_definition(i):
+    q, k, v, g, kw, ref = _setup(i)
+    got = _run(q, k, v, g, kw)
+    for t, name in zip(got, ("out", "dq", "dk", "dv")):
+        # 64-bit sums of fewer than a thousand terms of order one
+        assert torch.allclose(t, ref[name][0], rtol=1e-10, atol=1e-11), name
+
+
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_gradient_against_differences(i):
+    q, k, v, g, kw, _ = _setup(i)
+    _, dq, dk, dv = _run(q, k, v, g, kw)
+    rng = np.random.default_rng(50 + i)
+    eps = 1e-5
+    for which, grad in ((0, dq), (1, dk), (2, dv)):
+        step = torch.from_numpy(rng.standard_normal(grad.shape))
+        vals = []
+        for sgn in (1, -1):
+            a = [q, k, v]
+            a[which] = a[which] + sgn * eps * step
+            out = nd.multi_head_attention(*[nd.from_torch(t) for t in a], 4,
+                                          num_kv_heads=2, **kw)._t
+            vals.append((out * g).sum())
+        diff = float(vals[0] - vals[1]) / (2 * eps)
+        # central difference: eps**2 times third derivatives (at most about
+        # 1e3 here) and 1e-16 * 1e2 / eps of cancellation
+        assert abs(diff - float((grad * step).sum())) < 1e-6
+
+
+def test_bf16_cpu_and_empty_rows():
+    q = nd.from_torch(torch.randn(1, 3, 16).bfloat16())
+    out = nd.multi_head_attention(
+        q, q, q, 2, segment_ids=nd.from_torch(torch.tensor([[0, -1, 0]])))
+    assert out._t.dtype == torch.bfloat16
+    assert not out._t[0, 1].any() and out._t[0, 0].any()
+
+
+def test_nan_in_unseen_places():
+    q = torch.randn(1, 4, 16)
+    k = q.clone()
+    k[:, 3] = float("nan")
+    out = nd.multi_head_attention(
+        nd.from_torch(q), nd.from_torch(k), nd.from_torch(k), 2,
+        kv_length=nd.from_torch(torch.tensor([3])))
+    assert torch.isfinite(out._t).all()
+
+
+def _x(*s):
+    return nd.from_torch(torch.zeros(*s))
+
+
+def _i(*s):
+    return nd.from_torch(torch.zeros(*s, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(logit_cap=0.0), dict(logit_cap=-1.0), dict(logit_cap=float("inf")),
+    dict(logit_cap=float("nan")),
+    dict(num_kv_heads=3), dict(num_kv_heads=1),
+    dict(distance_slopes="bad"), dict(distance_slopes=_i(2)),
+    dict(distance_slopes=_x(3)),
+    dict(segment_ids=_x(2, 5)), dict(segment_ids=_i(2, 4)),
+    dict(kv_segment_ids=_i(2, 5)),
+    dict(prefix_length=_i(2)),                       # not causal
+    dict(prefix_length=_i(3), causal=True),
+    dict(kv_length=_i(1)), dict(kv_length=7.0),
+    dict(query_offset=_i(2, 1)), dict(query_offset=1 << 40),
+    dict(logit_cap=5.0, mask=_x(2, 2, 5, 5)),
+])
+def test_refuses(kw):
+    q = _x(2, 5, 16)
+    with pytest.raises(MXNetError):
+        nd.multi_head_attention(q, q, q, 2, **kw)
+
+
+def test_refuses_more():
+    q, k = _x(2, 5, 16), _x(2, 6, 16)
+    f = nd.multi_head_attention
+    with pytest.raises(MXNetError):
+        f(q, k, k, 2, segment_ids=_i(2, 5))          # keys' ids missing
+    with pytest.raises(MXNetError):
+        f(q, k, q, 2, logit_cap=1.0)                 # v unlike k
+    with pytest.raises(MXNetError):
+        f(q, _x(3, 5, 16), _x(3, 5, 16), 2, logit_cap=1.0)
+    with pytest.raises(MXNetError):
+        f(_x(2, 5, 15), q, q, 2, logit_cap=1.0)
+    s = nd.from_torch(torch.zeros(2))
+    s.attach_grad()
+    with pytest.raises(MXNetError):
+        f(q, q, q, 2, distance_slopes=s)
+    with mx.autograd.record():
+        with pytest.raises(MXNetError):
+            f(q, q, q, 2, logit_cap=1.0, dropout_p=0.1)
+    # outside training dropout does nothing
+    f(q, q, q, 2, logit_cap=1.0, dropout_p=0.1)
