@@ -27,6 +27,8 @@
 // is fetched in the same order by transposing LDS reads of four rows each.
 // Probabilities never leave the registers.
 #pragma once
+#include <hip/hip_runtime.h>
+
 #include "common.h"
 
 namespace mxa {
