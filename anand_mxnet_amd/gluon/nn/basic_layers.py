@@ -268,9 +268,14 @@ class InstanceNorm(HybridBlock):
 
 
 class Embedding(HybridBlock):
+    """Rows of a table; scale multiplies them (transformers: the square root
+    of output_dim) in the lookup itself, rounded once."""
+
     def __init__(self, input_dim, output_dim, dtype="float32",
-                 weight_initializer=None, sparse_grad=False, **kwargs):
+                 weight_initializer=None, sparse_grad=False, scale=1.0,
+                 **kwargs):
         super().__init__(**kwargs)
+        self._scale = float(scale)
         self._input_dim = input_dim
         self._output_dim = output_dim
         self.weight = self.params.get("weight", shape=(input_dim, output_dim),
@@ -278,8 +283,9 @@ class Embedding(HybridBlock):
                                       allow_deferred_init=True)
 
     def hybrid_forward(self, F, x, weight):
+        kw = {} if self._scale == 1.0 else {"scale": self._scale}
         return F.Embedding(x, weight, input_dim=self._input_dim,
-                           output_dim=self._output_dim)
+                           output_dim=self._output_dim, **kw)
 
 
 class Flatten(HybridBlock):

@@ -1,8 +1,11 @@
 """Gluon utils (parity with python/mxnet/gluon/utils.py)."""
 from __future__ import annotations
 
+import math
+
 import torch
 
+from ..base import MXNetError
 from ..ndarray.ndarray import NDArray, array
 from ..context import Context
 from .. import ndarray as nd
@@ -37,9 +40,22 @@ def split_and_load(data, ctx_list, batch_axis=0, even_split=True):
 def clip_global_norm(arrays, max_norm, check_isfinite=True):
     """Rescale arrays so that the sum of their 2-norms <= max_norm.
 
-    GPU path: fused multi_sum_sq kernel (one launch over all tensors)."""
+    GPU path: nd.multi_clip_global_norm, which sums and scales all arrays in
+    two kernels; call that one where the host need not wait for the norm."""
     assert len(arrays) > 0
     from ..ops.registry import RAW
+    ts = [a._t for a in arrays]
+    if ts[0].is_cuda:
+        try:
+            norm = float(RAW["multi_clip_global_norm"](ts, max_norm))
+        except MXNetError:
+            pass  # other types, several devices, shared memory: one by one
+        else:
+            if check_isfinite and not math.isfinite(norm):
+                import warnings
+                warnings.warn("nan or inf is detected. Clipping results "
+                              "will be undefined.", stacklevel=2)
+            return norm
     sums = RAW["multi_sum_sq"]([a._t for a in arrays])
     total = torch.stack([s if isinstance(s, torch.Tensor)
                          else torch.as_tensor(s) for s in sums]).sum()

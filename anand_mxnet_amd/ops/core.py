@@ -549,9 +549,13 @@ def smooth_l1(x, scalar=1.0):
 # ---------------- indexing ----------------
 @register("Embedding")
 def embedding(data, weight, input_dim=None, output_dim=None, dtype=None,
-              sparse_grad=False):
+              sparse_grad=False, scale=1.0):
+    """Rows of weight, times scale.  On the GPU (bfloat16, float16 and
+    float32; embedding.hip) an index outside the table gives a row of zeros,
+    and the gradient of the table is summed in 32 bits in the order of the
+    tokens: the same bits in every run."""
     from . import nn as _nn
-    return _nn.embedding_impl(data, weight)
+    return _nn.embedding_impl(data, weight, scale)
 
 
 @register("take")

@@ -713,24 +713,28 @@ def dropout(x, p):
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, idx, W):
+    def forward(ctx, idx, W, scale):
         ctx.save_for_backward(idx)
         ctx.vocab = W.shape[0]
-        ctx.wdtype = W.dtype
-        return _C.embedding_fwd(idx, W.contiguous())
+        ctx.scale = scale
+        return _C.embedding_fwd(idx, W.contiguous(), scale)
 
     @staticmethod
     def backward(ctx, dy):
         (idx,) = ctx.saved_tensors
-        dW = _C.embedding_bwd(idx, dy.contiguous(), ctx.vocab)
-        return None, dW.to(ctx.wdtype)
+        return None, _C.embedding_bwd(idx, dy.contiguous(), ctx.vocab,
+                                      ctx.scale), None
+
+
+_NATIVE_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 @register_gpu("embedding")
-def embedding(idx, W):
-    if W.dtype != torch.bfloat16 or W.shape[1] % 8 != 0:
-        return torch.nn.functional.embedding(idx.long(), W)
-    return _Embedding.apply(idx, W)
+def embedding(idx, W, scale=1.0):
+    if W.dtype not in _NATIVE_FLOATS:
+        out = torch.nn.functional.embedding(idx.long(), W)
+        return out if scale == 1.0 else out * scale
+    return _Embedding.apply(idx, W, scale)
 
 
 _ACT_IDS = {"relu": 0, "sigmoid": 1, "tanh": 2, "gelu": 3, "silu": 4,
@@ -785,6 +789,23 @@ def multi_opt_run(blob, ntens, nchunks, mode, wbf16, lr, momentum, beta1,
 
 def multi_sumsq(blob, ntens, nchunks, bf16in):
     return _C.multi_sumsq_run(blob, ntens, nchunks, bf16in)
+
+
+@register_gpu("multi_clip_global_norm")
+def multi_clip_global_norm(arrays, max_norm, out):
+    """One norm over all arrays and their clipping (clip_norm.hip); the
+    factor stays on the device."""
+    if all(t.is_contiguous() for t in arrays) and (
+            out is arrays or all(t.is_contiguous() for t in out)):
+        return _C.clip_global_norm(arrays, out, max_norm)
+    src = [t.contiguous() for t in arrays]
+    dst = [s if o is a else o if o.is_contiguous() else torch.empty_like(s)
+           for a, s, o in zip(arrays, src, out)]
+    norm = _C.clip_global_norm(src, dst, max_norm)
+    for o, d in zip(out, dst):
+        if o is not d:
+            o.copy_(d)
+    return norm
 
 
 # ---------------------------------------------------------------------------

@@ -198,6 +198,94 @@ def multi_sum_sq(arrays):
     return [a.float().pow(2).sum() for a in arrays]
 
 
+@register("multi_clip_global_norm")
+def multi_clip_global_norm(arrays, max_norm, out=None):
+    """Scale many arrays so that their common 2-norm is at most max_norm:
+    each becomes x * min(1, max_norm / (norm + 1e-8)), in place, or into the
+    arrays of out.  Returns the norm (float32, no host wait).
+
+    Squares are summed in 64 bits.  A NaN norm leaves the values as they
+    are.  GPU: bfloat16, float16 and float32, mixed as they come, two kernels
+    (clip_norm.hip) for up to 140 arrays.  An array that is written must not
+    overlap another one."""
+    from ..base import MXNetError
+
+    def need(ok, what):
+        if not ok:
+            raise MXNetError("multi_clip_global_norm: " + what)
+
+    need(isinstance(arrays, (list, tuple)) and len(arrays) > 0
+         and isinstance(arrays[0], torch.Tensor),
+         "a list of arrays is needed")
+    max_norm = float(max_norm)
+    need(max_norm >= 0.0, "max_norm must not be negative")
+    if out is None:
+        out = arrays
+    need(isinstance(out, (list, tuple)) and len(out) == len(arrays),
+         "one output for each array is needed")
+    with torch.no_grad():
+        if arrays[0].is_cuda and all(t.is_contiguous() for t in arrays) \
+                and all(t.is_contiguous() for t in out):
+            try:  # the extension checks the rest: many arrays, little time
+                return gpu_impl("multi_clip_global_norm")(arrays, max_norm,
+                                                          out)
+            except RuntimeError as e:
+                if "clip_global_norm: " not in str(e):
+                    raise
+                raise MXNetError("multi_" + str(e).splitlines()[0]) from None
+        for a, o in zip(arrays, out):
+            need(isinstance(a, torch.Tensor) and a.dtype.is_floating_point
+                 and a.device == arrays[0].device,
+                 "floating point arrays on one device are needed")
+            need(isinstance(o, torch.Tensor) and o.shape == a.shape
+                 and o.dtype == a.dtype and o.device == a.device,
+                 "an output is unlike its array")
+        _check_clip_overlap(arrays, out, need)
+        if _maybe_hip("multi_clip_global_norm", arrays[0]):
+            need(all(a.dtype in (torch.bfloat16, torch.float16,
+                                 torch.float32) for a in arrays),
+                 "the kernels take bfloat16, float16 and float32")
+            return gpu_impl("multi_clip_global_norm")(arrays, max_norm, out)
+        src = [a.detach() for a in arrays]
+        dst = [o.detach() for o in out]
+        total = sum(a.double().square().sum() for a in src)
+        norm = total.sqrt()
+        f = float(max_norm / (norm + 1e-8))
+        for s, d in zip(src, dst):
+            if f < 1.0:
+                ct = torch.promote_types(s.dtype, torch.float32)
+                d.copy_((s.to(ct) * f).to(s.dtype))
+            elif d.data_ptr() != s.data_ptr():
+                d.copy_(s)
+        return norm.float()
+
+
+def _span(t):
+    """First and last byte address of a tensor, and one behind."""
+    a = t.data_ptr()
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return a, a + (last + 1) * t.element_size()
+
+
+def _check_clip_overlap(src, dst, need):
+    spans = []
+    for s, d in zip(src, dst):
+        if s.numel() == 0:
+            continue
+        same = s.data_ptr() == d.data_ptr() and s.stride() == d.stride()
+        if not same:
+            spans.append(_span(s) + (False,))
+        spans.append(_span(d) + (True,))
+    spans.sort()
+    end = wend = 0
+    for a, e, write in spans:
+        need(a >= (end if write else wend),
+             "an array that is written overlaps another one")
+        end = max(end, e)
+        if write:
+            wend = max(wend, e)
+
+
 @register("adamw_update")
 def adamw_update(weight, grad, mean, var, rescale_grad, lr, beta1=0.9,
                  beta2=0.999, epsilon=1e-8, wd=0.0, eta=1.0,

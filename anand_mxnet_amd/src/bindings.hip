@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 #include <ATen/hip/HIPContext.h>
 
+#include <algorithm>
 #include <unordered_map>
 #include <vector>
 
@@ -100,10 +101,16 @@ void dropout_fwd_bf16(const bf16*, bf16*, unsigned char*, long,
 void rng_bump_launch(unsigned long long*, hipStream_t);
 void dropout_bwd_bf16(const bf16*, const unsigned char*, bf16*, long, float,
                       hipStream_t);
-void embedding_fwd_bf16(const long*, const bf16*, bf16*, long, int, long,
-                        hipStream_t);
-void embedding_bwd_bf16(const long*, const bf16*, float*, long, int, long,
-                        hipStream_t);
+// embedding.hip
+void emb_lookup(int, bool, bool, const void*, const void*, void*, long, int,
+                long, float, hipStream_t);
+int emb_chunks(long);
+void emb_grad(int, bool, bool, const void*, const void*, void*, int*, int2*,
+              float*, int, int, int, float, hipStream_t);
+// clip_norm.hip
+long clip_ws(long);
+void clip_norm(const void* const*, void* const*, const long*, const int*,
+               long, double, double*, float*, hipStream_t);
 void colsum_bf16(const bf16*, float*, long, int, hipStream_t);
 void im2col_stem_bf16(const bf16*, bf16*, int, int, int, int, int, int,
                       int, int, int, int, int, int, int, int, int, int,
@@ -1418,29 +1425,137 @@ at::Tensor dropout_bwd(const at::Tensor& dy, const at::Tensor& mask,
   return dx;
 }
 
-at::Tensor embedding_fwd(const at::Tensor& idx, const at::Tensor& W) {
-  auto idx_l = idx.to(at::kLong).contiguous();
-  long ntok = idx_l.numel();
-  int D = W.size(1);
-  TORCH_CHECK(D % 8 == 0, "embedding: dim must be %8");
+namespace {
+// 0 bf16, 1 fp16, 2 fp32
+int float_code(const at::Tensor& t, const char* op) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default:
+      TORCH_CHECK(false, op, ": bfloat16, float16 or float32 required, got ",
+                  t.scalar_type());
+  }
+}
+
+// rows of D values can be read 16 bytes at a time
+bool rows16(const void* p, long D, long elem) {
+  return (size_t)p % 16 == 0 && D * elem % 16 == 0;
+}
+}  // namespace
+
+// out[n] = scale * W[idx[n]]; rows outside the table are zero
+at::Tensor embedding_fwd(const at::Tensor& idx, const at::Tensor& W,
+                         double scale) {
+  c10::DeviceGuard guard(W.device());
+  TORCH_CHECK(W.dim() == 2 && W.is_contiguous() && W.is_cuda(),
+              "embedding: the table must be a contiguous GPU matrix");
+  TORCH_CHECK(idx.device() == W.device(),
+              "embedding: indices and table are on different devices");
+  const int dt = float_code(W, "embedding");
+  auto ix = idx.scalar_type() == at::kInt ? idx.contiguous()
+                                          : idx.to(at::kLong).contiguous();
+  const long ntok = ix.numel(), D = W.size(1);
+  TORCH_CHECK(D < (1L << 31), "embedding: rows are too long");
   auto sizes = idx.sizes().vec();
   sizes.push_back(D);
   auto out = at::empty(sizes, W.options());
-  mxa::embedding_fwd_bf16(idx_l.data_ptr<long>(), bfp(W), bfp_mut(out),
-                          ntok, D, W.size(0), cur_stream());
+  if (out.numel() == 0) return out;
+  mxa::emb_lookup(dt, rows16(W.data_ptr(), D, W.element_size()),
+                  ix.scalar_type() == at::kLong, ix.data_ptr(), W.data_ptr(),
+                  out.data_ptr(), ntok, (int)D, W.size(0), (float)scale,
+                  cur_stream());
   return out;
 }
 
+// dW[r] = scale * sum of dy[n] where idx[n] = r, in dy's type
 at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
-                         long vocab) {
-  auto idx_l = idx.to(at::kLong).contiguous();
-  long ntok = idx_l.numel();
-  int D = dy.size(-1);
-  auto dW = at::empty({vocab, D}, dy.options().dtype(at::kFloat));
-  mxa::embedding_bwd_bf16(idx_l.data_ptr<long>(), bfp(dy),
-                          dW.data_ptr<float>(), ntok, D, vocab,
-                          cur_stream());
+                         long vocab, double scale) {
+  c10::DeviceGuard guard(dy.device());
+  TORCH_CHECK(dy.is_contiguous() && dy.is_cuda() &&
+                  idx.device() == dy.device(),
+              "embedding: gradients must be contiguous, on the GPU");
+  const int dt = float_code(dy, "embedding");
+  auto ix = idx.scalar_type() == at::kInt ? idx.contiguous()
+                                          : idx.to(at::kLong).contiguous();
+  const long ntok = ix.numel(), D = dy.size(-1);
+  TORCH_CHECK(dy.numel() == ntok * D,
+              "embedding: one gradient row for each index");
+  TORCH_CHECK(vocab < 0x7fffffff && ntok < 0x7fffff00 && D < 0x7fffffff,
+              "embedding: too large");
+  if (ntok == 0) return at::zeros({vocab, D}, dy.options());
+  auto dW = at::empty({vocab, D}, dy.options());
+  if (dW.numel() == 0) return dW;
+  auto iopt = dy.options().dtype(at::kInt);
+  auto start = at::empty({vocab + 1}, iopt);
+  auto sorted = at::empty({ntok, 2}, iopt);
+  auto part = at::empty({(long)mxa::emb_chunks(ntok), 2, D},
+                        dy.options().dtype(at::kFloat));
+  mxa::emb_grad(dt, rows16(dy.data_ptr(), D, dy.element_size()),
+                ix.scalar_type() == at::kLong, ix.data_ptr(), dy.data_ptr(),
+                dW.data_ptr(), start.data_ptr<int>(),
+                (int2*)sorted.data_ptr<int>(), part.data_ptr<float>(),
+                (int)ntok, (int)D, (int)vocab, (float)scale, cur_stream());
   return dW;
+}
+
+// Writes src[i] * min(1, max_norm / (norm + 1e-8)) to dst[i] (which may be
+// src[i] itself), norm over all of src; returns the norm.
+at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
+                            const std::vector<at::Tensor>& dst,
+                            double max_norm) {
+  TORCH_CHECK(!src.empty() && src.size() == dst.size(),
+              "clip_global_norm: one output for each array");
+  const auto dev = src[0].device();
+  c10::DeviceGuard guard(dev);
+  struct Span {
+    size_t a, e;
+    bool write;
+  };
+  std::vector<Span> spans;
+  std::vector<const void*> sp;
+  std::vector<void*> dp;
+  std::vector<long> n;
+  std::vector<int> dt;
+  for (size_t i = 0; i < src.size(); ++i) {
+    TORCH_CHECK(src[i].is_cuda() && src[i].device() == dev &&
+                    dst[i].device() == dev,
+                "clip_global_norm: arrays on different devices");
+    TORCH_CHECK(src[i].is_contiguous() && dst[i].is_contiguous() &&
+                    src[i].sizes() == dst[i].sizes() &&
+                    src[i].scalar_type() == dst[i].scalar_type(),
+                "clip_global_norm: an output is unlike its array");
+    const int code = float_code(src[i], "clip_global_norm");
+    if (src[i].numel() == 0) continue;
+    const size_t a = (size_t)src[i].data_ptr(),
+                 b = (size_t)dst[i].data_ptr(), len = src[i].nbytes();
+    sp.push_back((const void*)a);
+    dp.push_back((void*)b);
+    n.push_back(src[i].numel());
+    dt.push_back(code);
+    if (a != b) spans.push_back({a, a + len, false});
+    spans.push_back({b, b + len, true});
+  }
+  std::sort(spans.begin(), spans.end(),
+            [](const Span& x, const Span& y) { return x.a < y.a; });
+  size_t end = 0, wend = 0;  // of all spans so far, of the written ones
+  for (const Span& s : spans) {
+    TORCH_CHECK(s.a >= (s.write ? end : wend),
+                "clip_global_norm: an array that is written overlaps "
+                "another one");
+    end = std::max(end, s.e);
+    if (s.write) wend = std::max(wend, s.e);
+  }
+  for (const auto& t : dst)  // autograd must know of the write
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  auto norm = at::empty({}, src[0].options().dtype(at::kFloat));
+  if (sp.empty()) return norm.zero_();
+  auto ws = at::empty({mxa::clip_ws((long)sp.size())},
+                      src[0].options().dtype(at::kDouble));
+  mxa::clip_norm(sp.data(), dp.data(), n.data(), dt.data(), (long)sp.size(),
+                 max_norm, ws.data_ptr<double>(), norm.data_ptr<float>(),
+                 cur_stream());
+  return norm;
 }
 
 at::Tensor act_fwd(long op, const at::Tensor& x) {
@@ -1865,8 +1980,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("softmax_dropout_fwd", &softmax_dropout_fwd);
   m.def("softmax_dropout_bwd", &softmax_dropout_bwd);
   m.def("dropout_bwd", &dropout_bwd);
-  m.def("embedding_fwd", &embedding_fwd);
-  m.def("embedding_bwd", &embedding_bwd);
+  m.def("embedding_fwd", &embedding_fwd, py::arg("idx"), py::arg("W"),
+        py::arg("scale") = 1.0);
+  m.def("embedding_bwd", &embedding_bwd, py::arg("idx"), py::arg("dy"),
+        py::arg("vocab"), py::arg("scale") = 1.0);
+  m.def("clip_global_norm", &clip_global_norm);
   m.def("act_fwd", &act_fwd);
   m.def("act_bwd", &act_bwd);
   m.def("build_opt_descs", &build_opt_descs);

@@ -1,7 +1,7 @@
-// Dropout (counter-based RNG), Embedding gather/scatter-grad, and the
-// generic vectorized elementwise/activation family for gfx950.
+// Dropout (counter-based RNG) and the generic vectorized
+// elementwise/activation family for gfx950.
 // Reference parity: src/operator/nn/dropout.cu (philox mask+scale fused),
-// tensor/indexing_op.cu (Embedding/AddTakeGrad), mxnet_op.h Kernel::Launch
+// mxnet_op.h Kernel::Launch
 // (the generic elementwise launcher — here a bf16x8 grid-stride template).
 #include "common.h"
 
@@ -54,42 +54,6 @@ __global__ __launch_bounds__(256) void dropout_bwd(
     for (int j = 0; j < 8; ++j)
       o[j] = mb[j] ? f2bf(bf2f(g[j]) * scale) : (bf16)0.f;
     *(bf16x8*)&dx[i * 8] = o;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Embedding: row gather fwd; scatter-add (atomic fp32) bwd.
-// ---------------------------------------------------------------------------
-
-__global__ __launch_bounds__(256) void embedding_fwd(
-    const long* __restrict__ idx, const bf16* __restrict__ W,
-    bf16* __restrict__ out, long ntok, int D, long vocab) {
-  long total = ntok * (D / 8);
-  int dv = D / 8;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long)gridDim.x * blockDim.x) {
-    long tok = i / dv;
-    int d0 = (int)(i % dv) * 8;
-    long row = idx[tok];
-    if (row < 0 || row >= vocab) {
-      *(bf16x8*)&out[tok * D + d0] = bf16x8{};
-      continue;
-    }
-    *(bf16x8*)&out[tok * D + d0] = *(const bf16x8*)&W[row * D + d0];
-  }
-}
-
-__global__ __launch_bounds__(256) void embedding_bwd(
-    const long* __restrict__ idx, const bf16* __restrict__ dy,
-    float* __restrict__ dW, long ntok, int D, long vocab) {
-  long total = ntok * D;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long)gridDim.x * blockDim.x) {
-    long tok = i / D;
-    int d = (int)(i % D);
-    long row = idx[tok];
-    if (row < 0 || row >= vocab) continue;
-    atomicAdd(&dW[row * D + d], bf2f(dy[i]));
   }
 }
 
@@ -263,19 +227,6 @@ void dropout_bwd_bf16(const bf16* dy, const unsigned char* mask, bf16* dx,
   long nvec = n / 8;
   dropout_bwd<<<ew_grid(nvec), 256, 0, s>>>(dy, mask, dx, nvec,
                                             1.f / (1.f - p));
-}
-
-void embedding_fwd_bf16(const long* idx, const bf16* W, bf16* out,
-                        long ntok, int D, long vocab, hipStream_t s) {
-  embedding_fwd<<<ew_grid(ntok * (D / 8)), 256, 0, s>>>(idx, W, out, ntok,
-                                                        D, vocab);
-}
-
-void embedding_bwd_bf16(const long* idx, const bf16* dy, float* dW,
-                        long ntok, int D, long vocab, hipStream_t s) {
-  HIP_CHECK(hipMemsetAsync(dW, 0, vocab * D * sizeof(float), s));
-  embedding_bwd<<<ew_grid(ntok * D), 256, 0, s>>>(idx, dy, dW, ntok, D,
-                                                  vocab);
 }
 
 // Column sum (bias gradient): out[c] = sum_m x[m][c], bf16 in / f32 out.
