@@ -187,6 +187,22 @@ DEVINL int wave_max(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
+// Which (batch, head) and which block of its rows a launch id stands for,
+// nb blocks to each of n heads; rank 0 is the block with the most work.
+// Blocks with the most work of all heads come first, so that the launch ends
+// evenly; where the heads divide among the 8 XCDs (ids go round them), an
+// XCD keeps its heads, whose other side then stays in its L2.
+DEVINL void attn_block(int id, int n, int& head, int& rank) {
+  if (n % 8 == 0) {
+    const int per = n / 8, li = id / 8;
+    head = (id % 8) * per + li % per;
+    rank = li / per;
+  } else {
+    head = id % n;
+    rank = id / n;
+  }
+}
+
 // Positions and document ids that a group of queries spans.
 struct RowSpan {
   int pmin, pmax, smin, smax;
@@ -312,16 +328,18 @@ DEVINL void attn_mask_keys(float* x, int has_seg, const int* ksg, int sq,
     x[i] = 8 * (i >> 2) + (i & 3) < lim ? x[i] : -MXA_INF;
 }
 
-// Constants of the score function, in units of log2.
+// Constants of the score function, in units of log2.  The sign of the scale
+// goes to the queries (attn_load_q), c1 is positive.
 struct ScoreFn {
   float c1, A, slope;
   template <bool CAP>
   DEVINL void set(float scale, float cap, float slope_) {
+    const float sc = scale == 0.f ? 1.f : fabsf(scale);
     if (CAP) {
-      c1 = scale / cap * 2.f * LOG2E;
+      c1 = sc / cap * 2.f * LOG2E;
       A = cap * LOG2E;
     } else {
-      c1 = scale * LOG2E;
+      c1 = sc * LOG2E;
       A = 0.f;
     }
     slope = -slope_ * LOG2E;
@@ -335,6 +353,18 @@ DEVINL float attn_score(const ScoreFn& f, float s, float* u = nullptr) {
   float r = frcp(1.f + fexp2(s * f.c1));
   if (u) *u = 4.f * (r - r * r);
   return f.A - (2.f * f.A) * r;
+}
+
+// Query fragments times the sign of the scale (exact).
+DEVINL bf16x8 attn_load_q(const bf16* p, int chunk, int Dact, bool ok,
+                          float scale) {
+  bf16x8 x = attn_load_row(p, chunk, Dact, ok && scale != 0.f);
+  if (scale < 0.f) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 y = __builtin_bit_cast(u32x4, x) ^ 0x80008000u;
+    x = __builtin_bit_cast(bf16x8, y);
+  }
+  return x;
 }
 
 DEVINL bf16x8 pack8(const float* x) {

@@ -27,10 +27,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int nqb = cdiv(a.Tq, 128);
-  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int qb = nqb - 1 - id % nqb;
-  const int h = (id / nqb) % a.H, b = id / nqb / a.H;
+  int bh, rank;
+  attn_block(blockIdx.x, a.B * a.H, bh, rank);
+  const int qb = cdiv(a.Tq, 128) - 1 - rank;
+  const int h = bh % a.H, b = bh / a.H;
   const int hk = h / a.G;
   const SeqMask m = attn_seq_mask(a, b);
 
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
     if (ok) lse = a.lse[row];
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      qf[kk] = attn_load_row(qp, kk * 2 + half, a.D, ok);
+      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
       gf[kk] = attn_load_row(gp, kk * 2 + half, a.D, ok);
       bf16x8 of = attn_load_row(op, kk * 2 + half, a.D, ok);
 #pragma unroll
@@ -178,10 +178,9 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int nkb = cdiv(a.Tk, 128);
-  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int kb = id % nkb;
-  const int hk = (id / nkb) % a.Hkv, b = id / nkb / a.Hkv;
+  int bh, kb;  // the first keys are seen by the most queries
+  attn_block(blockIdx.x, a.B * a.Hkv, bh, kb);
+  const int hk = bh % a.Hkv, b = bh / a.Hkv;
   const SeqMask m = attn_seq_mask(a, b);
 
   const int k0 = kb * 128 + wave * 32;
@@ -215,7 +214,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
     const bf16* vp = a.v + b * a.vsb + (long)kj * a.vst + (long)hk * a.D;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      kf[kk] = attn_load_row(kp, kk * 2 + half, a.D, kok);
+      kf[kk] = attn_load_q(kp, kk * 2 + half, a.D, kok, a.scale);
       vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
     }
 #pragma unroll

@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
     const bf16* qp = a.q + b * a.qsb + (long)tok * a.qst + (long)h * a.D;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
-      qf[kk] = attn_load_row(qp, kk * 2 + half, a.D, ok);
+      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
     asm volatile("" : "+v"(f.slope));

@@ -49,12 +49,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  // consecutive ids share a head, and so its keys, on one XCD; the last
-  // queries (the longest rows of a causal mask) start first
-  const int nqb = cdiv(a.Tq, 128);
-  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int qb = nqb - 1 - id % nqb;
-  const int h = (id / nqb) % a.H, b = id / nqb / a.H;
+  int bh, rank;
+  attn_block(blockIdx.x, a.B * a.H, bh, rank);
+  const int qb = cdiv(a.Tq, 128) - 1 - rank;  // last queries: longest rows
+  const int h = bh % a.H, b = bh / a.H;
   const int hk = h / a.G;
   const SeqMask m = attn_seq_mask(a, b);
 
@@ -77,7 +75,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
     const bool ok = qok && sq >= 0;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
-      qf[kk] = attn_load_row(qp, kk * 2 + half, a.D, ok);
+      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
   }
@@ -123,22 +121,53 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
               attn_row_frag<D>(kimg[buf], nb * 32 + col, kk * 2 + half),
               qf[kk], s[nb]);
 
+      // x[i] + base + (i >> 2) * step is the score.  A distance bias is
+      // linear in j where all keys of the tile lie before the wave's
+      // queries: it costs one addition for each four keys there.
       const int j0 = cur.t * 64 + 4 * half;
-      const float d0 = BIAS ? (float)(pos - j0) : 0.f;
-      float x[32], mx = -MXA_INF;
+      float x[32], base = 0.f, step = 0.f;
+      if (BIAS) {
+        const float d0 = (float)(pos - j0);
+        if (cur.t * 64 + 63 <= wav.pmin) {
+          base = f.slope * d0;
+          step = -8.f * f.slope;
+          const float e[4] = {0.f, -f.slope, -2.f * f.slope, -3.f * f.slope};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int dj = 8 * (i >> 2) + (i & 3);
-        x[i] = attn_score<CAP>(f, s[i >> 4][i & 15]);
-        if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
+          for (int i = 0; i < 32; ++i)
+            x[i] = CAP ? attn_score<CAP>(f, s[i >> 4][i & 15]) + e[i & 3]
+                       : fmaf(s[i >> 4][i & 15], f.c1, e[i & 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            x[i] = fmaf(f.slope,
+                        fabsf(d0 - (float)(8 * (i >> 2) + (i & 3))),
+                        attn_score<CAP>(f, s[i >> 4][i & 15]));
+        }
+      } else {
+        // without a cap the scores stay unscaled, exp2 scales them
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          x[i] = CAP ? attn_score<CAP>(f, s[i >> 4][i & 15])
+                     : s[i >> 4][i & 15];
       }
       if (!cur.full) {
         attn_mask_keys(x, m.has_seg, &ksg[buf][4 * half], sq, limit - j0);
         attn_mask_keys(x + 16, m.has_seg, &ksg[buf][32 + 4 * half], sq,
                        limit - j0 - 32);
       }
+      float mx = -MXA_INF;
+      if (BIAS) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
+        for (int g = 0; g < 8; ++g)
+          mx = fmaxf(mx, fmaf((float)g, step,
+                              fmaxf(fmaxf(x[4 * g], x[4 * g + 1]),
+                                    fmaxf(x[4 * g + 2], x[4 * g + 3]))));
+        mx += base;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
+        if (!CAP) mx *= f.c1;
+      }
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       if (__ballot(mx > mrow + 8.f)) {
         float mnew = fmaxf(mrow, mx);
@@ -156,7 +185,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = fexp2(x[8 * st + i] - mrow);
+          const int g = 2 * st + (i >> 2);
+          if (BIAS)
+            p[i] = fexp2(x[8 * st + i] - (mrow - base - (float)g * step));
+          else if (CAP)
+            p[i] = fexp2(x[8 * st + i] - mrow);
+          else
+            p[i] = fexp2(fmaf(x[8 * st + i], f.c1, -mrow));
           lsum += p[i];
         }
         pf[st] = pack8(p);
