@@ -75,25 +75,52 @@ DEVINL int attn_key(int r) {
                   : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
 }
 
+// The fragments of an image differ from lane to lane in a fixed way, and
+// from step to step in address bits that a lane's own address only meets by
+// exclusive or; whole rows are added.  A lane keeps these two addresses:
+//   row  its chunk of row (l & 31), for step 0
+//   tr   its place in the first transposing read of row 0, column 0
+struct LaneAddr {
+  unsigned row, tr;
+};
+
 template <int D>
-DEVINL bf16x8 attn_row_frag(const bf16* img, int row, int chunk) {
-  return *(const bf16x8*)&img[row * D + ((chunk ^ attn_key<D>(row)) << 3)];
+DEVINL LaneAddr attn_lane_addr(int lane) {
+  const int half = lane >> 5, col = lane & 31, a = (lane & 15) >> 2;
+  const int c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+  const int hi = D == 128 ? a : a >> 1;
+  LaneAddr x;
+  x.row = col * (2 * D) + ((half ^ attn_key<D>(col)) << 4);
+  x.tr = (4 * half + a) * (2 * D) + (((hi << 2) | (c ^ half)) << 4) +
+         (lane & 1) * 8;
+  return x;
 }
 
-// A operand of img^T: rows of A are columns col0..col0+31 of the image, k
-// runs over image rows row0 + {0-3, 8-11} (lower half) or {4-7, 12-15}.
+typedef __attribute__((address_space(3))) char lds_char;
+
+// A or B operand: rows 0..31 of the image at `row` (bytes, with the lane's
+// own part in it), columns 16 kk on.  `at`: a constant offset.
+DEVINL bf16x8 attn_row_frag(lds_char* sm, unsigned row, int kk, int at) {
+  typedef __attribute__((address_space(3))) const bf16x8 lds8;
+  return *(lds8*)(sm + ((row ^ (kk << 5)) + at));
+}
+
+// A operand of the transposed image: its rows are columns 32 db..32 db + 31
+// of the image, k runs over image rows {0-3, 8-11} (lower half of the wave)
+// or {4-7, 12-15}; `at` adds whole rows.
 template <int D>
-DEVINL bf16x8 attn_tr_frag(const bf16* img, int row0, int col0, int lane) {
-  int c = col0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-  int r = row0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+DEVINL bf16x8 attn_tr_frag(lds_char* sm, unsigned tr, int db, int at) {
   typedef __attribute__((address_space(3))) bf16x4 lds4;
-  auto at = [&](int row) {
-    return (lds4*)((__attribute__((address_space(3))) bf16*)img + row * D +
-                   (((c >> 3) ^ attn_key<D>(row)) << 3) + (c & 7));
-  };
-  bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at(r));
-  bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at(r + 8));
+  bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+      (lds4*)(sm + ((tr ^ (db << 6)) + at)));
+  bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+      (lds4*)(sm + ((tr ^ (db << 6) ^ 32) + at + 16 * D)));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <typename T>
+DEVINL T attn_lds(lds_char* sm, unsigned at) {
+  return *(__attribute__((address_space(3))) const T*)(sm + at);
 }
 
 // A direct copy into LDS: 16 bytes (or 4) a lane, from the lane's address to
@@ -124,23 +151,25 @@ DEVINL void attn_wait_copies() {
 // wait would catch the copies in flight too.
 DEVINL void attn_settle(bf16x8& x) { asm volatile("" : "+v"(x)); }
 
-DEVINL unsigned lds_addr(const void* p) {
-  return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(
-      (const __attribute__((address_space(3))) char*)p));
+// Keeps what is computed from x inside a loop, where it costs one
+// instruction, rather than in registers around it.
+DEVINL unsigned attn_here(unsigned x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // Copies NROW consecutive rows of a head (row0 on) into an image, by NW
-// waves.  Rows at or behind row_end, rows whose id in seg is negative (seg
+// waves; img is the image's LDS address.  Rows at or behind row_end, rows whose id in seg is negative (seg
 // may be null) and chunks at or behind Dact read as zero.
 template <int D, int NROW, int NW>
 DEVINL void attn_stage(const bf16* base, long stride, int row0, int row_end,
-                       int Dact, const int* seg, const bf16* img, int wave,
+                       int Dact, const int* seg, unsigned img, int wave,
                        int lane) {
   constexpr int RPI = 512 / D;  // rows of one instruction
   constexpr int CPR = D / 8;    // chunks of a row
   constexpr int N = NROW / RPI / NW;
   static_assert(N * RPI * NW == NROW, "rows divide among the waves");
-  const unsigned dst = lds_addr(img) + wave * (N * 1024);
+  const unsigned dst = img + wave * (N * 1024);
   const bool clean = row0 + NROW <= row_end && Dact == D && seg == nullptr;
   const int r0 = wave * N * RPI + lane / CPR;
   if (clean) {
@@ -165,10 +194,10 @@ DEVINL void attn_stage(const bf16* base, long stride, int row0, int row_end,
 }
 
 // 64 words into LDS, one instruction of one wave; index clamped to [0, n).
-DEVINL void attn_stage64(const void* base, int first, int n, const void* dst,
+DEVINL void attn_stage64(const void* base, int first, int n, unsigned dst,
                          int lane) {
   int j = min(first + lane, n - 1);
-  copy_lds4((const unsigned int*)base + j, lds_addr(dst));
+  copy_lds4((const unsigned int*)base + j, dst);
 }
 
 DEVINL bf16x8 attn_load_row(const bf16* p, int chunk, int Dact, bool ok) {
@@ -287,7 +316,7 @@ struct TileWalk {
 
 // The spans of a wave's 32 queries (q0 on) and of its block of 128.
 DEVINL void attn_spans(const SeqMask& m, int q0, int Tq, bool qok, int sq,
-                       int4* shared, int wave, int lane, RowSpan& wav,
+                       i32x4* shared, int wave, int lane, RowSpan& wav,
                        RowSpan& blk) {
   wav.pmin = q0 + m.off;
   wav.pmax = min(q0 + 31, Tq - 1) + m.off;
@@ -299,24 +328,25 @@ DEVINL void attn_spans(const SeqMask& m, int q0, int Tq, bool qok, int sq,
     wav.smax = -0x7fffffff - 1;
   }
   if (lane == 0)
-    shared[wave] = make_int4(wav.pmin, wav.pmax, wav.smin, wav.smax);
+    shared[wave] = i32x4{wav.pmin, wav.pmax, wav.smin, wav.smax};
   __syncthreads();
   blk = {q0 - wave * 32 + m.off, wav.pmax, wav.smin, wav.smax};
   for (int w = 0; w < 4; ++w) {
-    int4 s = shared[w];
+    i32x4 s = shared[w];
     blk.pmax = max(blk.pmax, __builtin_amdgcn_readfirstlane(s.y));
     blk.smin = min(blk.smin, __builtin_amdgcn_readfirstlane(s.z));
     blk.smax = max(blk.smax, __builtin_amdgcn_readfirstlane(s.w));
   }
 }
 
-// Masks 16 scores of one query (C order): ids at ksg, first `lim` keys seen.
-DEVINL void attn_mask_keys(float* x, int has_seg, const int* ksg, int sq,
-                           int lim) {
+// Masks 16 scores of one query (C order): ids at LDS address ksg, the first
+// `lim` keys are seen.
+DEVINL void attn_mask_keys(float* x, int has_seg, lds_char* sm, unsigned ksg,
+                           int sq, int lim) {
   if (has_seg) {
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii) {
-      const int4 k4 = *(const int4*)(ksg + 8 * ii);
+      const i32x4 k4 = attn_lds<i32x4>(sm, ksg + 32 * ii);
       x[ii * 4 + 0] = k4.x == sq ? x[ii * 4 + 0] : -MXA_INF;
       x[ii * 4 + 1] = k4.y == sq ? x[ii * 4 + 1] : -MXA_INF;
       x[ii * 4 + 2] = k4.z == sq ? x[ii * 4 + 2] : -MXA_INF;

@@ -19,10 +19,10 @@ namespace mxa {
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   constexpr int KK = D / 16, DB = D / 32;
-  __shared__ __align__(16) bf16 kimg[2][64 * D];
-  __shared__ __align__(16) bf16 vimg[2][64 * D];
-  __shared__ __align__(16) int ksg[2][64];
-  __shared__ int4 spans[4];
+  constexpr int TILE = 128 * D, V0 = 2 * TILE, ID0 = 4 * TILE;
+  __shared__ __align__(1024) char smem[ID0 + 512];
+  lds_char* const sm = (lds_char*)smem;
+  const unsigned lds0 = (unsigned)(size_t)sm;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -42,7 +42,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   if (m.has_seg) sq = qok ? a.seg_q[(long)b * a.Tq + qi] : -1;
 
   RowSpan wav, blk;
-  attn_spans(m, q0, a.Tq, qok, sq, spans, wave, lane, wav, blk);
+  attn_spans(m, q0, a.Tq, qok, sq, (i32x4*)smem, wave, lane, wav, blk);
+  __syncthreads();
   const int limit = m.has_seg && sq < 0 ? 0 : attn_limit(m, pos);
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
@@ -83,18 +84,19 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 
   auto stage = [&](int buf, const Tile& t) {
     const int* sg = t.neg ? skb : nullptr;
-    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg, kimg[buf],
-                         wave, lane);
-    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg, vimg[buf],
-                         wave, lane);
+    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg,
+                         lds0 + buf * TILE, wave, lane);
+    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg,
+                         lds0 + V0 + buf * TILE, wave, lane);
     if (m.has_seg && wave == 0)
-      attn_stage64(skb, t.t * 64, a.Tk, ksg[buf], lane);
+      attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
   };
 
   f32x16 dq[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dq[db] = zero16();
 
+  const LaneAddr la = attn_lane_addr<D>(lane);
   TileWalk walk;
   walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
   Tile cur = walk.next(m, blk, wav, rng, lane);
@@ -106,17 +108,15 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
     Tile nxt = walk.next(m, blk, wav, rng, lane);
     if (nxt.t >= 0) stage(buf ^ 1, nxt);
     if (cur.work) {
+      const unsigned krow = la.row + buf * TILE, ktr = la.tr + buf * TILE;
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) {
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-          s = mfma32(
-              attn_row_frag<D>(kimg[buf], nb * 32 + col, kk * 2 + half),
-              qf[kk], s);
-          dp = mfma32(
-              attn_row_frag<D>(vimg[buf], nb * 32 + col, kk * 2 + half),
-              gf[kk], dp);
+          s = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk], s);
+          dp = mfma32(attn_row_frag(sm, krow, kk, V0 + nb * 64 * D), gf[kk],
+                      dp);
         }
         const int j0 = cur.t * 64 + nb * 32 + 4 * half;
         const float d0 = BIAS ? (float)(pos - j0) : 0.f;
@@ -128,7 +128,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
           if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
         }
         if (!cur.full)
-          attn_mask_keys(x, m.has_seg, &ksg[buf][nb * 32 + 4 * half], sq,
+          attn_mask_keys(x, m.has_seg, sm,
+                         ID0 + buf * 256 + nb * 128 + 16 * half, sq,
                          limit - j0);
         bf16x8 df[2];
 #pragma unroll
@@ -145,9 +146,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int db = 0; db < DB; ++db)
-            dq[db] = mfma32(attn_tr_frag<D>(kimg[buf], nb * 32 + w * 16,
-                                            db * 32, lane),
-                            df[w], dq[db]);
+            dq[db] = mfma32(
+                attn_tr_frag<D>(sm, ktr, db, (nb * 2 + w) * 32 * D), df[w],
+                dq[db]);
       }
     }
     cur = nxt;
@@ -161,29 +162,45 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// dK, dV: block = 128 keys of one key head, wave = 32 keys along the lanes;
-// the queries of every head that shares them pass by in tiles of 64.
+// dK, dV: block = 128 keys of one key head, 32 of them along the lanes of a
+// wave; the queries of every head that shares them pass by in tiles of 64.
+//
+// D = 64: four waves that hold their K and V as operands in registers.
+// D = 128: those 64 registers beside 128 of accumulators would leave room
+// for one wave on a SIMD only, and nothing to overlap its phases with.  K
+// and V lie in LDS instead, and eight waves share the keys: one half takes
+// the first 32 queries of a tile, the other the last, and the two sums meet
+// in LDS at the end.
+//
+// nsplit > 1: a block takes every nsplit-th tile and leaves its sums in the
+// workspace for attn_dkv_join_kernel; for launches too small to fill the
+// chip evenly.
 // ---------------------------------------------------------------------------
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
+__global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
     AttnArgs a) {
-  constexpr int KK = D / 16, DB = D / 32;
-  __shared__ __align__(16) bf16 qimg[2][64 * D];
-  __shared__ __align__(16) bf16 gimg[2][64 * D];
-  __shared__ __align__(16) float lses[2][64];
-  __shared__ __align__(16) float dels[2][64];
-  __shared__ __align__(16) int qsg[2][64];
-  __shared__ int2 spans[4];
+  constexpr bool WIDE = D == 128;
+  constexpr int KK = D / 16, DB = D / 32, NW = WIDE ? 8 : 4;
+  // query and output-gradient tiles, two buffers of each; K and V where
+  // they lie here; log-sums, deltas and ids of the tiles
+  constexpr int TILE = 128 * D, G0 = 2 * TILE, K0 = 4 * TILE;
+  constexpr int V0 = K0 + 256 * D;
+  constexpr int ST0 = WIDE ? V0 + 256 * D : K0;
+  __shared__ __align__(1024) char smem[ST0 + 6 * 256];
+  lds_char* const sm = (lds_char*)smem;
+  const unsigned lds0 = (unsigned)(size_t)sm;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  int bh, kb;  // the first keys are seen by the most queries
-  attn_block(blockIdx.x, a.B * a.Hkv, bh, kb);
+  const int wk = wave & 3;  // this wave's 32 keys
+  int bh, rank;  // the first keys are seen by the most queries
+  attn_block(blockIdx.x, a.B * a.Hkv, bh, rank);
+  const int kb = rank / a.nsplit, split = rank % a.nsplit;
   const int hk = bh % a.Hkv, b = bh / a.Hkv;
   const SeqMask m = attn_seq_mask(a, b);
 
-  const int k0 = kb * 128 + wave * 32;
+  const int k0 = kb * 128 + wk * 32;
   const int kj = k0 + col;
   int sk = 0;
   if (m.has_seg) sk = kj < a.Tk ? a.seg_k[(long)b * a.Tk + kj] : -1;
@@ -195,32 +212,47 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
            : (!m.causal || kj < m.prefix ? -0x7fffffff : kj);
 
   // spans of the wave and the block: smallest `first`, largest, ids
-  int wlo = wave_min(first), whi = wave_max(first);
-  int slo = wave_min(sk), shi = wave_max(sk);
-  if (lane == 0) spans[wave] = make_int2(slo, shi);
-  __shared__ int firsts[4];
-  if (lane == 0) firsts[wave] = wlo;
+  const int wlo = wave_min(first), whi = wave_max(first);
+  const int slo = wave_min(sk), shi = wave_max(sk);
+  i32x4* spans = (i32x4*)smem;
+  if (lane == 0 && wave < 4) spans[wk] = i32x4{wlo, slo, shi, 0};
   __syncthreads();
   int blo = wlo, bslo = slo, bshi = shi;
   for (int w = 0; w < 4; ++w) {
-    blo = min(blo, __builtin_amdgcn_readfirstlane(firsts[w]));
-    bslo = min(bslo, __builtin_amdgcn_readfirstlane(spans[w].x));
-    bshi = max(bshi, __builtin_amdgcn_readfirstlane(spans[w].y));
+    i32x4 sp = spans[w];
+    blo = min(blo, __builtin_amdgcn_readfirstlane(sp.x));
+    bslo = min(bslo, __builtin_amdgcn_readfirstlane(sp.y));
+    bshi = max(bshi, __builtin_amdgcn_readfirstlane(sp.z));
   }
 
-  bf16x8 kf[KK], vf[KK];
+  __syncthreads();
+
+  bf16x8 kf[WIDE ? 1 : KK], vf[WIDE ? 1 : KK];
   {
     const bf16* kp = a.k + b * a.ksb + (long)kj * a.kst + (long)hk * a.D;
     const bf16* vp = a.v + b * a.vsb + (long)kj * a.vst + (long)hk * a.D;
+    if constexpr (WIDE) {
+      // a wave writes the chunks that it would hold, K or V
+      const bool isv = wave >= 4;
+      bf16* img = (bf16*)(smem + (isv ? V0 : K0));
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      kf[kk] = attn_load_q(kp, kk * 2 + half, a.D, kok, a.scale);
-      vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
-    }
+      for (int kk = 0; kk < KK; ++kk) {
+        const int ch = kk * 2 + half, row = wk * 32 + col;
+        bf16x8 x = isv ? attn_load_row(vp, ch, a.D, kok)
+                       : attn_load_q(kp, ch, a.D, kok, a.scale);
+        *(bf16x8*)&img[row * D + ((ch ^ attn_key<D>(row)) << 3)] = x;
+      }
+    } else {
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      attn_settle(kf[kk]);
-      attn_settle(vf[kk]);
+      for (int kk = 0; kk < KK; ++kk) {
+        kf[kk] = attn_load_q(kp, kk * 2 + half, a.D, kok, a.scale);
+        vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
+      }
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        attn_settle(kf[kk]);
+        attn_settle(vf[kk]);
+      }
     }
   }
 
@@ -244,6 +276,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
       wany = wany && max(max(slo, r.x), 0) <= min(shi, r.y);
       all = all && slo == shi && r.x == slo && r.y == slo;
     }
+    any = any && t % a.nsplit == split;
     return (any ? 1 : 0) | (wany ? 2 : 0) | (all ? 4 : 0) |
            (m.has_seg && r.x < 0 ? 8 : 0);
   };
@@ -277,19 +310,20 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
   auto stage = [&](int buf, const QTile& t) {
     const int h = hk * a.G + t.g;
     const int* sg = t.neg ? sqb : nullptr;
-    attn_stage<D, 64, 4>(a.q + b * a.qsb + (long)h * a.D, a.qst, t.t * 64,
-                         a.Tq, a.D, sg, qimg[buf], wave, lane);
-    attn_stage<D, 64, 4>(a.dout + b * a.gsb + (long)h * a.D, a.gst, t.t * 64,
-                         a.Tq, a.D, sg, gimg[buf], wave, lane);
+    attn_stage<D, 64, NW>(a.q + b * a.qsb + (long)h * a.D, a.qst, t.t * 64,
+                          a.Tq, a.D, sg, lds0 + buf * TILE, wave, lane);
+    attn_stage<D, 64, NW>(a.dout + b * a.gsb + (long)h * a.D, a.gst,
+                          t.t * 64, a.Tq, a.D, sg, lds0 + G0 + buf * TILE, wave, lane);
     const long row = ((long)b * a.H + h) * a.TqP;
     if (wave == 0)
-      attn_stage64(a.lse + row, t.t * 64, a.TqP, lses[buf], lane);
+      attn_stage64(a.lse + row, t.t * 64, a.TqP, lds0 + ST0 + buf * 256, lane);
     if (wave == 1)
-      attn_stage64(a.delta + row, t.t * 64, a.TqP, dels[buf], lane);
+      attn_stage64(a.delta + row, t.t * 64, a.TqP, lds0 + ST0 + 512 + buf * 256, lane);
     if (wave == 2 && m.has_seg)
-      attn_stage64(sqb, t.t * 64, a.Tq, qsg[buf], lane);
+      attn_stage64(sqb, t.t * 64, a.Tq, lds0 + ST0 + 1024 + buf * 256, lane);
   };
 
+  const LaneAddr la = attn_lane_addr<D>(lane);
   ScoreFn f;
   QTile cur = next();
   if (cur.g >= 0) stage(0, cur);
@@ -302,56 +336,66 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
     if (cur.work) {
       f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[hk * a.G + cur.g] : 0.f);
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
+      for (int it = 0; it < (WIDE ? 1 : 2); ++it) {
+        const int nb = WIDE ? wave >> 2 : it;  // 32 queries of the tile
+        const unsigned at = buf * TILE + nb * 64 * D;
+        const unsigned qrow = la.row + at, qtr = la.tr + at;
+        const unsigned krow = attn_here(la.row + wk * 64 * D);
+        const unsigned st = ST0 + buf * 256 + nb * 128 + 16 * half;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-          s = mfma32(
-              attn_row_frag<D>(qimg[buf], nb * 32 + col, kk * 2 + half),
-              kf[kk], s);
-          dp = mfma32(
-              attn_row_frag<D>(gimg[buf], nb * 32 + col, kk * 2 + half),
-              vf[kk], dp);
+          bf16x8 kx, vx;
+          if constexpr (WIDE) {
+            kx = attn_row_frag(sm, krow, kk, K0);
+            vx = attn_row_frag(sm, krow, kk, V0);
+          } else {
+            kx = kf[kk];
+            vx = vf[kk];
+          }
+          s = mfma32(attn_row_frag(sm, qrow, kk, 0), kx, s);
+          dp = mfma32(attn_row_frag(sm, qrow, kk, G0), vx, dp);
         }
         const int r0 = nb * 32 + 4 * half;  // this lane's first tile row
         const int p0 = cur.t * 64 + r0 + m.off;
         const float d0 = BIAS ? (float)(p0 - kj) : 0.f;
-        float x[16], u[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int dj = 8 * (i >> 2) + (i & 3);
-          x[i] = attn_score<CAP>(f, s[i], &u[i]);
-          if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 + (float)dj), x[i]);
-        }
-        if (!cur.full) {
-          if (m.has_seg) {
-#pragma unroll
-            for (int ii = 0; ii < 4; ++ii) {
-              const int4 q4 = *(const int4*)&qsg[buf][r0 + 8 * ii];
-              x[ii * 4 + 0] = q4.x == sk ? x[ii * 4 + 0] : -MXA_INF;
-              x[ii * 4 + 1] = q4.y == sk ? x[ii * 4 + 1] : -MXA_INF;
-              x[ii * 4 + 2] = q4.z == sk ? x[ii * 4 + 2] : -MXA_INF;
-              x[ii * 4 + 3] = q4.w == sk ? x[ii * 4 + 3] : -MXA_INF;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[i] = p0 + 8 * (i >> 2) + (i & 3) >= first ? x[i] : -MXA_INF;
-        }
         bf16x8 pf[2], df[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           float p[8], ds[8];
 #pragma unroll
           for (int ii = 0; ii < 2; ++ii) {
-            const f32x4 l4 = *(const f32x4*)&lses[buf][r0 + 8 * (2 * w + ii)];
-            const f32x4 e4 = *(const f32x4*)&dels[buf][r0 + 8 * (2 * w + ii)];
+            const int pr = p0 + 16 * w + 8 * ii;  // of four rows, pr..pr+3
+            const unsigned sr = st + 64 * w + 32 * ii;
+            const f32x4 l4 = attn_lds<f32x4>(sm, sr);
+            const f32x4 e4 = attn_lds<f32x4>(sm, sr + 512);
+            float x[4], u[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int k = 8 * w + 4 * ii + i;
-              p[4 * ii + i] = fexp2(x[k] - l4[i]);
-              ds[4 * ii + i] = p[4 * ii + i] * (dp[k] - e4[i]);
-              if (CAP) ds[4 * ii + i] *= u[k];
+              x[i] = attn_score<CAP>(f, s[8 * w + 4 * ii + i], &u[i]);
+              if (BIAS)
+                x[i] = fmaf(f.slope,
+                            fabsf(d0 + (float)(16 * w + 8 * ii + i)), x[i]);
+            }
+            if (!cur.full) {
+              if (m.has_seg) {
+                const i32x4 q4 = attn_lds<i32x4>(sm, sr + 1024);
+                x[0] = q4.x == sk ? x[0] : -MXA_INF;
+                x[1] = q4.y == sk ? x[1] : -MXA_INF;
+                x[2] = q4.z == sk ? x[2] : -MXA_INF;
+                x[3] = q4.w == sk ? x[3] : -MXA_INF;
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                x[i] = pr + i >= first ? x[i] : -MXA_INF;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float pi = fexp2(x[i] - l4[i]);
+              float di = pi * (dp[8 * w + 4 * ii + i] - e4[i]);
+              if (CAP) di *= u[i];
+              p[4 * ii + i] = pi;
+              ds[4 * ii + i] = di;
             }
           }
           pf[w] = pack8(p);
@@ -361,12 +405,10 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            dv[db] = mfma32(attn_tr_frag<D>(gimg[buf], nb * 32 + w * 16,
-                                            db * 32, lane),
+            dv[db] = mfma32(attn_tr_frag<D>(sm, qtr, db, G0 + w * 32 * D),
                             pf[w], dv[db]);
-            dk[db] = mfma32(attn_tr_frag<D>(qimg[buf], nb * 32 + w * 16,
-                                            db * 32, lane),
-                            df[w], dk[db]);
+            dk[db] = mfma32(attn_tr_frag<D>(sm, qtr, db, w * 32 * D), df[w],
+                            dk[db]);
           }
       }
     }
@@ -374,22 +416,102 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_mod_dkv_kernel(
     buf ^= 1;
   }
 
+  if constexpr (WIDE) {
+    // the second half's sums pass through the query tiles' LDS: 64 KB, dK
+    // and then dV of 128 keys
+    f32x4* box = (f32x4*)smem + (wk * 64 + lane) * 16;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      f32x16* acc = which ? dv : dk;
+      __syncthreads();
+      if (wave >= 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          f32x4 y = {acc[i >> 2][(i & 3) * 4], acc[i >> 2][(i & 3) * 4 + 1],
+                     acc[i >> 2][(i & 3) * 4 + 2],
+                     acc[i >> 2][(i & 3) * 4 + 3]};
+          box[(i + lane) & 15] = y;
+        }
+      }
+      __syncthreads();
+      if (wave < 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          f32x4 y = box[(i + lane) & 15];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i >> 2][(i & 3) * 4 + j] += y[j];
+        }
+      }
+    }
+    if (wave >= 4) return;
+  }
+
   if (kj < a.Tk) {
     const long off = ((long)b * a.Tk + kj) * a.Hkv * a.D + (long)hk * a.D;
-    attn_store_t<DB>(a.dk + off, dk, a.scale, a.D, half);
-    attn_store_t<DB>(a.dv + off, dv, 1.f, a.D, half);
+    if (a.nsplit == 1) {
+      attn_store_t<DB>(a.dk + off, dk, a.scale, a.D, half);
+      attn_store_t<DB>(a.dv + off, dv, 1.f, a.D, half);
+    } else {
+      const long n = (long)a.B * a.Tk * a.Hkv * a.D;
+      float* w = a.ws + (long)split * 2 * n + off;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int ii = 0; ii < 4; ++ii) {
+          const int d = db * 32 + 8 * ii + 4 * half;
+          if (d >= a.D) continue;
+          f32x4 y, z;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[i] = dk[db][ii * 4 + i] * a.scale;
+            z[i] = dv[db][ii * 4 + i];
+          }
+          *(f32x4*)(w + d) = y;
+          *(f32x4*)(w + n + d) = z;
+        }
+    }
   }
+}
+
+// Adds the parts of a split launch in order: n values of dK, then of dV.
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(
+    const float* __restrict__ ws, bf16* __restrict__ dk,
+    bf16* __restrict__ dv, long n, int nsplit) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n / 4;
+       i += (long)gridDim.x * 256) {
+    const long at = i * 8;  // n is a multiple of 8: no group crosses over
+    f32x4 y = {0, 0, 0, 0}, z = {0, 0, 0, 0};
+    for (int s = 0; s < nsplit; ++s) {
+      const float* p = ws + (long)s * 2 * n + at;
+      y += *(const f32x4*)p;
+      z += *(const f32x4*)(p + 4);
+    }
+    float x[8] = {y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
+    bf16* o = at < n ? dk + at : dv + (at - n);
+    *(bf16x8*)o = pack8(x);
+  }
+}
+
+// Blocks of 128 keys are the unit of work and differ a lot under a causal
+// mask.  Fewer than 512 of them leave compute units idle at the end: their
+// queries are divided, as long as a part keeps some 16 tiles.
+int attn_dkv_splits(int B, int Hkv, int G, int Tq, int Tk) {
+  const long base = (long)B * Hkv * cdiv_h(Tk, 128);
+  const long want = (511 + base) / base;
+  const long most = (long)cdiv_h(Tq, 64) * G / 16;
+  const long n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
 }
 
 void attn_mod_bwd(const AttnArgs& a, bool need_kv, hipStream_t s) {
   dim3 gq((unsigned)((long)a.B * a.H * cdiv_h(a.Tq, 128)));
-  dim3 gk((unsigned)((long)a.B * a.Hkv * cdiv_h(a.Tk, 128)));
+  dim3 gk((unsigned)((long)a.B * a.Hkv * cdiv_h(a.Tk, 128) * a.nsplit));
   const bool c = a.cap != 0.f, w = a.slopes != nullptr;
 #define GO(D, C, W)                                 \
   do {                                              \
     attn_mod_dq_kernel<D, C, W><<<gq, 256, 0, s>>>(a);  \
     if (need_kv)                                         \
-      attn_mod_dkv_kernel<D, C, W><<<gk, 256, 0, s>>>(a); \
+      attn_mod_dkv_kernel<D, C, W><<<gk, (D == 64 ? 256 : 512), 0, s>>>(a); \
   } while (0)
 #define PICK(D)                       \
   do {                                \
@@ -408,6 +530,11 @@ void attn_mod_bwd(const AttnArgs& a, bool need_kv, hipStream_t s) {
     PICK(128);
 #undef PICK
 #undef GO
+  if (need_kv && a.nsplit > 1) {
+    const long n = (long)a.B * a.Tk * a.Hkv * a.D;
+    attn_dkv_join_kernel<<<ew_grid(n / 4), 256, 0, s>>>(a.ws, a.dk, a.dv, n,
+                                                        a.nsplit);
+  }
 }
 
 }  // namespace mxa

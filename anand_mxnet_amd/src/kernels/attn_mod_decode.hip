@@ -20,8 +20,12 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
   constexpr int KK = D / 16, DB = D / 32;
   constexpr int NCOPY = 2 * 32 * D / 512;  // copies of one tile, K and V
   // per wave: two buffers of K and V tiles; later the partial outputs
-  __shared__ __align__(16) bf16 img[4][2][2][32 * D];
-  __shared__ float sm[4][32], sl[4][32];
+  constexpr int TILE = 64 * D;
+  __shared__ __align__(1024) char smem[16 * TILE + 1024];
+  lds_char* const sm = (lds_char*)smem;
+  const unsigned lds0 = (unsigned)(size_t)sm;
+  float(*smax)[32] = (float(*)[32])(smem + 16 * TILE);
+  float(*ssum)[32] = smax + 4;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -67,9 +71,9 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
   auto stage = [&](int buf, int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     attn_stage<D, 32, 1>(kb, a.kst, tile * 32, m.kv_len, a.D, nullptr,
-                         img[wave][buf][0], 0, lane);
+                         lds0 + (wave * 4 + buf * 2) * TILE, 0, lane);
     attn_stage<D, 32, 1>(vb, a.vst, tile * 32, m.kv_len, a.D, nullptr,
-                         img[wave][buf][1], 0, lane);
+                         lds0 + (wave * 4 + buf * 2 + 1) * TILE, 0, lane);
   };
 
   f32x16 o[DB];
@@ -77,6 +81,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
   for (int db = 0; db < DB; ++db) o[db] = zero16();
   float mrow = M_INIT, lsum = 0.f;
 
+  const LaneAddr la = attn_lane_addr<D>(lane);
   int buf = 0;
   if (t < t1) stage(0, t);
   for (; t < t1; t += 4, buf ^= 1) {
@@ -86,12 +91,12 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
     } else {
       attn_wait_copies<0>();
     }
-    const bf16* kimg = img[wave][buf][0];
-    const bf16* vimg = img[wave][buf][1];
+    const unsigned at = (wave * 4 + buf * 2) * TILE;
+    const unsigned krow = la.row + at, vtr = la.tr + at;
     f32x16 s = zero16();
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
-      s = mfma32(attn_row_frag<D>(kimg, col, kk * 2 + half), qf[kk], s);
+      s = mfma32(attn_row_frag(sm, krow, kk, 0), qf[kk], s);
     const int j0 = t * 32 + 4 * half;
     const float d0 = BIAS ? (float)(pos - j0) : 0.f;
     float x[16], mx = -MXA_INF;
@@ -102,7 +107,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
       if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
     }
     if (t * 32 + 32 > full_end)
-      attn_mask_keys(x, 0, nullptr, 0, limit - j0);
+      attn_mask_keys(x, 0, sm, 0, 0, limit - j0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -131,15 +136,15 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
     for (int w = 0; w < 2; ++w)
 #pragma unroll
       for (int db = 0; db < DB; ++db)
-        o[db] = mfma32(attn_tr_frag<D>(vimg, w * 16, db * 32, lane), pf[w],
-                       o[db]);
+        o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, TILE + w * 32 * D),
+                       pf[w], o[db]);
   }
   lsum += __shfl_xor(lsum, 32, 64);
 
   // ---- join the four waves ----
   // partial outputs [32][D] fp32 lie over the wave's own buffers, whose
   // reads are done; float4 slots are rotated by the row against conflicts
-  float* po = (float*)img[wave];
+  float* po = (float*)(smem + wave * 4 * TILE);
   __syncthreads();
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -151,8 +156,8 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
       *(f32x4*)&po[col * D + slot * 4] = y;
     }
   if (half == 0) {
-    sm[wave][col] = mrow;
-    sl[wave][col] = lsum;
+    smax[wave][col] = mrow;
+    ssum[wave][col] = lsum;
   }
   __syncthreads();
   const int nrow = min(DEC_ROWS, R - rt * DEC_ROWS);
@@ -161,14 +166,14 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
     const int slot = (d4 + row) & (D / 4 - 1);
     float mm = M_INIT;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][row]);
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, smax[w][row]);
     float l = 0.f;
     f32x4 y = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float e = fexp2(sm[w][row] - mm);
-      l += sl[w][row] * e;
-      y += *(const f32x4*)((const float*)img[w] + row * D + slot * 4) * e;
+      const float e = fexp2(smax[w][row] - mm);
+      l += ssum[w][row] * e;
+      y += *(const f32x4*)((const float*)(smem + w * 4 * TILE) + row * D + slot * 4) * e;
     }
     const int rr = rt * DEC_ROWS + row;
     if (d4 * 4 >= a.D) continue;

@@ -41,10 +41,11 @@ void attn_seg_ranges(const int* seg, int2* out, int B, int T,
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   constexpr int KK = D / 16, DB = D / 32;
-  __shared__ __align__(16) bf16 kimg[2][64 * D];
-  __shared__ __align__(16) bf16 vimg[2][64 * D];
-  __shared__ __align__(16) int ksg[2][64];
-  __shared__ int4 spans[4];
+  // K and V tiles, two buffers of each; then the tiles' ids
+  constexpr int TILE = 128 * D, V0 = 2 * TILE, ID0 = 4 * TILE;
+  __shared__ __align__(1024) char smem[ID0 + 512];
+  lds_char* const sm = (lds_char*)smem;
+  const unsigned lds0 = (unsigned)(size_t)sm;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -64,7 +65,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   if (m.has_seg) sq = qok ? a.seg_q[(long)b * a.Tq + qi] : -1;
 
   RowSpan wav, blk;
-  attn_spans(m, q0, a.Tq, qok, sq, spans, wave, lane, wav, blk);
+  attn_spans(m, q0, a.Tq, qok, sq, (i32x4*)smem, wave, lane, wav, blk);
+  __syncthreads();
   const int limit = m.has_seg && sq < 0 ? 0 : attn_limit(m, pos);
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
@@ -88,12 +90,12 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
 
   auto stage = [&](int buf, const Tile& t) {
     const int* sg = t.neg ? skb : nullptr;
-    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg, kimg[buf],
-                         wave, lane);
-    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg, vimg[buf],
-                         wave, lane);
+    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg,
+                         lds0 + buf * TILE, wave, lane);
+    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg,
+                         lds0 + V0 + buf * TILE, wave, lane);
     if (m.has_seg && wave == 0)
-      attn_stage64(skb, t.t * 64, a.Tk, ksg[buf], lane);
+      attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
   };
 
   f32x16 o[DB];
@@ -101,6 +103,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   for (int db = 0; db < DB; ++db) o[db] = zero16();
   float mrow = M_INIT, lsum = 0.f;
 
+  const LaneAddr la = attn_lane_addr<D>(lane);
   TileWalk walk;
   walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
   Tile cur = walk.next(m, blk, wav, rng, lane);
@@ -112,14 +115,15 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
     Tile nxt = walk.next(m, blk, wav, rng, lane);
     if (nxt.t >= 0) stage(buf ^ 1, nxt);
     if (cur.work) {
+      const unsigned krow = la.row + buf * TILE, vtr = la.tr + buf * TILE;
+      const unsigned ids = ID0 + buf * 256 + 16 * half;
       f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
-          s[nb] = mfma32(
-              attn_row_frag<D>(kimg[buf], nb * 32 + col, kk * 2 + half),
-              qf[kk], s[nb]);
+          s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
+                         s[nb]);
 
       // x[i] + base + (i >> 2) * step is the score.  A distance bias is
       // linear in j where all keys of the tile lie before the wave's
@@ -151,8 +155,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
                      : s[i >> 4][i & 15];
       }
       if (!cur.full) {
-        attn_mask_keys(x, m.has_seg, &ksg[buf][4 * half], sq, limit - j0);
-        attn_mask_keys(x + 16, m.has_seg, &ksg[buf][32 + 4 * half], sq,
+        attn_mask_keys(x, m.has_seg, sm, ids, sq, limit - j0);
+        attn_mask_keys(x + 16, m.has_seg, sm, ids + 128, sq,
                        limit - j0 - 32);
       }
       float mx = -MXA_INF;
@@ -200,9 +204,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
       for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          o[db] = mfma32(
-              attn_tr_frag<D>(vimg[buf], st * 16, db * 32, lane), pf[st],
-              o[db]);
+          o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, V0 + st * 32 * D),
+                         pf[st], o[db]);
     }
     cur = nxt;
     buf ^= 1;

@@ -131,6 +131,14 @@ TRAIN = [
          causal=True),
     dict(B=1, Tq=80, Tk=80, H=2, Hkv=2, D=128, cap=50.0, std=6.0,
          causal=True),
+    # queries divided among blocks in the backward, more than 64 tiles
+    dict(B=1, Tq=1100, Tk=1100, H=2, Hkv=1, D=64, causal=True, docs=3,
+         pad=50, slopes=True),
+    dict(B=1, Tq=1030, Tk=1030, H=4, Hkv=1, D=128, causal=True, cap=10.0,
+         prefix=[300]),
+    dict(B=1, Tq=4200, Tk=70, H=1, Hkv=1, D=64, cap=10.0),
+    dict(B=1, Tq=70, Tk=4200, H=1, Hkv=1, D=128, docs=0, slopes=True,
+         kv_len=[4161]),
 ]
 
 
