@@ -913,9 +913,10 @@ class _FlashMha(torch.autograd.Function):
 
 def _rows16(t):
     """The tensor itself if the kernels can read its rows 16 bytes at a
-    time (any batch and row stride), else a packed copy."""
+    time (any batch stride, rows up to 2**25 elements apart), else a packed
+    copy."""
     if (t.stride(2) == 1 and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0
-            and t.data_ptr() % 16 == 0):
+            and 0 <= t.stride(1) < 1 << 25 and t.data_ptr() % 16 == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

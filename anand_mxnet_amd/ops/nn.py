@@ -496,7 +496,7 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
     cap = 0.0
     if logit_cap is not None:
         cap = float(logit_cap)
-        need(0.0 < cap < float("inf"), "logit_cap must be positive")
+        need(1e-3 <= cap <= 1e3, "logit_cap must lie between 1e-3 and 1e3")
     if slopes is not None:
         need(isinstance(slopes, torch.Tensor)
              and slopes.dtype.is_floating_point
@@ -597,7 +597,8 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
 
     num_kv_heads    heads of k and v, (B, Tk, num_kv_heads*D); each is shared
                     by num_heads / num_kv_heads consecutive query heads
-    logit_cap       s -> cap * tanh(s / cap), on the scaled scores
+    logit_cap       s -> cap * tanh(s / cap), on the scaled scores;
+                    between 1e-3 and 1e3
     distance_slopes (H,) floats: s -> s - slope_h * |P - j|, after the cap
     segment_ids     (B, Tq) integers: a query sees the keys with its own id;
                     negative ids are padding that sees and shows nothing

@@ -1120,7 +1120,8 @@ void attn_operand(const at::Tensor& t, const at::Tensor& like,
               "attention: ", what, " must be a 3-d bfloat16 GPU tensor");
   // rows are read 16 bytes at a time
   TORCH_CHECK((t.size(2) == 1 || t.stride(2) == 1) && t.stride(1) % 8 == 0 &&
-                  t.stride(0) % 8 == 0 && (size_t)t.data_ptr() % 16 == 0,
+                  t.stride(0) % 8 == 0 && (size_t)t.data_ptr() % 16 == 0 &&
+                  t.stride(1) >= 0 && t.stride(1) < (1L << 25),
               "attention: ", what, " must have contiguous, aligned rows");
 }
 

@@ -11,10 +11,13 @@
 //   seg_q[i] == seg_k[j] >= 0            (documents)
 // A query that sees nothing gives a zero row and zero gradients.
 //
-// Scores are held in units of log2 (x = s * log2 e), so that the softmax
-// needs exp2 alone.  tanh(y) = 1 - 2 / (1 + exp(2 y)) costs one exp2 and one
-// reciprocal and saturates by itself: exp2 -> inf gives 1, exp2 -> 0 gives
-// -1.  Its error is about 1e-7 of the cap, 1e-5 in a probability at most.
+// Scores are held in units of log2, x = mu * z + bias, so that the softmax
+// needs exp2 alone and one multiply-add in front of it.  Without a cap z is
+// the product q.k itself.  tanh(y) = 1 - 2 / (1 + exp(2 y)), and a softmax
+// does not see a constant: with a cap z = -1 / (1 + exp(2 y)), mu = 2 cap
+// log2 e.  That is one exp2 and one reciprocal, and saturates by itself:
+// exp2 -> inf gives 0, exp2 -> 0 gives -1.  1 - tanh^2 = -4 (z^2 + z).  The
+// error of z is about 1e-7, 1e-5 in a probability at most.
 //
 // Matrix operands (v_mfma_f32_32x32x16_bf16, wave of 64 lanes, l = lane):
 //   A row  l & 31,  k = 8 (l >> 5) + 0..7
@@ -135,6 +138,14 @@ DEVINL void copy_lds16(const void* g, unsigned dst) {
       : "v"(g), "s"(dst)
       : "memory");
 }
+// the same from base + off
+DEVINL void copy_lds16(const void* base, unsigned off, unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(off), "s"(base), "s"(dst)
+      : "memory");
+}
 DEVINL void copy_lds4(const void* g, unsigned dst) {
   asm volatile(
       "s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
@@ -158,40 +169,51 @@ DEVINL unsigned attn_here(unsigned x) {
   return x;
 }
 
-// Copies NROW consecutive rows of a head (row0 on) into an image, by NW
-// waves; img is the image's LDS address.  Rows at or behind row_end, rows whose id in seg is negative (seg
-// may be null) and chunks at or behind Dact read as zero.
+// Copies NROW consecutive rows of a head into an image, by NW waves, each
+// lane 16 bytes of N instructions.  off holds where its chunks lie behind
+// the first row, so a copy costs no vector arithmetic; rows are less than
+// 2**25 elements apart.
 template <int D, int NROW, int NW>
-DEVINL void attn_stage(const bf16* base, long stride, int row0, int row_end,
-                       int Dact, const int* seg, unsigned img, int wave,
-                       int lane) {
-  constexpr int RPI = 512 / D;  // rows of one instruction
-  constexpr int CPR = D / 8;    // chunks of a row
-  constexpr int N = NROW / RPI / NW;
+struct Stager {
+  static constexpr int RPI = 512 / D;  // rows of one instruction
+  static constexpr int CPR = D / 8;    // chunks of a row
+  static constexpr int N = NROW / RPI / NW;
   static_assert(N * RPI * NW == NROW, "rows divide among the waves");
-  const unsigned dst = img + wave * (N * 1024);
-  const bool clean = row0 + NROW <= row_end && Dact == D && seg == nullptr;
-  const int r0 = wave * N * RPI + lane / CPR;
-  if (clean) {
+  unsigned off[N];
+
+  DEVINL void init(long stride, int wave, int lane) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-      int r = r0 + p * RPI;
-      int ch = (lane % CPR) ^ attn_key<D>(r);
-      copy_lds16(base + (long)(row0 + r) * stride + ch * 8, dst + p * 1024);
-    }
-  } else {
-#pragma unroll
-    for (int p = 0; p < N; ++p) {
-      int r = r0 + p * RPI;
-      int ch = (lane % CPR) ^ attn_key<D>(r);
-      const bf16* g = base + (long)(row0 + r) * stride + ch * 8;
-      bool ok = row0 + r < row_end && ch * 8 < Dact;
-      if (ok && seg) ok = seg[row0 + r] >= 0;
-      if (!ok) g = (const bf16*)attn_zero16;
-      copy_lds16(g, dst + p * 1024);
+      const int r = (wave * N + p) * RPI + lane / CPR;
+      const int ch = (lane % CPR) ^ attn_key<D>(r);
+      off[p] = (unsigned)r * (unsigned)stride * 2u + ch * 16;
     }
   }
-}
+  // Rows row0 on; img is the image's LDS address.  Rows at or behind
+  // row_end, rows whose id in seg is negative (seg may be null) and chunks at
+  // or behind Dact read as zero.
+  DEVINL void copy(const bf16* base, long stride, int row0, int row_end,
+                   int Dact, const int* seg, unsigned img, int wave,
+                   int lane) const {
+    const unsigned dst = img + wave * (N * 1024);
+    const bf16* g0 = base + (long)row0 * stride;
+    if (row0 + NROW <= row_end && Dact == D && seg == nullptr) {
+#pragma unroll
+      for (int p = 0; p < N; ++p) copy_lds16(g0, off[p], dst + p * 1024);
+    } else {
+#pragma unroll
+      for (int p = 0; p < N; ++p) {
+        const int r = (wave * N + p) * RPI + lane / CPR;
+        const int ch = (lane % CPR) ^ attn_key<D>(r);
+        const bf16* g = (const bf16*)((const char*)g0 + off[p]);
+        bool ok = row0 + r < row_end && ch * 8 < Dact;
+        if (ok && seg) ok = seg[row0 + r] >= 0;
+        if (!ok) g = (const bf16*)attn_zero16;
+        copy_lds16(g, dst + p * 1024);
+      }
+    }
+  }
+};
 
 // 64 words into LDS, one instruction of one wave; index clamped to [0, n).
 DEVINL void attn_stage64(const void* base, int first, int n, unsigned dst,
@@ -340,49 +362,59 @@ DEVINL void attn_spans(const SeqMask& m, int q0, int Tq, bool qok, int sq,
 }
 
 // Masks 16 scores of one query (C order): ids at LDS address ksg, the first
-// `lim` keys are seen.
+// `lim` keys are seen.  A masked score becomes `gone`.
 DEVINL void attn_mask_keys(float* x, int has_seg, lds_char* sm, unsigned ksg,
-                           int sq, int lim) {
+                           int sq, int lim, float gone) {
   if (has_seg) {
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii) {
       const i32x4 k4 = attn_lds<i32x4>(sm, ksg + 32 * ii);
-      x[ii * 4 + 0] = k4.x == sq ? x[ii * 4 + 0] : -MXA_INF;
-      x[ii * 4 + 1] = k4.y == sq ? x[ii * 4 + 1] : -MXA_INF;
-      x[ii * 4 + 2] = k4.z == sq ? x[ii * 4 + 2] : -MXA_INF;
-      x[ii * 4 + 3] = k4.w == sq ? x[ii * 4 + 3] : -MXA_INF;
+      x[ii * 4 + 0] = k4.x == sq ? x[ii * 4 + 0] : gone;
+      x[ii * 4 + 1] = k4.y == sq ? x[ii * 4 + 1] : gone;
+      x[ii * 4 + 2] = k4.z == sq ? x[ii * 4 + 2] : gone;
+      x[ii * 4 + 3] = k4.w == sq ? x[ii * 4 + 3] : gone;
     }
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    x[i] = 8 * (i >> 2) + (i & 3) < lim ? x[i] : -MXA_INF;
+    x[i] = 8 * (i >> 2) + (i & 3) < lim ? x[i] : gone;
 }
 
-// Constants of the score function, in units of log2.  The sign of the scale
-// goes to the queries (attn_load_q), c1 is positive.
+// Constants of the score function.  The sign of the scale goes to the
+// queries (attn_load_q): c1 and mu are positive, and z of a masked pair is
+// minus infinity.  A cap between 1e-3 and 1e3 keeps the error of mu z below
+// 3e-4 and mu times attn_gone beyond any exponent.
 struct ScoreFn {
-  float c1, A, slope;
+  float c1, mu, slope;
   template <bool CAP>
   DEVINL void set(float scale, float cap, float slope_) {
     const float sc = scale == 0.f ? 1.f : fabsf(scale);
-    if (CAP) {
-      c1 = sc / cap * 2.f * LOG2E;
-      A = cap * LOG2E;
-    } else {
-      c1 = sc * LOG2E;
-      A = 0.f;
-    }
+    c1 = CAP ? sc / cap * 2.f * LOG2E : 1.f;
+    mu = CAP ? 2.f * cap * LOG2E : sc * LOG2E;
     slope = -slope_ * LOG2E;
   }
 };
 
-// x of one raw product; u is 4 r (1 - r) = 1 - tanh^2 where CAP.
 template <bool CAP>
-DEVINL float attn_score(const ScoreFn& f, float s, float* u = nullptr) {
-  if (!CAP) return s * f.c1;
-  float r = frcp(1.f + fexp2(s * f.c1));
-  if (u) *u = 4.f * (r - r * r);
-  return f.A - (2.f * f.A) * r;
+DEVINL float attn_z(const ScoreFn& f, float s) {
+  return CAP ? frcp(-1.f - fexp2(s * f.c1)) : s;
+}
+
+// (1 - tanh^2) / -4
+DEVINL float attn_dtanh(float z) { return fmaf(z, z, z); }
+
+// A masked z in the backward: its probability is zero like that of minus
+// infinity, and attn_dtanh of it is finite.
+template <bool CAP>
+DEVINL float attn_gone() {
+  return CAP ? -1.0e18f : -MXA_INF;
+}
+
+// What dS is to be multiplied with at the end: the scale, and -4 of the
+// derivative of tanh.
+template <bool CAP>
+DEVINL float attn_ds_scale(float scale) {
+  return CAP ? -4.f * scale : scale;
 }
 
 // Query fragments times the sign of the scale (exact).

@@ -82,12 +82,15 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
   const int2* rng = m.has_seg ? a.rng_k + (long)b * cdiv(a.Tk, 64) : nullptr;
 
+  Stager<D, 64, 4> ks, vs;
+  ks.init(a.kst, wave, lane);
+  vs.init(a.vst, wave, lane);
   auto stage = [&](int buf, const Tile& t) {
     const int* sg = t.neg ? skb : nullptr;
-    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg,
-                         lds0 + buf * TILE, wave, lane);
-    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg,
-                         lds0 + V0 + buf * TILE, wave, lane);
+    const int r = t.t * 64;
+    ks.copy(kb, a.kst, r, m.kv_len, a.D, sg, lds0 + buf * TILE, wave, lane);
+    vs.copy(vb, a.vst, r, m.kv_len, a.D, sg, lds0 + V0 + buf * TILE, wave,
+            lane);
     if (m.has_seg && wave == 0)
       attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
   };
@@ -120,25 +123,24 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
         }
         const int j0 = cur.t * 64 + nb * 32 + 4 * half;
         const float d0 = BIAS ? (float)(pos - j0) : 0.f;
-        float x[16], u[16];
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int dj = 8 * (i >> 2) + (i & 3);
-          x[i] = attn_score<CAP>(f, s[i], &u[i]);
-          if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
-        }
+        for (int i = 0; i < 16; ++i) x[i] = attn_z<CAP>(f, s[i]);
         if (!cur.full)
           attn_mask_keys(x, m.has_seg, sm,
                          ID0 + buf * 256 + nb * 128 + 16 * half, sq,
-                         limit - j0);
+                         limit - j0, attn_gone<CAP>());
         bf16x8 df[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           float ds[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ds[i] = fexp2(x[8 * w + i] - lse) * (dp[8 * w + i] - delta);
-            if (CAP) ds[i] *= u[8 * w + i];
+          for (int k = 0; k < 8; ++k) {
+            const int i = 8 * w + k, dj = 8 * (i >> 2) + (i & 3);
+            const float off =
+                BIAS ? fmaf(f.slope, fabsf(d0 - (float)dj), -lse) : -lse;
+            ds[k] = fexp2(fmaf(x[i], f.mu, off)) * (dp[i] - delta);
+            if (CAP) ds[k] *= attn_dtanh(x[i]);
           }
           df[w] = pack8(ds);
         }
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 
   if (qok) {
     bf16* op = a.dq + ((long)b * a.Tq + qi) * a.H * a.D + (long)h * a.D;
-    attn_store_t<DB>(op, dq, a.scale, a.D, half);
+    attn_store_t<DB>(op, dq, attn_ds_scale<CAP>(a.scale), a.D, half);
   }
 }
 
@@ -307,20 +309,24 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
                  (bool)((wful >> i) & 1), (bool)((neg >> i) & 1)};
   };
 
+  Stager<D, 64, NW> qs, gs;
+  qs.init(a.qst, wave, lane);
+  gs.init(a.gst, wave, lane);
   auto stage = [&](int buf, const QTile& t) {
-    const int h = hk * a.G + t.g;
+    const int h = hk * a.G + t.g, r = t.t * 64;
     const int* sg = t.neg ? sqb : nullptr;
-    attn_stage<D, 64, NW>(a.q + b * a.qsb + (long)h * a.D, a.qst, t.t * 64,
-                          a.Tq, a.D, sg, lds0 + buf * TILE, wave, lane);
-    attn_stage<D, 64, NW>(a.dout + b * a.gsb + (long)h * a.D, a.gst,
-                          t.t * 64, a.Tq, a.D, sg, lds0 + G0 + buf * TILE, wave, lane);
+    qs.copy(a.q + b * a.qsb + (long)h * a.D, a.qst, r, a.Tq, a.D, sg,
+            lds0 + buf * TILE, wave, lane);
+    gs.copy(a.dout + b * a.gsb + (long)h * a.D, a.gst, r, a.Tq, a.D, sg,
+            lds0 + G0 + buf * TILE, wave, lane);
     const long row = ((long)b * a.H + h) * a.TqP;
     if (wave == 0)
-      attn_stage64(a.lse + row, t.t * 64, a.TqP, lds0 + ST0 + buf * 256, lane);
+      attn_stage64(a.lse + row, r, a.TqP, lds0 + ST0 + buf * 256, lane);
     if (wave == 1)
-      attn_stage64(a.delta + row, t.t * 64, a.TqP, lds0 + ST0 + 512 + buf * 256, lane);
+      attn_stage64(a.delta + row, r, a.TqP, lds0 + ST0 + 512 + buf * 256,
+                   lane);
     if (wave == 2 && m.has_seg)
-      attn_stage64(sqb, t.t * 64, a.Tq, lds0 + ST0 + 1024 + buf * 256, lane);
+      attn_stage64(sqb, r, a.Tq, lds0 + ST0 + 1024 + buf * 256, lane);
   };
 
   const LaneAddr la = attn_lane_addr<D>(lane);
@@ -369,31 +375,31 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
             const unsigned sr = st + 64 * w + 32 * ii;
             const f32x4 l4 = attn_lds<f32x4>(sm, sr);
             const f32x4 e4 = attn_lds<f32x4>(sm, sr + 512);
-            float x[4], u[4];
+            float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[i] = attn_score<CAP>(f, s[8 * w + 4 * ii + i], &u[i]);
-              if (BIAS)
-                x[i] = fmaf(f.slope,
-                            fabsf(d0 + (float)(16 * w + 8 * ii + i)), x[i]);
-            }
+            for (int i = 0; i < 4; ++i)
+              x[i] = attn_z<CAP>(f, s[8 * w + 4 * ii + i]);
             if (!cur.full) {
               if (m.has_seg) {
                 const i32x4 q4 = attn_lds<i32x4>(sm, sr + 1024);
-                x[0] = q4.x == sk ? x[0] : -MXA_INF;
-                x[1] = q4.y == sk ? x[1] : -MXA_INF;
-                x[2] = q4.z == sk ? x[2] : -MXA_INF;
-                x[3] = q4.w == sk ? x[3] : -MXA_INF;
+                x[0] = q4.x == sk ? x[0] : attn_gone<CAP>();
+                x[1] = q4.y == sk ? x[1] : attn_gone<CAP>();
+                x[2] = q4.z == sk ? x[2] : attn_gone<CAP>();
+                x[3] = q4.w == sk ? x[3] : attn_gone<CAP>();
               }
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                x[i] = pr + i >= first ? x[i] : -MXA_INF;
+                x[i] = pr + i >= first ? x[i] : attn_gone<CAP>();
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float pi = fexp2(x[i] - l4[i]);
+              const float off =
+                  BIAS ? fmaf(f.slope,
+                              fabsf(d0 + (float)(16 * w + 8 * ii + i)), -l4[i])
+                       : -l4[i];
+              const float pi = fexp2(fmaf(x[i], f.mu, off));
               float di = pi * (dp[8 * w + 4 * ii + i] - e4[i]);
-              if (CAP) di *= u[i];
+              if (CAP) di *= attn_dtanh(x[i]);
               p[4 * ii + i] = pi;
               ds[4 * ii + i] = di;
             }
@@ -449,7 +455,8 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
   if (kj < a.Tk) {
     const long off = ((long)b * a.Tk + kj) * a.Hkv * a.D + (long)hk * a.D;
     if (a.nsplit == 1) {
-      attn_store_t<DB>(a.dk + off, dk, a.scale, a.D, half);
+      attn_store_t<DB>(a.dk + off, dk, attn_ds_scale<CAP>(a.scale), a.D,
+                       half);
       attn_store_t<DB>(a.dv + off, dv, 1.f, a.D, half);
     } else {
       const long n = (long)a.B * a.Tk * a.Hkv * a.D;
@@ -463,7 +470,7 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
           f32x4 y, z;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            y[i] = dk[db][ii * 4 + i] * a.scale;
+            y[i] = dk[db][ii * 4 + i] * attn_ds_scale<CAP>(a.scale);
             z[i] = dv[db][ii * 4 + i];
           }
           *(f32x4*)(w + d) = y;

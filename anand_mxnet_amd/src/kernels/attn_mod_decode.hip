@@ -68,12 +68,14 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
 
   const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
   const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
+  Stager<D, 32, 1> ks, vs;
+  ks.init(a.kst, 0, lane);
+  vs.init(a.vst, 0, lane);
   auto stage = [&](int buf, int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    attn_stage<D, 32, 1>(kb, a.kst, tile * 32, m.kv_len, a.D, nullptr,
-                         lds0 + (wave * 4 + buf * 2) * TILE, 0, lane);
-    attn_stage<D, 32, 1>(vb, a.vst, tile * 32, m.kv_len, a.D, nullptr,
-                         lds0 + (wave * 4 + buf * 2 + 1) * TILE, 0, lane);
+    const unsigned at = lds0 + (wave * 4 + buf * 2) * TILE;
+    ks.copy(kb, a.kst, tile * 32, m.kv_len, a.D, nullptr, at, 0, lane);
+    vs.copy(vb, a.vst, tile * 32, m.kv_len, a.D, nullptr, at + TILE, 0, lane);
   };
 
   f32x16 o[DB];
@@ -101,15 +103,16 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
     const float d0 = BIAS ? (float)(pos - j0) : 0.f;
     float x[16], mx = -MXA_INF;
 #pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = attn_z<CAP>(f, s[i]);
+    if (t * 32 + 32 > full_end)
+      attn_mask_keys(x, 0, sm, 0, 0, limit - j0, -MXA_INF);
+#pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int dj = 8 * (i >> 2) + (i & 3);
-      x[i] = attn_score<CAP>(f, s[i]);
+      x[i] *= f.mu;
       if (BIAS) x[i] = fmaf(f.slope, fabsf(d0 - (float)dj), x[i]);
+      mx = fmaxf(mx, x[i]);
     }
-    if (t * 32 + 32 > full_end)
-      attn_mask_keys(x, 0, sm, 0, 0, limit - j0);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     if (__ballot(mx > mrow + 8.f)) {
       float mnew = fmaxf(mrow, mx);

@@ -88,12 +88,15 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   const int ntk = cdiv(a.Tk, 64);
   const int2* rng = m.has_seg ? a.rng_k + (long)b * ntk : nullptr;
 
+  Stager<D, 64, 4> ks, vs;
+  ks.init(a.kst, wave, lane);
+  vs.init(a.vst, wave, lane);
   auto stage = [&](int buf, const Tile& t) {
     const int* sg = t.neg ? skb : nullptr;
-    attn_stage<D, 64, 4>(kb, a.kst, t.t * 64, m.kv_len, a.D, sg,
-                         lds0 + buf * TILE, wave, lane);
-    attn_stage<D, 64, 4>(vb, a.vst, t.t * 64, m.kv_len, a.D, sg,
-                         lds0 + V0 + buf * TILE, wave, lane);
+    const int r = t.t * 64;
+    ks.copy(kb, a.kst, r, m.kv_len, a.D, sg, lds0 + buf * TILE, wave, lane);
+    vs.copy(vb, a.vst, r, m.kv_len, a.D, sg, lds0 + V0 + buf * TILE, wave,
+            lane);
     if (m.has_seg && wave == 0)
       attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
   };
@@ -125,11 +128,20 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
           s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
                          s[nb]);
 
-      // x[i] + base + (i >> 2) * step is the score.  A distance bias is
-      // linear in j where all keys of the tile lie before the wave's
-      // queries: it costs one addition for each four keys there.
       const int j0 = cur.t * 64 + 4 * half;
-      float x[32], base = 0.f, step = 0.f;
+      float x[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        x[i] = attn_z<CAP>(f, s[i >> 4][i & 15]);
+      if (!cur.full) {
+        attn_mask_keys(x, m.has_seg, sm, ids, sq, limit - j0, -MXA_INF);
+        attn_mask_keys(x + 16, m.has_seg, sm, ids + 128, sq, limit - j0 - 32,
+                       -MXA_INF);
+      }
+      // with a bias, x[i] + base + (i >> 2) * step becomes the score.  The
+      // bias is linear in j where all keys of the tile lie before the wave's
+      // queries: one addition for each four keys there.
+      float mx = -MXA_INF, base = 0.f, step = 0.f;
       if (BIAS) {
         const float d0 = (float)(pos - j0);
         if (cur.t * 64 + 63 <= wav.pmin) {
@@ -137,30 +149,14 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
           step = -8.f * f.slope;
           const float e[4] = {0.f, -f.slope, -2.f * f.slope, -3.f * f.slope};
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            x[i] = CAP ? attn_score<CAP>(f, s[i >> 4][i & 15]) + e[i & 3]
-                       : fmaf(s[i >> 4][i & 15], f.c1, e[i & 3]);
+          for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], f.mu, e[i & 3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            x[i] = fmaf(f.slope,
-                        fabsf(d0 - (float)(8 * (i >> 2) + (i & 3))),
-                        attn_score<CAP>(f, s[i >> 4][i & 15]));
+            x[i] = fmaf(x[i], f.mu,
+                        f.slope *
+                            fabsf(d0 - (float)(8 * (i >> 2) + (i & 3))));
         }
-      } else {
-        // without a cap the scores stay unscaled, exp2 scales them
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          x[i] = CAP ? attn_score<CAP>(f, s[i >> 4][i & 15])
-                     : s[i >> 4][i & 15];
-      }
-      if (!cur.full) {
-        attn_mask_keys(x, m.has_seg, sm, ids, sq, limit - j0);
-        attn_mask_keys(x + 16, m.has_seg, sm, ids + 128, sq,
-                       limit - j0 - 32);
-      }
-      float mx = -MXA_INF;
-      if (BIAS) {
 #pragma unroll
         for (int g = 0; g < 8; ++g)
           mx = fmaxf(mx, fmaf((float)g, step,
@@ -170,7 +166,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
-        if (!CAP) mx *= f.c1;
+        mx *= f.mu;
       }
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       if (__ballot(mx > mrow + 8.f)) {
@@ -190,12 +186,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int g = 2 * st + (i >> 2);
-          if (BIAS)
-            p[i] = fexp2(x[8 * st + i] - (mrow - base - (float)g * step));
-          else if (CAP)
-            p[i] = fexp2(x[8 * st + i] - mrow);
-          else
-            p[i] = fexp2(fmaf(x[8 * st + i], f.c1, -mrow));
+          p[i] = BIAS ? fexp2(x[8 * st + i] - (mrow - base - (float)g * step))
+                      : fexp2(fmaf(x[8 * st + i], f.mu, -mrow));
           lsum += p[i];
         }
         pf[st] = pack8(p);
