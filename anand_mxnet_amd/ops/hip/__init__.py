@@ -795,17 +795,7 @@ def multi_sumsq(blob, ntens, nchunks, bf16in):
 def multi_clip_global_norm(arrays, max_norm, out):
     """One norm over all arrays and their clipping (clip_norm.hip); the
     factor stays on the device."""
-    if all(t.is_contiguous() for t in arrays) and (
-            out is arrays or all(t.is_contiguous() for t in out)):
-        return _C.clip_global_norm(arrays, out, max_norm)
-    src = [t.contiguous() for t in arrays]
-    dst = [s if o is a else o if o.is_contiguous() else torch.empty_like(s)
-           for a, s, o in zip(arrays, src, out)]
-    norm = _C.clip_global_norm(src, dst, max_norm)
-    for o, d in zip(out, dst):
-        if o is not d:
-            o.copy_(d)
-    return norm
+    return _C.clip_global_norm(arrays, out, max_norm)
 
 
 # ---------------------------------------------------------------------------

@@ -454,11 +454,11 @@ class _ScaledLookup(torch.autograd.Function):
 def _attn_ints(x, shape, what, q):
     """An optional integer tensor of the given shape, as int32 on q's
     device."""
-    from ..base import MXNetError
     if x is None:
         return None
+    from ..base import MXNetError
     if not isinstance(x, torch.Tensor) or x.dtype.is_floating_point \
-            or x.dtype in (torch.bool, torch.complex64):
+            or x.dtype.is_complex or x.dtype == torch.bool:
         raise MXNetError(f"multi_head_attention: {what} must be an integer "
                          f"array")
     if tuple(x.shape) != shape:
@@ -473,62 +473,70 @@ def _attn_ints(x, shape, what, q):
 def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
                 causal, seg_q, seg_k, prefix, kv_len, q_off):
     """Checks and dispatch of the shaped forms of multi_head_attention."""
-    from ..base import MXNetError
+    def bad(what):
+        from ..base import MXNetError
+        raise MXNetError("multi_head_attention: " + what)
 
-    def need(ok, what):
-        if not ok:
-            raise MXNetError("multi_head_attention: " + what)
-
-    need(q.dim() == 3 and k.dim() == 3 and v.dim() == 3,
-         "query, key and value must be (batch, tokens, heads * size)")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        bad("query, key and value must be (batch, tokens, heads * size)")
     B, Tq, HD = q.shape
-    Tk = k.shape[1]
+    Bk, Tk, KD = k.shape
     H, Hkv = int(num_heads), int(num_kv_heads or num_heads)
-    need(H > 0 and HD % H == 0, f"{HD} columns do not divide into {H} heads")
-    need(Hkv > 0 and H % Hkv == 0,
-         f"{H} heads cannot share {Hkv} key heads")
+    if H <= 0 or HD % H:
+        bad(f"{HD} columns do not divide into {H} heads")
+    if Hkv <= 0 or H % Hkv:
+        bad(f"{H} heads cannot share {Hkv} key heads")
     D = HD // H
-    need(k.shape[0] == B and k.shape[2] == Hkv * D and v.shape == k.shape,
-         f"key and value must be ({B}, tokens, {Hkv * D}), got "
-         f"{tuple(k.shape)} and {tuple(v.shape)}")
-    need(q.dtype == k.dtype == v.dtype and q.device == k.device == v.device,
-         "query, key and value must agree in type and device")
+    if Bk != B or KD != Hkv * D or v.shape != k.shape:
+        bad(f"key and value must be ({B}, tokens, {Hkv * D}), got "
+            f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype
+            and q.device == k.device == v.device):
+        bad("query, key and value must agree in type and device")
     cap = 0.0
     if logit_cap is not None:
         cap = float(logit_cap)
-        need(1e-3 <= cap <= 1e3, "logit_cap must lie between 1e-3 and 1e3")
+        if not 1e-3 <= cap <= 1e3:
+            bad("logit_cap must lie between 1e-3 and 1e3")
     if slopes is not None:
-        need(isinstance(slopes, torch.Tensor)
-             and slopes.dtype.is_floating_point
-             and tuple(slopes.shape) == (H,) and slopes.device == q.device,
-             f"distance_slopes must be {H} floats on the queries' device")
-        need(not slopes.requires_grad,
-             "distance_slopes are constants, they get no gradient")
+        if not (isinstance(slopes, torch.Tensor)
+                and slopes.dtype.is_floating_point
+                and tuple(slopes.shape) == (H,)
+                and slopes.device == q.device):
+            bad(f"distance_slopes must be {H} floats on the queries' device")
+        if slopes.requires_grad:
+            bad("distance_slopes are constants, they get no gradient")
         slopes = slopes.float().contiguous()
     if seg_q is None:
-        need(seg_k is None, "kv_segment_ids without segment_ids")
-    elif seg_k is None:
-        need(Tq == Tk, "segment_ids of other tokens than the keys': "
-                       "kv_segment_ids is needed too")
-        seg_k = seg_q
-    same = seg_k is seg_q
-    seg_q = _attn_ints(seg_q, (B, Tq), "segment_ids", q)
-    seg_k = seg_q if same else _attn_ints(seg_k, (B, Tk), "kv_segment_ids",
-                                          q)
-    need(prefix is None or causal, "prefix_length opens a causal mask; "
-                                   "without causal=True it has no meaning")
+        if seg_k is not None:
+            bad("kv_segment_ids without segment_ids")
+    else:
+        if seg_k is None:
+            if Tq != Tk:
+                bad("segment_ids of other tokens than the keys': "
+                    "kv_segment_ids is needed too")
+            seg_k = seg_q
+        same = seg_k is seg_q
+        seg_q = _attn_ints(seg_q, (B, Tq), "segment_ids", q)
+        seg_k = seg_q if same else _attn_ints(seg_k, (B, Tk),
+                                              "kv_segment_ids", q)
+    if prefix is not None and not causal:
+        bad("prefix_length opens a causal mask; without causal=True it has "
+            "no meaning")
     prefix = _attn_ints(prefix, (B,), "prefix_length", q)
     kv_len = _attn_ints(kv_len, (B,), "kv_length", q)
     off0 = 0
     if q_off is not None and not isinstance(q_off, torch.Tensor):
         off0, q_off = int(q_off), None
-        need(abs(off0) < 1 << 30, "query_offset is out of range")
+        if abs(off0) >= 1 << 30:
+            bad("query_offset is out of range")
     q_off = _attn_ints(q_off, (B,), "query_offset", q)
     args = (H, Hkv, float(scale if scale is not None else D ** -0.5), cap,
             bool(causal), slopes, seg_q, seg_k, prefix, kv_len, q_off, off0)
     if _use_hip(q, "shaped_mha", _BF16):
-        need(D % 8 == 0 and D <= 128, f"heads of {D} columns: the kernels "
-                                      "take multiples of 8 up to 128")
+        if D % 8 or D > 128:
+            bad(f"heads of {D} columns: the kernels take multiples of 8 up "
+                "to 128")
         return gpu_impl("shaped_mha")(q, k, v, *args)
     return _shaped_mha_oracle(q, k, v, *args)
 

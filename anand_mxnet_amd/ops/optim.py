@@ -224,15 +224,19 @@ def multi_clip_global_norm(arrays, max_norm, out=None):
     need(isinstance(out, (list, tuple)) and len(out) == len(arrays),
          "one output for each array is needed")
     with torch.no_grad():
-        if arrays[0].is_cuda and all(t.is_contiguous() for t in arrays) \
-                and all(t.is_contiguous() for t in out):
-            try:  # the extension checks the rest: many arrays, little time
+        if arrays[0].is_cuda:
+            # the extension checks the rest: many arrays, little time
+            try:
                 return gpu_impl("multi_clip_global_norm")(arrays, max_norm,
                                                           out)
-            except RuntimeError as e:
-                if "clip_global_norm: " not in str(e):
-                    raise
-                raise MXNetError("multi_" + str(e).splitlines()[0]) from None
+            except (RuntimeError, TypeError) as e:
+                if "not contiguous" not in str(e):
+                    if isinstance(e, RuntimeError) \
+                            and "clip_global_norm: " not in str(e):
+                        raise
+                    raise MXNetError("multi_clip_global_norm: "
+                                     + str(e).split("norm: ")[-1]
+                                     .splitlines()[0]) from None
         for a, o in zip(arrays, out):
             need(isinstance(a, torch.Tensor) and a.dtype.is_floating_point
                  and a.device == arrays[0].device,
@@ -245,7 +249,14 @@ def multi_clip_global_norm(arrays, max_norm, out=None):
             need(all(a.dtype in (torch.bfloat16, torch.float16,
                                  torch.float32) for a in arrays),
                  "the kernels take bfloat16, float16 and float32")
-            return gpu_impl("multi_clip_global_norm")(arrays, max_norm, out)
+            src = [a.contiguous() for a in arrays]
+            dst = [o if o.is_contiguous() else torch.empty_like(s)
+                   for s, o in zip(src, out)]
+            norm = gpu_impl("multi_clip_global_norm")(src, max_norm, dst)
+            for o, d in zip(out, dst):
+                if o is not d:
+                    o.copy_(d)
+            return norm
         src = [a.detach() for a in arrays]
         dst = [o.detach() for o in out]
         total = sum(a.double().square().sum() for a in src)

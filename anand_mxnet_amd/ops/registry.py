@@ -24,18 +24,25 @@ RAW = {}
 GPU_IMPL = {}
 
 
+_NDArray = None  # filled at the first call: ndarray imports this module
+
+
 def _unwrap(x):
-    from ..ndarray.ndarray import NDArray
-    if isinstance(x, NDArray):
+    global _NDArray
+    if _NDArray is None:
+        from ..ndarray.ndarray import NDArray
+        _NDArray = NDArray
+    if isinstance(x, _NDArray):
         return x._t
     if isinstance(x, (list, tuple)):
-        return type(x)(_unwrap(v) for v in x)
+        return type(x)([v._t if isinstance(v, _NDArray) else _unwrap(v)
+                        for v in x])
     return x
 
 
 def _wrap_out(out):
-    from ..ndarray.ndarray import NDArray
     if isinstance(out, torch.Tensor):
+        from ..ndarray.ndarray import NDArray
         return NDArray(out)
     if isinstance(out, (list, tuple)):
         return [_wrap_out(o) for o in out]

@@ -1523,6 +1523,7 @@ at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
     bool write;
   };
   std::vector<Span> spans;
+  spans.reserve(2 * src.size());
   std::vector<const void*> sp;
   std::vector<void*> dp;
   std::vector<long> n;
@@ -1531,10 +1532,11 @@ at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
     TORCH_CHECK(src[i].is_cuda() && src[i].device() == dev &&
                     dst[i].device() == dev,
                 "clip_global_norm: arrays on different devices");
-    TORCH_CHECK(src[i].is_contiguous() && dst[i].is_contiguous() &&
-                    src[i].sizes() == dst[i].sizes() &&
+    TORCH_CHECK(src[i].sizes() == dst[i].sizes() &&
                     src[i].scalar_type() == dst[i].scalar_type(),
                 "clip_global_norm: an output is unlike its array");
+    TORCH_CHECK(src[i].is_contiguous() && dst[i].is_contiguous(),
+                "clip_global_norm: an array is not contiguous");
     const int code = float_code(src[i], "clip_global_norm");
     if (src[i].numel() == 0) continue;
     const size_t a = (size_t)src[i].data_ptr(),

@@ -38,6 +38,29 @@ void attn_seg_ranges(const int* seg, int2* out, int B, int T,
       seg, out, T, nt, total);
 }
 
+#ifndef QKL
+#define QKL 4
+#endif
+#define SCHED_QK \
+  __builtin_amdgcn_sched_group_barrier(0x100, QKL, 0); \
+  _Pragma("unroll") for (int i = 0; i < KK - QKL / 2; ++i) { \
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); \
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); \
+  } \
+  __builtin_amdgcn_sched_group_barrier(0x008, QKL, 0);
+#ifdef PVS
+#define SCHED_PV \
+  __builtin_amdgcn_sched_group_barrier(0x100, 2*DB, 0); \
+  __builtin_amdgcn_sched_group_barrier(0x002, 24, 0); \
+  _Pragma("unroll") for (int i = 0; i < 3 * DB; ++i) { \
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); \
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); \
+    __builtin_amdgcn_sched_group_barrier(0x002, 24 / DB, 0); \
+  } \
+  __builtin_amdgcn_sched_group_barrier(0x008, DB, 0);
+#else
+#define SCHED_PV
+#endif
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   constexpr int KK = D / 16, DB = D / 32;
@@ -127,6 +150,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
         for (int nb = 0; nb < 2; ++nb)
           s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
                          s[nb]);
+      SCHED_QK
 
       const int j0 = cur.t * 64 + 4 * half;
       float x[32];
@@ -198,6 +222,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
         for (int db = 0; db < DB; ++db)
           o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, V0 + st * 32 * D),
                          pf[st], o[db]);
+      SCHED_PV
     }
     cur = nxt;
     buf ^= 1;
