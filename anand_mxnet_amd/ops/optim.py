@@ -206,7 +206,7 @@ def multi_clip_global_norm(arrays, max_norm, out=None):
 
     Squares are summed in 64 bits.  A NaN norm leaves the values as they
     are.  GPU: bfloat16, float16 and float32, mixed as they come, two kernels
-    (clip_norm.hip) for up to 140 arrays.  An array that is written must not
+    (clip_norm.hip) for up to 164 arrays.  An array that is written must not
     overlap another one."""
     from ..base import MXNetError
 

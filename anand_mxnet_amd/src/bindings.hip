@@ -108,6 +108,7 @@ int emb_chunks(long);
 void emb_grad(int, bool, bool, const void*, const void*, void*, int*, int2*,
               float*, int, int, int, float, hipStream_t);
 // clip_norm.hip
+long clip_entries(long);
 long clip_ws(long);
 void clip_norm(const void* const*, void* const*, const long*, const int*,
                long, double, double*, float*, hipStream_t);
@@ -1541,10 +1542,17 @@ at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
     if (src[i].numel() == 0) continue;
     const size_t a = (size_t)src[i].data_ptr(),
                  b = (size_t)dst[i].data_ptr(), len = src[i].nbytes();
-    sp.push_back((const void*)a);
-    dp.push_back((void*)b);
-    n.push_back(src[i].numel());
-    dt.push_back(code);
+    // an entry counts elements in 32 bits: longer arrays take several
+    const long parts = mxa::clip_entries(src[i].numel());
+    for (long p = 0; p < parts; ++p) {
+      const long per = (src[i].numel() + parts - 1) / parts + 63 & ~63l;
+      const long e0 = p * per, e1 = std::min(e0 + per, src[i].numel());
+      if (e0 >= e1) break;
+      sp.push_back((const char*)a + e0 * src[i].element_size());
+      dp.push_back((char*)b + e0 * src[i].element_size());
+      n.push_back(e1 - e0);
+      dt.push_back(code);
+    }
     if (a != b) spans.push_back({a, a + len, false});
     spans.push_back({b, b + len, true});
   }

@@ -135,7 +135,7 @@ DEVINL void copy_lds16(const void* g, unsigned dst) {
   asm volatile(
       "s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
       :
-      : "v"(g), "s"(dst)
+      : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory");
 }
 // the same from base + off
@@ -143,14 +143,14 @@ DEVINL void copy_lds16(const void* base, unsigned off, unsigned dst) {
   asm volatile(
       "s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
       :
-      : "v"(off), "s"(base), "s"(dst)
+      : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory");
 }
 DEVINL void copy_lds4(const void* g, unsigned dst) {
   asm volatile(
       "s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
       :
-      : "v"(g), "s"(dst)
+      : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory");
 }
 // All but the last N copies have landed.
@@ -167,6 +167,14 @@ DEVINL void attn_settle(bf16x8& x) { asm volatile("" : "+v"(x)); }
 DEVINL unsigned attn_here(unsigned x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// A pointer that is the same in all lanes, where the compiler knows it.
+DEVINL const bf16* uniform_ptr(const bf16* p) {
+  const size_t x = (size_t)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(x >> 32));
+  return (const bf16*)((size_t)hi << 32 | lo);
 }
 
 // Copies NROW consecutive rows of a head into an image, by NW waves, each
@@ -196,7 +204,7 @@ struct Stager {
                    int Dact, const int* seg, unsigned img, int wave,
                    int lane) const {
     const unsigned dst = img + wave * (N * 1024);
-    const bf16* g0 = base + (long)row0 * stride;
+    const bf16* g0 = uniform_ptr(base + (long)row0 * stride);
     if (row0 + NROW <= row_end && Dact == D && seg == nullptr) {
 #pragma unroll
       for (int p = 0; p < N; ++p) copy_lds16(g0, off[p], dst + p * 1024);

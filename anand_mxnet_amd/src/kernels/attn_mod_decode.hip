@@ -5,9 +5,10 @@
 // head form the 32 columns of one product (row r = token r / G, head r % G),
 // so a shared cache is read once for its whole group.  The keys of a
 // sequence are divided among `nsplit` blocks and, tile by tile of 32, among
-// the four waves of a block; a wave streams its tiles through LDS buffers of
-// its own with counted waits and no barriers.  Partial softmaxes are joined
-// in LDS, then (nsplit > 1) by a second kernel, in a fixed order.
+// the four waves of a block; a wave streams its tiles through LDS of its own
+// with counted waits and no barriers: the next K is on its way while this
+// tile's V is used, and the other way round.  Partial softmaxes are joined in
+// LDS, then (nsplit > 1) by a second kernel, in a fixed order.
 #include "attn_mod.h"
 
 namespace mxa {
@@ -15,16 +16,16 @@ namespace mxa {
 constexpr int DEC_ROWS = 32;
 
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
+__global__ __launch_bounds__(256, 2) void attn_decode_kernel(
     AttnArgs a) {
   constexpr int KK = D / 16, DB = D / 32;
-  constexpr int NCOPY = 2 * 32 * D / 512;  // copies of one tile, K and V
-  // per wave: two buffers of K and V tiles; later the partial outputs
+  constexpr int NCOPY = 32 * D / 512;  // copies of one tile
+  // per wave: a K and a V tile; later the partial outputs
   constexpr int TILE = 64 * D;
-  __shared__ __align__(1024) char smem[16 * TILE + 1024];
+  __shared__ __align__(1024) char smem[8 * TILE + 1024];
   lds_char* const sm = (lds_char*)smem;
   const unsigned lds0 = (unsigned)(size_t)sm;
-  float(*smax)[32] = (float(*)[32])(smem + 16 * TILE);
+  float(*smax)[32] = (float(*)[32])(smem + 8 * TILE);
   float(*ssum)[32] = smax + 4;
 
   const int lane = threadIdx.x & 63;
@@ -71,11 +72,17 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
   Stager<D, 32, 1> ks, vs;
   ks.init(a.kst, 0, lane);
   vs.init(a.vst, 0, lane);
-  auto stage = [&](int buf, int tile) {
+  const unsigned kat = wave * 2 * TILE, vat = kat + TILE;
+  // the wave's own reads of a tile end before the next one is copied over it
+  auto stage_k = [&](int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const unsigned at = lds0 + (wave * 4 + buf * 2) * TILE;
-    ks.copy(kb, a.kst, tile * 32, m.kv_len, a.D, nullptr, at, 0, lane);
-    vs.copy(vb, a.vst, tile * 32, m.kv_len, a.D, nullptr, at + TILE, 0, lane);
+    ks.copy(kb, a.kst, tile * 32, m.kv_len, a.D, nullptr, lds0 + kat, 0,
+            lane);
+  };
+  auto stage_v = [&](int tile) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    vs.copy(vb, a.vst, tile * 32, m.kv_len, a.D, nullptr, lds0 + vat, 0,
+            lane);
   };
 
   f32x16 o[DB];
@@ -84,21 +91,19 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
   float mrow = M_INIT, lsum = 0.f;
 
   const LaneAddr la = attn_lane_addr<D>(lane);
-  int buf = 0;
-  if (t < t1) stage(0, t);
-  for (; t < t1; t += 4, buf ^= 1) {
-    if (t + 4 < t1) {
-      stage(buf ^ 1, t + 4);
-      attn_wait_copies<NCOPY>();
-    } else {
-      attn_wait_copies<0>();
-    }
-    const unsigned at = (wave * 4 + buf * 2) * TILE;
-    const unsigned krow = la.row + at, vtr = la.tr + at;
+  const unsigned krow = la.row + kat, vtr = la.tr + vat;
+  if (t < t1) {
+    stage_k(t);
+    stage_v(t);
+  }
+  for (; t < t1; t += 4) {
+    const bool more = t + 4 < t1;
+    attn_wait_copies<NCOPY>();  // K is there, V may be on its way
     f32x16 s = zero16();
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
       s = mfma32(attn_row_frag(sm, krow, kk, 0), qf[kk], s);
+    if (more) stage_k(t + 4);
     const int j0 = t * 32 + 4 * half;
     const float d0 = BIAS ? (float)(pos - j0) : 0.f;
     float x[16], mx = -MXA_INF;
@@ -135,19 +140,24 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
       }
       pf[w] = pack8(p);
     }
+    if (more)
+      attn_wait_copies<NCOPY>();
+    else
+      attn_wait_copies<0>();
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll
       for (int db = 0; db < DB; ++db)
-        o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, TILE + w * 32 * D),
-                       pf[w], o[db]);
+        o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, w * 32 * D), pf[w],
+                       o[db]);
+    if (more) stage_v(t + 4);
   }
   lsum += __shfl_xor(lsum, 32, 64);
 
   // ---- join the four waves ----
-  // partial outputs [32][D] fp32 lie over the wave's own buffers, whose
-  // reads are done; float4 slots are rotated by the row against conflicts
-  float* po = (float*)(smem + wave * 4 * TILE);
+  // partial outputs [32][D] fp32 lie over the wave's own tiles, whose reads
+  // are done; float4 slots are rotated by the row against conflicts
+  float* po = (float*)(smem + kat);
   __syncthreads();
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -176,7 +186,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
     for (int w = 0; w < 4; ++w) {
       const float e = fexp2(smax[w][row] - mm);
       l += ssum[w][row] * e;
-      y += *(const f32x4*)((const float*)(smem + w * 4 * TILE) + row * D + slot * 4) * e;
+      y += *(const f32x4*)((const float*)(smem + w * 2 * TILE) + row * D + slot * 4) * e;
     }
     const int rr = rt * DEC_ROWS + row;
     if (d4 * 4 >= a.D) continue;
@@ -200,10 +210,12 @@ __global__ __launch_bounds__(256, (D == 64 ? 2 : 1)) void attn_decode_kernel(
   }
 }
 
-// Joins the blocks of one row: a wave per row, D / 4 lanes hold the row.
+// Joins the blocks of one row: a wave per row.  Lane s holds the weight of
+// split s (64 at a time); the two halves of the wave add the even and the odd
+// splits, four columns a lane.
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   const int R = a.Tq * a.G;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
   const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (long)a.B * a.Hkv * R) return;
   const int rr = (int)(row % R);
@@ -214,20 +226,37 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   const long i0 = bh * a.nsplit * R + rr;
 
   float mm = M_INIT;
-  for (int s = 0; s < a.nsplit; ++s)
+  for (int s = lane; s < a.nsplit; s += 64)
     mm = fmaxf(mm, wm[(i0 + (long)s * R) * 2]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
   float l = 0.f;
   f32x4 y = {0, 0, 0, 0};
-  if (lane * 4 < a.D) {
-    for (int s = 0; s < a.nsplit; ++s) {
-      const long i = i0 + (long)s * R;
-      const float e = fexp2(wm[i * 2] - mm);
-      l += wm[i * 2 + 1] * e;
-      y += *(const f32x4*)&a.ws[i * a.D + lane * 4] * e;
+  const int d = (lane & 31) * 4;
+  for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
+    const int n = min(64, a.nsplit - s0);
+    float e = 0.f;
+    if (lane < n) {
+      const long i = (i0 + (long)(s0 + lane) * R) * 2;
+      e = fexp2(wm[i] - mm);
+      l += wm[i + 1] * e;
     }
+#pragma unroll 8
+    for (int s = 0; s < n; s += 2) {
+      const int k = min(s + half, n - 1);
+      const float w = s + half < n ? __shfl(e, k, 64) : 0.f;
+      if (d < a.D)
+        y += *(const f32x4*)&a.ws[(i0 + (long)(s0 + k) * R) * a.D + d] * w;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] += __shfl_xor(y[k], 32, 64);
+  if (half == 0 && d < a.D) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bf16* op = a.o + b * a.osb + (long)(rr / a.G) * a.ost +
-               (long)(hk * a.G + rr % a.G) * a.D + lane * 4;
+               (long)(hk * a.G + rr % a.G) * a.D + d;
     bf16x4 z;
 #pragma unroll
     for (int k = 0; k < 4; ++k) z[k] = (bf16)(y[k] * inv);
@@ -239,7 +268,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
 // over, but no block with fewer than eight tiles (two a wave).
 int attn_decode_splits(int B, int Hkv, int R, int Tk) {
   long base = (long)B * Hkv * cdiv_h(R, DEC_ROWS);
-  long want = (1024 + base - 1) / base;
+  long want = (2048 + base - 1) / base;
   long most = (Tk + 255) / 256;
   long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);

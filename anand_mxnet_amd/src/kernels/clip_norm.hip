@@ -18,18 +18,21 @@
 
 namespace mxa {
 
-constexpr int CLIP_MAX = 140;       // entries: 28 bytes each, 4 KB in all
-constexpr int CLIP_CHUNK = 16384;   // bytes a block takes at a time
+constexpr int CLIP_MAX = 164;       // entries: 24 bytes each, 4 KB in all
 constexpr int CLIP_BLOCKS = 1024;   // partial sums of a launch
+constexpr long CLIP_LONG = 1l << 31;  // elements of an entry at most
 
 struct ClipList {
   const void* src[CLIP_MAX];
   void* dst[CLIP_MAX];
-  long n[CLIP_MAX];           // elements, and the type in the top bits
-  unsigned chunk0[CLIP_MAX];  // first chunk of each tensor
+  unsigned n[CLIP_MAX];       // elements
+  unsigned chunk0[CLIP_MAX];  // first chunk; the type in the top 4 bits
   unsigned nchunks;
   int ntens;
+  int chunk;  // bytes a block takes at a time
 };
+
+constexpr unsigned CLIP_ID = 0x0fffffff;
 
 DEVINL float clip_f(float x) { return x; }
 DEVINL float clip_f(bf16 x) { return (float)x; }
@@ -39,7 +42,7 @@ DEVINL int clip_find(const ClipList& l, unsigned c) {
   int lo = 0, hi = l.ntens - 1;
   while (lo < hi) {
     int mid = (lo + hi + 1) >> 1;
-    if (l.chunk0[mid] <= c)
+    if ((l.chunk0[mid] & CLIP_ID) <= c)
       lo = mid;
     else
       hi = mid - 1;
@@ -93,7 +96,7 @@ DEVINL void clip_scale(const T* p, T* y, long len, float f) {
     vt v = q[i];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = one(v[k]);
-    z[i] = v;
+    __builtin_nontemporal_store(v, &z[i]);
   }
   const long rest = len - nv * V;
   for (long i = threadIdx.x; i < rest; i += 256) {
@@ -119,11 +122,10 @@ __global__ __launch_bounds__(256) void clip_sumsq_kernel(
   double s = 0;
   for (unsigned c = blockIdx.x; c < l.nchunks; c += gridDim.x) {
     const int i = clip_find(l, c);
-    const int dt = (int)(l.n[i] >> 60);
-    const long n = l.n[i] & ((1l << 60) - 1);
-    const long ce = CLIP_CHUNK / (dt == 2 ? 4 : 2);
-    const long a = (long)(c - l.chunk0[i]) * ce;
-    const long len = min(ce, n - a);
+    const int dt = (int)(l.chunk0[i] >> 28);
+    const long ce = l.chunk >> (dt == 2 ? 2 : 1);
+    const long a = (long)(c - (l.chunk0[i] & CLIP_ID)) * ce;
+    const long len = min(ce, (long)l.n[i] - a);
     if (dt == 0)
       s += clip_sumsq((const bf16*)l.src[i] + a, len);
     else if (dt == 1)
@@ -147,11 +149,10 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(
     const unsigned c = l.nchunks - 1 - b;
     const int i = clip_find(l, c);
     if (!(f < 1.f) && l.src[i] == l.dst[i]) continue;
-    const int dt = (int)(l.n[i] >> 60);
-    const long n = l.n[i] & ((1l << 60) - 1);
-    const long ce = CLIP_CHUNK / (dt == 2 ? 4 : 2);
-    const long a = (long)(c - l.chunk0[i]) * ce;
-    const long len = min(ce, n - a);
+    const int dt = (int)(l.chunk0[i] >> 28);
+    const long ce = l.chunk >> (dt == 2 ? 2 : 1);
+    const long a = (long)(c - (l.chunk0[i] & CLIP_ID)) * ce;
+    const long len = min(ce, (long)l.n[i] - a);
     if (dt == 0)
       clip_scale((const bf16*)l.src[i] + a, (bf16*)l.dst[i] + a, len, f);
     else if (dt == 1)
@@ -162,37 +163,47 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(
   }
 }
 
-// Doubles of workspace for n tensors.
+// Entries of a tensor of n elements, doubles of workspace for n entries.
+long clip_entries(long n) { return (n + CLIP_LONG - 1) / CLIP_LONG; }
 long clip_ws(long n) { return (n + CLIP_MAX - 1) / CLIP_MAX * CLIP_BLOCKS; }
 
-// dtype: 0 bf16, 1 fp16, 2 fp32; every numel is positive
+// dtype: 0 bf16, 1 fp16, 2 fp32; every numel is positive, at most CLIP_LONG
 void clip_norm(const void* const* src, void* const* dst, const long* numel,
                const int* dtype, long ntens, double max_norm, double* ws,
                float* norm, hipStream_t s) {
+  long bytes = 0;
+  for (long i = 0; i < ntens; ++i) bytes += numel[i] * (dtype[i] == 2 ? 4 : 2);
+  // finding a chunk's tensor takes about as long as reading 16 KB; where
+  // every block has many chunks, larger ones
+  const int chunk = bytes > 16384l * 4 * CLIP_BLOCKS ? 65536 : 16384;
+  const long groups = (ntens + CLIP_MAX - 1) / CLIP_MAX;
   long nsum = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (long t0 = 0; t0 < ntens; t0 += CLIP_MAX) {
-      ClipList l;
-      l.ntens = (int)(ntens - t0 < CLIP_MAX ? ntens - t0 : CLIP_MAX);
-      unsigned chunks = 0;
-      for (int i = 0; i < l.ntens; ++i) {
-        const int dt = dtype[t0 + i];
-        const long ce = CLIP_CHUNK / (dt == 2 ? 4 : 2);
-        l.src[i] = src[t0 + i];
-        l.dst[i] = dst[t0 + i];
-        l.n[i] = numel[t0 + i] | (long)dt << 60;
-        l.chunk0[i] = chunks;
-        chunks += (unsigned)((numel[t0 + i] + ce - 1) / ce);
-      }
-      l.nchunks = chunks;
-      const unsigned nb = chunks < CLIP_BLOCKS ? chunks : CLIP_BLOCKS;
-      if (pass == 0) {
-        clip_sumsq_kernel<<<nb, 256, 0, s>>>(l, ws + nsum);
-        nsum += nb;
-      } else {
-        clip_scale_kernel<<<nb, 256, 0, s>>>(l, ws, (int)nsum, max_norm,
-                                             t0 == 0 ? norm : nullptr);
-      }
+  for (long step = 0; step < 2 * groups; ++step) {
+    // the sums forwards, the scaling backwards
+    const bool scale = step >= groups;
+    const long grp = scale ? 2 * groups - 1 - step : step;
+    const long t0 = grp * CLIP_MAX;
+    ClipList l;
+    l.ntens = (int)(ntens - t0 < CLIP_MAX ? ntens - t0 : CLIP_MAX);
+    l.chunk = chunk;
+    unsigned chunks = 0;
+    for (int i = 0; i < l.ntens; ++i) {
+      const int dt = dtype[t0 + i];
+      const long ce = chunk / (dt == 2 ? 4 : 2);
+      l.src[i] = src[t0 + i];
+      l.dst[i] = dst[t0 + i];
+      l.n[i] = (unsigned)numel[t0 + i];
+      l.chunk0[i] = chunks | (unsigned)dt << 28;
+      chunks += (unsigned)((numel[t0 + i] + ce - 1) / ce);
+    }
+    l.nchunks = chunks;
+    const unsigned nb = chunks < CLIP_BLOCKS ? chunks : CLIP_BLOCKS;
+    if (!scale) {
+      clip_sumsq_kernel<<<nb, 256, 0, s>>>(l, ws + nsum);
+      nsum += nb;
+    } else {
+      clip_scale_kernel<<<nb, 256, 0, s>>>(l, ws, (int)nsum, max_norm,
+                                           grp == 0 ? norm : nullptr);
     }
   }
 }

@@ -82,52 +82,112 @@ __global__ __launch_bounds__(256) void emb_lookup_kernel(
 
 // ---------------------------------------------------------------------------
 // 1. Order the tokens by row.  Block p owns rows [p R, p R + R): it reads all
-// indices twice.  The first time it counts its own, by row and by wave (a
-// wave has a contiguous sixteenth of the tokens), and those of lower rows,
-// which tells it where its part of the order begins without a word from
-// another block.  The second time it places them; lanes of a wave that hold
-// the same row are ranked by their lane, so the order is stable.
-// Reading N indices in every block is cheap beside the gradients themselves
-// while there are a few hundred blocks; they come from L2.
+// indices twice, a wave a contiguous sixteenth of the tokens, and keeps a
+// list of those that are its own.  The first time it counts them, by row and
+// by wave, and the tokens of lower rows, which tells it where its part of the
+// order begins without a word from another block.  The second time it places
+// them; equal rows within a wave are ranked by lane, so the order is stable.
+// Most groups of 64 tokens hold none of a block's rows and cost a handful of
+// instructions; some 256 blocks of rows (what a block does with its own
+// tokens takes longer than all blocks' reading of the same indices from L2).
 // ---------------------------------------------------------------------------
 constexpr int EMB_WAVES = 16;
+constexpr int EMB_BATCH = 8;     // groups of 64 tokens that are read at once
+constexpr int EMB_ROWS = 512;    // rows of a block at most
 
 template <typename I>
 __global__ __launch_bounds__(1024) void emb_sort_kernel(
     const I* __restrict__ idx, int ntok, int vocab, int R, int rlog2,
     int* __restrict__ start, int2* __restrict__ sorted) {
-  extern __shared__ int cnt[];  // [R][16]
+  __shared__ int cnt[EMB_ROWS * EMB_WAVES];  // [row][wave]
+  __shared__ unsigned list[EMB_WAVES][64 * EMB_BATCH];
   __shared__ int below[EMB_WAVES], tot[EMB_WAVES];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u64 lower = (1ull << lane) - 1;
   const int r0 = blockIdx.x * R;
-  const int r1 = min(r0 + R, vocab);
+  const int nr = min(R, vocab - r0);
   for (int i = threadIdx.x; i < R * EMB_WAVES; i += 1024) cnt[i] = 0;
   __syncthreads();
 
-  const int seg = ((ntok + EMB_WAVES * 64 - 1) / (EMB_WAVES * 64)) * 64;
+  constexpr int STEP = 64 * EMB_BATCH;
+  const int seg = (ntok + EMB_WAVES * 64 - 1) / (EMB_WAVES * 64) * 64;
   const int t0 = min(ntok, wave * seg), t1 = min(ntok, t0 + seg);
-  // a row outside the table counts as behind all rows
-  auto row_of = [&](int t) -> int {
-    long r = (long)idx[t];
-    return r < 0 || r >= vocab ? 0x7fffffff : (int)r;
-  };
-  int low = 0;
-  for (int t = t0 + lane; t < t1; t += 64) {
-    int r = row_of(t);
-    low += r < r0;
-    if (r >= r0 && r < r1) atomicAdd(&cnt[(r - r0) * EMB_WAVES + wave], 1);
-  }
+
+  // Tokens tb..tb + STEP - 1: a list of (row, place) of the block's own, in
+  // order; returns how many.  low counts the tokens of lower rows.
+  auto filter = [&](int tb, int& low) -> int {
+    unsigned r[EMB_BATCH];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) low += __shfl_xor(low, o, 64);
+    for (int u = 0; u < EMB_BATCH; ++u) {
+      const int t = tb + u * 64 + lane;
+      r[u] = 0xffffffffu;  // outside the table: behind all rows
+      if (t < t1) {
+        const I x = idx[t];
+        // a negative index is a large one when read without its sign
+        const bool in = sizeof(I) == 8
+                            ? (u64)x < (u64)(unsigned)vocab
+                            : (unsigned)x < (unsigned)vocab;
+        if (in) r[u] = (unsigned)x;
+      }
+    }
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < EMB_BATCH; ++u) {
+      low += __popcll(__ballot(r[u] < (unsigned)r0));
+      const bool mine = r[u] - (unsigned)r0 < (unsigned)nr;
+      const u64 m = __ballot(mine);
+      if (m == 0) continue;
+      if (mine)
+        list[wave][n + __popcll(m & lower)] =
+            (r[u] - (unsigned)r0) * STEP + u * 64 + lane;
+      n += __popcll(m);
+    }
+    return n;
+  };
+  // lanes whose entry has the same row as this lane's
+  auto same_row = [&](unsigned row, bool on) -> u64 {
+    u64 same = __ballot(on);
+    if (__popcll(same) > 4) {
+      for (int bit = 0; bit < rlog2; ++bit) {
+        const bool one = (row >> bit) & 1;
+        const u64 bal = __ballot(one);
+        same &= one ? bal : ~bal;
+      }
+    } else {
+      u64 rest = same;
+      while (rest) {
+        const int lead = __builtin_ctzll(rest);
+        const u64 eq = __ballot(
+            on && row == (unsigned)__builtin_amdgcn_readlane((int)row, lead));
+        if (eq >> lane & 1) same = eq;
+        rest &= ~eq;
+      }
+    }
+    return on ? same : 0;
+  };
+
+  // a wave's list and counters are its own, and its LDS accesses stay in
+  // order: one lane of each row writes for all
+  int low = 0, n = 0;
+  for (int tb = t0; tb < t1; tb += STEP) {
+    n = filter(tb, low);
+    for (int k = 0; k < n; k += 64) {
+      const bool on = k + lane < n;
+      const unsigned row = on ? list[wave][k + lane] / STEP : 0;
+      const u64 same = same_row(row, on);
+      if (same && (same & lower) == 0)
+        cnt[row * EMB_WAVES + wave] += __popcll(same);
+    }
+  }
   if (lane == 0) below[wave] = low;
   __syncthreads();
 
   // exclusive sums over (row, wave); a thread takes a run of the counters
   int first = 0;
   for (int w = 0; w < EMB_WAVES; ++w) first += below[w];
-  const int n = R * EMB_WAVES, per = (n + 1023) / 1024;
-  const int a = min(n, (int)threadIdx.x * per), e = min(n, a + per);
+  const int nc = R * EMB_WAVES, per = (nc + 1023) / 1024;
+  const int a = min(nc, (int)threadIdx.x * per), e = min(nc, a + per);
   int sum = 0;
   for (int i = a; i < e; ++i) sum += cnt[i];
   int inc = sum;
@@ -143,43 +203,27 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
   for (int i = a; i < e; ++i) {
     int c = cnt[i];
     cnt[i] = run;
-    if (i % EMB_WAVES == 0 && r0 + i / EMB_WAVES < r1)
+    if (i % EMB_WAVES == 0 && i / EMB_WAVES < nr)
       start[r0 + i / EMB_WAVES] = run;
     run += c;
   }
-  if (r1 == vocab && threadIdx.x == 1023) start[vocab] = run;
+  if (r0 + nr == vocab && threadIdx.x == 1023) start[vocab] = run;
   __syncthreads();
 
-  for (int tb = t0; tb < t1; tb += 64) {
-    const int t = tb + lane;
-    int r = t < t1 ? row_of(t) : 0x7fffffff;
-    const bool mine = r >= r0 && r < r1;
-    u64 left = __ballot(mine);
-    if (left == 0) continue;
-    const int lr = mine ? r - r0 : 0;
-    u64 same = left;  // lanes with this lane's row
-    if (__popcll(left) > 4) {
-      for (int bit = 0; bit < rlog2; ++bit) {
-        u64 bal = __ballot((lr >> bit) & 1);
-        same &= ((lr >> bit) & 1) ? bal : ~bal;
+  const bool once = t1 - t0 <= STEP;  // the list still holds them all
+  for (int tb = t0; tb < t1; tb += STEP) {
+    if (!once) n = filter(tb, low);
+    for (int k = 0; k < n; k += 64) {
+      const bool on = k + lane < n;
+      const unsigned x = on ? list[wave][k + lane] : 0, row = x / STEP;
+      const u64 same = same_row(row, on);
+      if (same) {
+        const int rank = __popcll(same & lower);
+        const int pos = cnt[row * EMB_WAVES + wave] + rank;
+        sorted[pos] = make_int2(r0 + (int)row, tb + (int)(x % STEP));
+        // the last lane of a row moves its counter on
+        if (rank == __popcll(same) - 1) cnt[row * EMB_WAVES + wave] = pos + 1;
       }
-    } else {
-      u64 rest = left;
-      while (rest) {
-        int lead = __builtin_ctzll(rest);
-        u64 eq = __ballot(mine && lr == __builtin_amdgcn_readlane(lr, lead));
-        if (mine && (eq >> lane & 1)) same = eq;
-        rest &= ~eq;
-      }
-    }
-    if (mine) {
-      const int rank = __popcll(same & ((1ull << lane) - 1));
-      const int at = lr * EMB_WAVES + wave;
-      const int pos = cnt[at] + rank;
-      sorted[pos] = make_int2(r, t);
-      // the last lane of a row moves its counter on; the counters of a wave
-      // are its own, and LDS accesses of a wave stay in order
-      if (rank == __popcll(same) - 1) cnt[at] = pos + 1;
     }
   }
 }
@@ -226,7 +270,7 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
   int key = __builtin_amdgcn_readlane(kt.x, 0);
   bool head = key == prev;  // this row began in an earlier chunk
-  constexpr int U = 8;      // rows in flight
+  constexpr int U = 16;     // rows in flight
   for (int b = 0; b < p1 - p0; b += U) {
     T x[U][V];
 #pragma unroll
@@ -389,18 +433,15 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
               const void* dy, void* dW, int* start, int2* sorted,
               float* part, int ntok, int D, int vocab, float scale,
               hipStream_t s) {
-  // about 256 blocks of rows: each reads every index, and fewer would leave
-  // compute units idle; the counters of 512 rows take 32 KB of LDS
   int lg = 0;
-  while (lg < 9 && (long)256 << lg < vocab) ++lg;
+  while ((1 << lg) < EMB_ROWS && (long)256 << lg < vocab) ++lg;
   const int R = 1 << lg;
   const unsigned nb = (unsigned)(((long)vocab + R - 1) / R);
-  const size_t lds = (size_t)R * EMB_WAVES * sizeof(int);
   if (idx64)
-    emb_sort_kernel<long><<<nb, 1024, lds, s>>>((const long*)idx, ntok,
+    emb_sort_kernel<long><<<nb, 1024, 0, s>>>((const long*)idx, ntok,
                                                 vocab, R, lg, start, sorted);
   else
-    emb_sort_kernel<int><<<nb, 1024, lds, s>>>((const int*)idx, ntok, vocab,
+    emb_sort_kernel<int><<<nb, 1024, 0, s>>>((const int*)idx, ntok, vocab,
                                                R, lg, start, sorted);
   const int nchunk = emb_chunks(ntok);
 #define GO(T, V)                                                            \
