@@ -48,6 +48,33 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
 
+  const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
+  const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
+  const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
+  const int2* rng = m.has_seg ? a.rng_k + (long)b * cdiv(a.Tk, 64) : nullptr;
+
+  Stager<D, 64, 4> ks, vs;
+  ks.init(a.kst, wave, lane);
+  vs.init(a.vst, wave, lane);
+  auto stage = [&](int buf, const Tile& t) {
+    const int* sg = t.neg ? skb : nullptr;
+    const int r = t.t * 64;
+    ks.copy(kb, a.kst, r, m.kv_len, a.D, sg, lds0 + buf * TILE, wave, lane);
+    vs.copy(vb, a.vst, r, m.kv_len, a.D, sg, lds0 + V0 + buf * TILE, wave,
+            lane);
+    if (m.has_seg && wave == 0)
+      attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
+  };
+
+  f32x16 dq[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dq[db] = zero16();
+
+  const LaneAddr la = attn_lane_addr<D>(lane);
+  TileWalk walk;
+  walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
+  Tile cur = walk.next(m, blk, wav, rng, lane);
+  if (cur.t >= 0) stage(0, cur);
   // queries, their output gradients and delta
   bf16x8 qf[KK], gf[KK];
   float lse = MXA_INF, delta = 0.f;
@@ -76,34 +103,6 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
     }
     asm volatile("" : "+v"(lse));
   }
-
-  const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
-  const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
-  const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
-  const int2* rng = m.has_seg ? a.rng_k + (long)b * cdiv(a.Tk, 64) : nullptr;
-
-  Stager<D, 64, 4> ks, vs;
-  ks.init(a.kst, wave, lane);
-  vs.init(a.vst, wave, lane);
-  auto stage = [&](int buf, const Tile& t) {
-    const int* sg = t.neg ? skb : nullptr;
-    const int r = t.t * 64;
-    ks.copy(kb, a.kst, r, m.kv_len, a.D, sg, lds0 + buf * TILE, wave, lane);
-    vs.copy(vb, a.vst, r, m.kv_len, a.D, sg, lds0 + V0 + buf * TILE, wave,
-            lane);
-    if (m.has_seg && wave == 0)
-      attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
-  };
-
-  f32x16 dq[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) dq[db] = zero16();
-
-  const LaneAddr la = attn_lane_addr<D>(lane);
-  TileWalk walk;
-  walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
-  Tile cur = walk.next(m, blk, wav, rng, lane);
-  if (cur.t >= 0) stage(0, cur);
   int buf = 0;
   while (cur.t >= 0) {
     attn_wait_copies<0>();
@@ -229,35 +228,6 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
 
   __syncthreads();
 
-  bf16x8 kf[WIDE ? 1 : KK], vf[WIDE ? 1 : KK];
-  {
-    const bf16* kp = a.k + b * a.ksb + (long)kj * a.kst + (long)hk * a.D;
-    const bf16* vp = a.v + b * a.vsb + (long)kj * a.vst + (long)hk * a.D;
-    if constexpr (WIDE) {
-      // a wave writes the chunks that it would hold, K or V
-      const bool isv = wave >= 4;
-      bf16* img = (bf16*)(smem + (isv ? V0 : K0));
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int ch = kk * 2 + half, row = wk * 32 + col;
-        bf16x8 x = isv ? attn_load_row(vp, ch, a.D, kok)
-                       : attn_load_q(kp, ch, a.D, kok, a.scale);
-        *(bf16x8*)&img[row * D + ((ch ^ attn_key<D>(row)) << 3)] = x;
-      }
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        kf[kk] = attn_load_q(kp, kk * 2 + half, a.D, kok, a.scale);
-        vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
-      }
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        attn_settle(kf[kk]);
-        attn_settle(vf[kk]);
-      }
-    }
-  }
-
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
@@ -333,6 +303,34 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
   ScoreFn f;
   QTile cur = next();
   if (cur.g >= 0) stage(0, cur);
+  bf16x8 kf[WIDE ? 1 : KK], vf[WIDE ? 1 : KK];
+  {
+    const bf16* kp = a.k + b * a.ksb + (long)kj * a.kst + (long)hk * a.D;
+    const bf16* vp = a.v + b * a.vsb + (long)kj * a.vst + (long)hk * a.D;
+    if constexpr (WIDE) {
+      // a wave writes the chunks that it would hold, K or V
+      const bool isv = wave >= 4;
+      bf16* img = (bf16*)(smem + (isv ? V0 : K0));
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const int ch = kk * 2 + half, row = wk * 32 + col;
+        bf16x8 x = isv ? attn_load_row(vp, ch, a.D, kok)
+                       : attn_load_q(kp, ch, a.D, kok, a.scale);
+        *(bf16x8*)&img[row * D + ((ch ^ attn_key<D>(row)) << 3)] = x;
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        kf[kk] = attn_load_q(kp, kk * 2 + half, a.D, kok, a.scale);
+        vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
+      }
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        attn_settle(kf[kk]);
+        attn_settle(vf[kk]);
+      }
+    }
+  }
   int buf = 0;
   while (cur.g >= 0) {
     attn_wait_copies<0>();

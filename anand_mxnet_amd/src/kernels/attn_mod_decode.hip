@@ -50,17 +50,6 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
 
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS && ok ? a.slopes[h] : 0.f);
-  bf16x8 qf[KK];
-  {
-    const bf16* qp = a.q + b * a.qsb + (long)tok * a.qst + (long)h * a.D;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
-    asm volatile("" : "+v"(f.slope));
-  }
-
   // this block's tiles: an equal share of what the sequence has
   const int nt = cdiv(max(attn_limit(m, pmax), 0), 32);
   const int share = cdiv(nt, a.nsplit);
@@ -95,6 +84,17 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
   if (t < t1) {
     stage_k(t);
     stage_v(t);
+  }
+  // the queries come while the first tiles are on their way
+  bf16x8 qf[KK];
+  {
+    const bf16* qp = a.q + b * a.qsb + (long)tok * a.qst + (long)h * a.D;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
+    asm volatile("" : "+v"(f.slope));
   }
   for (; t < t1; t += 4) {
     const bool more = t + 4 < t1;
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
   float l = 0.f;
   f32x4 y = {0, 0, 0, 0};
-  const int d = (lane & 31) * 4;
+  const int d = min((lane & 31) * 4, a.D - 4);  // D < 128: lanes repeat
   for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
     const int n = min(64, a.nsplit - s0);
     float e = 0.f;
@@ -241,19 +241,26 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
       e = fexp2(wm[i] - mm);
       l += wm[i + 1] * e;
     }
-#pragma unroll 8
-    for (int s = 0; s < n; s += 2) {
-      const int k = min(s + half, n - 1);
-      const float w = s + half < n ? __shfl(e, k, 64) : 0.f;
-      if (d < a.D)
-        y += *(const f32x4*)&a.ws[(i0 + (long)(s0 + k) * R) * a.D + d] * w;
+    // eight loads in flight: the parts come from other XCDs' writes
+    for (int s = 0; s < n; s += 16) {
+      f32x4 x[8];
+      float w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int k = min(s + 2 * u + half, n - 1);
+        x[u] = *(const f32x4*)&a.ws[(i0 + (long)(s0 + k) * R) * a.D + d];
+        w[u] = __shfl(e, k, 64);
+        if (s + 2 * u + half >= n) w[u] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) y += x[u] * w[u];
     }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
 #pragma unroll
   for (int k = 0; k < 4; ++k) y[k] += __shfl_xor(y[k], 32, 64);
-  if (half == 0 && d < a.D) {
+  if (half == 0) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bf16* op = a.o + b * a.osb + (long)(rr / a.G) * a.ost +
                (long)(hk * a.G + rr % a.G) * a.D + d;
@@ -268,7 +275,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
 // over, but no block with fewer than eight tiles (two a wave).
 int attn_decode_splits(int B, int Hkv, int R, int Tk) {
   long base = (long)B * Hkv * cdiv_h(R, DEC_ROWS);
-  long want = (2048 + base - 1) / base;
+  long want = (1536 + base - 1) / base;
   long most = (Tk + 255) / 256;
   long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);

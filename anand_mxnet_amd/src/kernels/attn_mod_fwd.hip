@@ -94,17 +94,6 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
 
-  bf16x8 qf[KK];
-  {
-    const bf16* qp = a.q + b * a.qsb + (long)qi * a.qst + (long)h * a.D;
-    const bool ok = qok && sq >= 0;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
-  }
-
   const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
   const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
   const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
@@ -134,6 +123,16 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
   Tile cur = walk.next(m, blk, wav, rng, lane);
   if (cur.t >= 0) stage(0, cur);
+  bf16x8 qf[KK];
+  {
+    const bf16* qp = a.q + b * a.qsb + (long)qi * a.qst + (long)h * a.D;
+    const bool ok = qok && sq >= 0;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
+  }
   int buf = 0;
   while (cur.t >= 0) {
     attn_wait_copies<0>();
