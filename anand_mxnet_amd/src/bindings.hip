@@ -1188,7 +1188,8 @@ mxa::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k,
 
 at::Tensor attn_ranges(const int* seg, long B, long T,
                        const at::Tensor& like) {
-  auto r = at::empty({B, (T + 63) / 64, 2}, like.options().dtype(at::kInt));
+  auto r = at::empty({B, (T + 127) / 128 * 4, 2},
+                     like.options().dtype(at::kInt));
   mxa::attn_seg_ranges(seg, (int2*)r.data_ptr<int>(), (int)B, (int)T,
                        cur_stream());
   return r;
@@ -1214,11 +1215,11 @@ std::vector<at::Tensor> attn_mod_fwd(
   at::Tensor rq, rk;
   if (a.seg_q) {
     rk = attn_ranges(a.seg_k, a.B, a.Tk, q);
+    rq = a.seg_q == a.seg_k && a.Tq == a.Tk
+             ? rk
+             : attn_ranges(a.seg_q, a.B, a.Tq, q);
     a.rng_k = (const int2*)rk.data_ptr<int>();
-    if (with_stats)
-      rq = a.seg_q == a.seg_k && a.Tq == a.Tk
-               ? rk
-               : attn_ranges(a.seg_q, a.B, a.Tq, q);
+    a.rng_q = (const int2*)rq.data_ptr<int>();
   }
   if (with_stats) {
     auto lse = at::empty({a.B, H, a.TqP}, q.options().dtype(at::kFloat));

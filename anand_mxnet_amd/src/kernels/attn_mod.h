@@ -52,7 +52,8 @@ struct AttnArgs {
   const int *seg_q, *seg_k, *prefix, *kv_len, *q_off;
   const float* slopes;
   int off0;  // added to every query_offset
-  const int2 *rng_q, *rng_k;  // smallest and largest id of each 64 rows
+  // smallest and largest id of each 32 rows, 4 ceil(T / 128) of a sequence
+  const int2 *rng_q, *rng_k;
   int nsplit;
 };
 
@@ -209,11 +210,11 @@ struct Stager {
 #pragma unroll
       for (int p = 0; p < N; ++p) copy_lds16(g0, off[p], dst + p * 1024);
     } else {
-#pragma unroll
+#pragma unroll 1  // rare: small code counts for more
       for (int p = 0; p < N; ++p) {
         const int r = (wave * N + p) * RPI + lane / CPR;
         const int ch = (lane % CPR) ^ attn_key<D>(r);
-        const bf16* g = (const bf16*)((const char*)g0 + off[p]);
+        const bf16* g = g0 + (long)r * stride + ch * 8;
         bool ok = row0 + r < row_end && ch * 8 < Dact;
         if (ok && seg) ok = seg[row0 + r] >= 0;
         if (!ok) g = (const bf16*)attn_zero16;
@@ -233,17 +234,6 @@ DEVINL void attn_stage64(const void* base, int first, int n, unsigned dst,
 DEVINL bf16x8 attn_load_row(const bf16* p, int chunk, int Dact, bool ok) {
   bf16x8 z = {};
   return ok && chunk * 8 < Dact ? *(const bf16x8*)(p + chunk * 8) : z;
-}
-
-DEVINL int wave_min(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);
-}
-DEVINL int wave_max(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);
 }
 
 // Which (batch, head) and which block of its rows a launch id stands for,
@@ -305,6 +295,10 @@ DEVINL bool attn_tile_all(const SeqMask& m, const RowSpan& s, int j0,
   return ok;
 }
 
+DEVINL int2 attn_join(int2 x, int2 y) {
+  return make_int2(min(x.x, y.x), max(x.y, y.y));
+}
+
 struct Tile {
   int t;      // index of 64 keys; negative: no more
   bool work;  // this wave has pairs in it
@@ -331,9 +325,10 @@ struct TileWalk {
       int t = base + lane;
       int2 r = make_int2(0, 0);
       bool in = t < nt;
-      if (in && m.has_seg) r = rng[t];
+      if (in && m.has_seg) r = attn_join(rng[2 * t], rng[2 * t + 1]);
       act = __ballot(in && attn_tile_any(m, blk, t * 64, r));
-      wact = __ballot(in && attn_tile_any(m, wav, t * 64, r));
+      wact = __ballot(in && wav.pmax != -0x7fffffff &&
+                      attn_tile_any(m, wav, t * 64, r));
       wful = __ballot(in && attn_tile_all(m, wav, t * 64, r));
       neg = __ballot(in && m.has_seg && r.x < 0);
     }
@@ -344,29 +339,28 @@ struct TileWalk {
   }
 };
 
-// The spans of a wave's 32 queries (q0 on) and of its block of 128.
-DEVINL void attn_spans(const SeqMask& m, int q0, int Tq, bool qok, int sq,
-                       i32x4* shared, int wave, int lane, RowSpan& wav,
-                       RowSpan& blk) {
-  wav.pmin = q0 + m.off;
-  wav.pmax = min(q0 + 31, Tq - 1) + m.off;
-  wav.smin = wave_min(qok ? sq : 0x7fffffff);
-  wav.smax = wave_max(qok ? sq : -0x7fffffff - 1);
-  if (q0 >= Tq) {  // a wave without rows sees no tile
-    wav.pmin = wav.pmax = -0x7fffffff;
-    wav.smin = 0x7fffffff;
-    wav.smax = -0x7fffffff - 1;
+// The ranges of ids of one side of sequence b.
+DEVINL const int2* attn_ranges(const int2* rng, long b, int T) {
+  return rng + b * (4 * cdiv(T, 128));
+}
+
+// The spans of a wave's 32 queries and of its block qb of 128.
+DEVINL void attn_spans(const AttnArgs& a, const SeqMask& m, int b, int qb,
+                       int wave, RowSpan& wav, RowSpan& blk) {
+  const int q0 = qb * 128 + wave * 32;
+  blk = {qb * 128 + m.off, min(qb * 128 + 127, a.Tq - 1) + m.off, 0, 0};
+  wav = {q0 + m.off, min(q0 + 31, a.Tq - 1) + m.off, 0, 0};
+  if (m.has_seg) {
+    const int2* r = attn_ranges(a.rng_q, b, a.Tq) + qb * 4;
+    const int2 w = r[wave];
+    const int2 j = attn_join(attn_join(r[0], r[1]), attn_join(r[2], r[3]));
+    wav.smin = __builtin_amdgcn_readfirstlane(w.x);
+    wav.smax = __builtin_amdgcn_readfirstlane(w.y);
+    blk.smin = __builtin_amdgcn_readfirstlane(j.x);
+    blk.smax = __builtin_amdgcn_readfirstlane(j.y);
   }
-  if (lane == 0)
-    shared[wave] = i32x4{wav.pmin, wav.pmax, wav.smin, wav.smax};
-  __syncthreads();
-  blk = {q0 - wave * 32 + m.off, wav.pmax, wav.smin, wav.smax};
-  for (int w = 0; w < 4; ++w) {
-    i32x4 s = shared[w];
-    blk.pmax = max(blk.pmax, __builtin_amdgcn_readfirstlane(s.y));
-    blk.smin = min(blk.smin, __builtin_amdgcn_readfirstlane(s.z));
-    blk.smax = max(blk.smax, __builtin_amdgcn_readfirstlane(s.w));
-  }
+  // a wave without rows sees no tile
+  if (q0 >= a.Tq) wav.pmin = wav.pmax = -0x7fffffff;
 }
 
 // Masks 16 scores of one query (C order): ids at LDS address ksg, the first

@@ -42,8 +42,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   if (m.has_seg) sq = qok ? a.seg_q[(long)b * a.Tq + qi] : -1;
 
   RowSpan wav, blk;
-  attn_spans(m, q0, a.Tq, qok, sq, (i32x4*)smem, wave, lane, wav, blk);
-  __syncthreads();
+  attn_spans(a, m, b, qb, wave, wav, blk);
   const int limit = m.has_seg && sq < 0 ? 0 : attn_limit(m, pos);
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
@@ -51,7 +50,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
   const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
   const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
-  const int2* rng = m.has_seg ? a.rng_k + (long)b * cdiv(a.Tk, 64) : nullptr;
+  const int2* rng = m.has_seg ? attn_ranges(a.rng_k, b, a.Tk) : nullptr;
 
   Stager<D, 64, 4> ks, vs;
   ks.init(a.kst, wave, lane);
@@ -212,34 +211,38 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
       !kok ? NEVER
            : (!m.causal || kj < m.prefix ? -0x7fffffff : kj);
 
-  // spans of the wave and the block: smallest `first`, largest, ids
-  const int wlo = wave_min(first), whi = wave_max(first);
-  const int slo = wave_min(sk), shi = wave_max(sk);
-  i32x4* spans = (i32x4*)smem;
-  if (lane == 0 && wave < 4) spans[wk] = i32x4{wlo, slo, shi, 0};
-  __syncthreads();
-  int blo = wlo, bslo = slo, bshi = shi;
-  for (int w = 0; w < 4; ++w) {
-    i32x4 sp = spans[w];
-    blo = min(blo, __builtin_amdgcn_readfirstlane(sp.x));
-    bslo = min(bslo, __builtin_amdgcn_readfirstlane(sp.y));
-    bshi = max(bshi, __builtin_amdgcn_readfirstlane(sp.z));
+  // spans of the wave and the block: the smallest `first` of a key that is
+  // there, the largest (NEVER if one is not), ids
+  auto first_of = [&](int j) {
+    return !m.causal || j < m.prefix ? -0x7fffffff : j;
+  };
+  const int wlo = k0 < m.kv_len ? first_of(k0) : NEVER;
+  const int whi = k0 + 31 < m.kv_len ? first_of(k0 + 31) : NEVER;
+  const int blo = kb * 128 < m.kv_len ? first_of(kb * 128) : NEVER;
+  int slo = 0, shi = 0, bslo = 0, bshi = 0;
+  if (m.has_seg) {
+    const int2* r = attn_ranges(a.rng_k, b, a.Tk) + kb * 4;
+    const int2 w = r[wk];
+    const int2 j = attn_join(attn_join(r[0], r[1]), attn_join(r[2], r[3]));
+    slo = __builtin_amdgcn_readfirstlane(w.x);
+    shi = __builtin_amdgcn_readfirstlane(w.y);
+    bslo = __builtin_amdgcn_readfirstlane(j.x);
+    bshi = __builtin_amdgcn_readfirstlane(j.y);
   }
-
-  __syncthreads();
 
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = zero16();
 
   const int ntq = cdiv(a.Tq, 64);
-  const int2* rng = m.has_seg ? a.rng_q + (long)b * ntq : nullptr;
+  const int2* rng = m.has_seg ? attn_ranges(a.rng_q, b, a.Tq) : nullptr;
   const int* sqb = m.has_seg ? a.seg_q + (long)b * a.Tq : nullptr;
 
   // Verdict on query tile t: bit 0 block, bit 1 wave, bit 2 all pairs of the
   // wave visible, bit 3 negative ids.
   auto judge = [&](int t) {
-    int2 r = m.has_seg ? rng[t] : make_int2(0, 0);
+    int2 r = make_int2(0, 0);
+    if (m.has_seg) r = attn_join(rng[2 * t], rng[2 * t + 1]);
     const int p0 = t * 64 + m.off, p1 = min(t * 64 + 63, a.Tq - 1) + m.off;
     bool any = p1 >= blo && blo != NEVER, wany = p1 >= wlo && wlo != NEVER;
     bool all = p0 >= whi && whi != NEVER;

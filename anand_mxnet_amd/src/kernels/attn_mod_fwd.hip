@@ -14,53 +14,33 @@
 
 namespace mxa {
 
-// Smallest and largest document id of every 64 rows: [B][nt].
+// Smallest and largest document id of every 32 rows, 4 ceil(T / 128) entries
+// of a sequence; behind its end, an empty range.
 __global__ __launch_bounds__(256) void attn_seg_ranges_kernel(
-    const int* __restrict__ seg, int2* __restrict__ out, int T, int nt,
+    const int* __restrict__ seg, int2* __restrict__ out, int T, int nr,
     long total) {
-  long w = (long)blockIdx.x * 4 + threadIdx.x / 64;
-  int lane = threadIdx.x & 63;
+  const long w = (long)blockIdx.x * 8 + threadIdx.x / 32;
   if (w >= total) return;
-  long b = w / nt;
-  int t = (int)(w % nt) * 64 + lane;
+  const long b = w / nr;
+  const int t = (int)(w % nr) * 32 + (threadIdx.x & 31);
   int lo = 0x7fffffff, hi = -0x7fffffff - 1;
   if (t < T) lo = hi = seg[b * T + t];
-  lo = wave_min(lo);
-  hi = wave_max(hi);
-  if (lane == 0) out[w] = make_int2(lo, hi);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o, 32));
+    hi = max(hi, __shfl_xor(hi, o, 32));
+  }
+  if ((threadIdx.x & 31) == 0) out[w] = make_int2(lo, hi);
 }
 
 void attn_seg_ranges(const int* seg, int2* out, int B, int T,
                      hipStream_t s) {
-  int nt = cdiv_h(T, 64);
-  long total = (long)B * nt;
-  attn_seg_ranges_kernel<<<(unsigned)((total + 3) / 4), 256, 0, s>>>(
-      seg, out, T, nt, total);
+  const int nr = 4 * cdiv_h(T, 128);
+  const long total = (long)B * nr;
+  attn_seg_ranges_kernel<<<(unsigned)((total + 7) / 8), 256, 0, s>>>(
+      seg, out, T, nr, total);
 }
 
-#ifndef QKL
-#define QKL 4
-#endif
-#define SCHED_QK \
-  __builtin_amdgcn_sched_group_barrier(0x100, QKL, 0); \
-  _Pragma("unroll") for (int i = 0; i < KK - QKL / 2; ++i) { \
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); \
-    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); \
-  } \
-  __builtin_amdgcn_sched_group_barrier(0x008, QKL, 0);
-#ifdef PVS
-#define SCHED_PV \
-  __builtin_amdgcn_sched_group_barrier(0x100, 2*DB, 0); \
-  __builtin_amdgcn_sched_group_barrier(0x002, 24, 0); \
-  _Pragma("unroll") for (int i = 0; i < 3 * DB; ++i) { \
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); \
-    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); \
-    __builtin_amdgcn_sched_group_barrier(0x002, 24 / DB, 0); \
-  } \
-  __builtin_amdgcn_sched_group_barrier(0x008, DB, 0);
-#else
-#define SCHED_PV
-#endif
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   constexpr int KK = D / 16, DB = D / 32;
@@ -88,8 +68,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   if (m.has_seg) sq = qok ? a.seg_q[(long)b * a.Tq + qi] : -1;
 
   RowSpan wav, blk;
-  attn_spans(m, q0, a.Tq, qok, sq, (i32x4*)smem, wave, lane, wav, blk);
-  __syncthreads();
+  attn_spans(a, m, b, qb, wave, wav, blk);
   const int limit = m.has_seg && sq < 0 ? 0 : attn_limit(m, pos);
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS ? a.slopes[h] : 0.f);
@@ -97,8 +76,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   const bf16* kb = a.k + b * a.ksb + (long)hk * a.D;
   const bf16* vb = a.v + b * a.vsb + (long)hk * a.D;
   const int* skb = m.has_seg ? a.seg_k + (long)b * a.Tk : nullptr;
-  const int ntk = cdiv(a.Tk, 64);
-  const int2* rng = m.has_seg ? a.rng_k + (long)b * ntk : nullptr;
+  const int2* rng = m.has_seg ? attn_ranges(a.rng_k, b, a.Tk) : nullptr;
 
   Stager<D, 64, 4> ks, vs;
   ks.init(a.kst, wave, lane);
@@ -149,7 +127,6 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
         for (int nb = 0; nb < 2; ++nb)
           s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
                          s[nb]);
-      SCHED_QK
 
       const int j0 = cur.t * 64 + 4 * half;
       float x[32];
@@ -221,7 +198,6 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
         for (int db = 0; db < DB; ++db)
           o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, V0 + st * 32 * D),
                          pf[st], o[db]);
-      SCHED_PV
     }
     cur = nxt;
     buf ^= 1;
