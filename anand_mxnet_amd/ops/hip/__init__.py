@@ -920,18 +920,19 @@ class _ShapedMha(torch.autograd.Function):
     def forward(ctx, q, k, v, conf, slopes, seg_q, seg_k, prefix, kv_len,
                 q_off, off0):
         opts = (slopes, seg_q, seg_k, prefix, kv_len, q_off)
-        out, lse, *rng = _C.attn_mod_fwd(q, k, v, *conf, *opts, off0, True)
-        ctx.save_for_backward(q, k, v, out, lse, *opts, *rng)
+        out, lse, lo, *rng = _C.attn_mod_fwd(q, k, v, *conf, *opts, off0,
+                                             True)
+        ctx.save_for_backward(q, k, v, out, lse, lo, *opts, *rng)
         ctx.conf = conf
         ctx.off0 = off0
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, *rest = ctx.saved_tensors
+        q, k, v, out, lse, lo, *rest = ctx.saved_tensors
         opts, rng = rest[:6], (rest[6:] or [None, None])
         need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        grads = _C.attn_mod_bwd(q, k, v, out, _rows16(dout), lse, *rng,
+        grads = _C.attn_mod_bwd(q, k, v, out, _rows16(dout), lse, lo, *rng,
                                 *ctx.conf, *opts, ctx.off0, need_kv)
         return tuple(grads) + (None,) * (11 - len(grads))
 

@@ -1196,8 +1196,9 @@ at::Tensor attn_ranges(const int* seg, long B, long T,
 }
 }  // namespace
 
-// Returns the output, and where with_stats is set the log2 sums and (with
-// ids) the id ranges of the query and key tiles, which the backward reuses.
+// Returns the output, and where with_stats is set what the backward needs:
+// the log2 sums, what rounding took from the output, and (with ids) the id
+// ranges of queries and keys.
 std::vector<at::Tensor> attn_mod_fwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, long H,
     long Hkv, double scale, double cap, bool causal, const OptT& slopes,
@@ -1225,6 +1226,9 @@ std::vector<at::Tensor> attn_mod_fwd(
     auto lse = at::empty({a.B, H, a.TqP}, q.options().dtype(at::kFloat));
     a.lse = lse.data_ptr<float>();
     res.push_back(lse);
+    auto lo = at::empty_like(out);
+    a.olo = bfp_mut(lo);
+    res.push_back(lo);
     if (a.seg_q) {
       res.push_back(rq);
       res.push_back(rk);
@@ -1237,7 +1241,7 @@ std::vector<at::Tensor> attn_mod_fwd(
 std::vector<at::Tensor> attn_mod_bwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& out, const at::Tensor& dout, const at::Tensor& lse,
-    const OptT& rng_q, const OptT& rng_k, long H, long Hkv, double scale,
+    const at::Tensor& lo, const OptT& rng_q, const OptT& rng_k, long H, long Hkv, double scale,
     double cap, bool causal, const OptT& slopes, const OptT& seg_q,
     const OptT& seg_k, const OptT& prefix, const OptT& kv_len,
     const OptT& q_off, long off0, bool need_kv) {
@@ -1246,12 +1250,15 @@ std::vector<at::Tensor> attn_mod_bwd(
                      seg_k, prefix, kv_len, q_off, off0);
   attn_operand(out, q, "output");
   attn_operand(dout, q, "output gradient");
+  attn_operand(lo, q, "output remainder");
   TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes() &&
+                  lo.sizes() == q.sizes() && lo.is_contiguous() &&
                   lse.numel() == (long)a.B * H * a.TqP &&
                   (a.seg_q == nullptr) == !rng_q.has_value() &&
                   rng_q.has_value() == rng_k.has_value(),
               "attention: backward does not match its forward");
   a.o = const_cast<bf16*>(bfp(out));
+  a.olo = const_cast<bf16*>(bfp(lo));
   a.osb = out.stride(0);
   a.ost = out.stride(1);
   a.dout = bfp(dout);

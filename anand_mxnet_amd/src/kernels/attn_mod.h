@@ -39,6 +39,7 @@ namespace mxa {
 struct AttnArgs {
   const bf16 *q, *k, *v;
   bf16* o;
+  bf16* olo;   // what rounding took from o, [B, Tq, H, D]; may be null
   float* lse;  // [B, H, TqP] log2 of the softmax sum; +inf: row sees nothing
   const bf16* dout;
   float* delta;  // [B, H, TqP] sum_d dout * out
@@ -438,6 +439,23 @@ DEVINL bf16x8 pack8(const float* x) {
   return y;
 }
 
+// acc + sum of a[i] * b[i], in 32 bits
+DEVINL float dot8(bf16x8 a, bf16x8 b, float acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a[2 * i], a[2 * i + 1]},
+                                          bf16x2{b[2 * i], b[2 * i + 1]}, acc,
+                                          false);
+  return acc;
+}
+
+DEVINL bf16x8 ones8() {
+  bf16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (bf16)1.f;
+  return y;
+}
+
 DEVINL f32x16 zero16() {
   f32x16 z;
 #pragma unroll
@@ -450,10 +468,10 @@ DEVINL f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 
 // Writes one row of a transposed accumulator: d = 8 ii + 4 half + 0..3 of
-// each 32.
+// each 32; what the rounding takes goes to lo, if it is not null.
 template <int DB>
 DEVINL void attn_store_t(bf16* p, const f32x16* acc, float mul, int Dact,
-                         int half) {
+                         int half, bf16* lo = nullptr) {
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -463,6 +481,13 @@ DEVINL void attn_store_t(bf16* p, const f32x16* acc, float mul, int Dact,
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = (bf16)(acc[db][ii * 4 + i] * mul);
       if (d < Dact) *(bf16x4*)(p + d) = y;
+      if (lo && d < Dact) {
+        bf16x4 z;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          z[i] = (bf16)(acc[db][ii * 4 + i] * mul - (float)y[i]);
+        *(bf16x4*)(lo + d) = z;
+      }
     }
 }
 

@@ -83,15 +83,14 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
     const bf16* qp = a.q + b * a.qsb + (long)qi * a.qst + (long)h * a.D;
     const bf16* gp = a.dout + b * a.gsb + (long)qi * a.gst + (long)h * a.D;
     const bf16* op = a.o + b * a.osb + (long)qi * a.ost + (long)h * a.D;
+    const bf16* lp = a.olo + (((long)b * a.Tq + qi) * a.H + h) * a.D;
     if (ok) lse = a.lse[row];
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       qf[kk] = attn_load_q(qp, kk * 2 + half, a.D, ok, a.scale);
       gf[kk] = attn_load_row(gp, kk * 2 + half, a.D, ok);
-      bf16x8 of = attn_load_row(op, kk * 2 + half, a.D, ok);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        delta = fmaf((float)gf[kk][i], (float)of[i], delta);
+      delta = dot8(gf[kk], attn_load_row(op, kk * 2 + half, a.D, ok), delta);
+      delta = dot8(gf[kk], attn_load_row(lp, kk * 2 + half, a.D, ok), delta);
     }
     delta += __shfl_xor(delta, 32, 64);
     if (half == 0 && qi < a.TqP) a.delta[row] = delta;

@@ -136,9 +136,9 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] = fexp2(x[8 * w + i] - mrow);
-        lsum += p[i];
       }
       pf[w] = pack8(p);
+      lsum = dot8(pf[w], ones8(), lsum);
     }
     if (more)
       attn_wait_copies<NCOPY>();

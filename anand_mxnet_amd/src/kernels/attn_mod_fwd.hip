@@ -7,6 +7,12 @@
 // of a query lie in one lane of each half of the wave, and feeds the rounded
 // P^T straight into O^T += V^T P^T.
 //
+// The sum of a row is that of its rounded probabilities, so that rounding
+// them leaves the weights of the values at one in all.  In training the part
+// of the output that rounding takes is kept too: the backward subtracts
+// delta = sum_d dO O from every dP, and with the rounded O alone that error,
+// the same for a whole row, is twice all others together.
+//
 // The running maximum moves only when some row's scores pass it by more
 // than 8 (a factor of 256, harmless in fp32 sums and bf16 probabilities), so
 // the rescaling of the accumulators is skipped for almost every tile.
@@ -188,9 +194,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
           const int g = 2 * st + (i >> 2);
           p[i] = BIAS ? fexp2(x[8 * st + i] - (mrow - base - (float)g * step))
                       : fexp2(fmaf(x[8 * st + i], f.mu, -mrow));
-          lsum += p[i];
         }
         pf[st] = pack8(p);
+        lsum = dot8(pf[st], ones8(), lsum);
       }
 #pragma unroll
       for (int st = 0; st < 4; ++st)
@@ -208,7 +214,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
   if (qok) {
     bf16* op = a.o + b * a.osb + (long)qi * a.ost + (long)h * a.D;
-    attn_store_t<DB>(op, o, inv, a.D, half);
+    bf16* lo =
+        a.olo ? a.olo + (((long)b * a.Tq + qi) * a.H + h) * a.D : nullptr;
+    attn_store_t<DB>(op, o, inv, a.D, half, lo);
   }
   if (a.lse && half == 0 && qi < a.TqP)
     a.lse[((long)b * a.H + h) * a.TqP + qi] =
