@@ -467,28 +467,40 @@ DEVINL f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// Writes one row of a transposed accumulator: d = 8 ii + 4 half + 0..3 of
-// each 32; what the rounding takes goes to lo, if it is not null.
-template <int DB>
-DEVINL void attn_store_t(bf16* p, const f32x16* acc, float mul, int Dact,
-                         int half, bf16* lo = nullptr) {
+// Writes a wave's transposed accumulator (32 rows from row0 on, those below
+// row_end) as rows of bf16.  They pass through 64 D bytes of LDS of the
+// wave's own at `box`: a lane has four columns of a row at a time, and
+// stores of 8 bytes to 32 rows took a third of a short block's time.
+// REST writes what the rounding takes instead.
+template <int DB, bool REST>
+DEVINL void attn_store_rows(lds_char* sm, unsigned box, const f32x16* acc,
+                            float mul, bf16* base, long stride, int row0,
+                            int row_end, int Dact, int lane) {
+  constexpr int D = 32 * DB, CPR = D / 8, RPI = 64 / CPR;
+  typedef __attribute__((address_space(3))) bf16x4 lds4;
+  const int half = lane >> 5, col = lane & 31;
+  const unsigned at = box + col * (2 * D) + half * 8;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii) {
-      const int d = db * 32 + 8 * ii + 4 * half;
       bf16x4 y;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = (bf16)(acc[db][ii * 4 + i] * mul);
-      if (d < Dact) *(bf16x4*)(p + d) = y;
-      if (lo && d < Dact) {
-        bf16x4 z;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          z[i] = (bf16)(acc[db][ii * 4 + i] * mul - (float)y[i]);
-        *(bf16x4*)(lo + d) = z;
+      for (int i = 0; i < 4; ++i) {
+        const float x = acc[db][ii * 4 + i] * mul;
+        y[i] = (bf16)x;
+        if (REST) y[i] = (bf16)(x - (float)y[i]);
       }
+      *(lds4*)(sm + (at + (((db * 4 + ii) ^ (col & 7)) << 4))) = y;
     }
+#pragma unroll
+  for (int p = 0; p < 32 / RPI; ++p) {
+    const int r = p * RPI + lane / CPR, ch = lane % CPR;
+    const bf16x8 y = attn_lds<bf16x8>(
+        sm, box + r * (2 * D) + ((ch ^ (r & 7)) << 4));
+    if (row0 + r < row_end && ch * 8 < Dact)
+      *(bf16x8*)(base + (long)(row0 + r) * stride + ch * 8) = y;
+  }
 }
 
 }  // namespace mxa

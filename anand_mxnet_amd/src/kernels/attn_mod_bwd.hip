@@ -154,10 +154,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
     buf ^= 1;
   }
 
-  if (qok) {
-    bf16* op = a.dq + ((long)b * a.Tq + qi) * a.H * a.D + (long)h * a.D;
-    attn_store_t<DB>(op, dq, attn_ds_scale<CAP>(a.scale), a.D, half);
-  }
+  __syncthreads();
+  attn_store_rows<DB, false>(sm, wave * 64 * D, dq, attn_ds_scale<CAP>(a.scale),
+                             a.dq + ((long)b * a.Tq * a.H + h) * a.D,
+                             (long)a.H * a.D, q0, a.Tq, a.D, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -452,31 +452,35 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
     if (wave >= 4) return;
   }
 
-  if (kj < a.Tk) {
-    const long off = ((long)b * a.Tk + kj) * a.Hkv * a.D + (long)hk * a.D;
-    if (a.nsplit == 1) {
-      attn_store_t<DB>(a.dk + off, dk, attn_ds_scale<CAP>(a.scale), a.D,
-                       half);
-      attn_store_t<DB>(a.dv + off, dv, 1.f, a.D, half);
-    } else {
-      const long n = (long)a.B * a.Tk * a.Hkv * a.D;
-      float* w = a.ws + (long)split * 2 * n + off;
+  const long off = ((long)b * a.Tk * a.Hkv + hk) * a.D;
+  const long kst = (long)a.Hkv * a.D;
+  if (a.nsplit == 1) {
+    // the waves that are left may still read the LDS of others: WIDE waves
+    // take theirs from K and V, which no one reads any more
+    if constexpr (!WIDE) __syncthreads();
+    const unsigned box = (WIDE ? K0 : 0) + wave * 64 * D;
+    attn_store_rows<DB, false>(sm, box, dk, attn_ds_scale<CAP>(a.scale),
+                               a.dk + off, kst, k0, a.Tk, a.D, lane);
+    attn_store_rows<DB, false>(sm, box, dv, 1.f, a.dv + off, kst, k0, a.Tk,
+                               a.D, lane);
+  } else if (kj < a.Tk) {
+    const long n = (long)a.B * a.Tk * a.Hkv * a.D;
+    float* w = a.ws + (long)split * 2 * n + off + kj * kst;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int ii = 0; ii < 4; ++ii) {
-          const int d = db * 32 + 8 * ii + 4 * half;
-          if (d >= a.D) continue;
-          f32x4 y, z;
+      for (int ii = 0; ii < 4; ++ii) {
+        const int d = db * 32 + 8 * ii + 4 * half;
+        if (d >= a.D) continue;
+        f32x4 y, z;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            y[i] = dk[db][ii * 4 + i] * attn_ds_scale<CAP>(a.scale);
-            z[i] = dv[db][ii * 4 + i];
-          }
-          *(f32x4*)(w + d) = y;
-          *(f32x4*)(w + n + d) = z;
+        for (int i = 0; i < 4; ++i) {
+          y[i] = dk[db][ii * 4 + i] * attn_ds_scale<CAP>(a.scale);
+          z[i] = dv[db][ii * 4 + i];
         }
-    }
+        *(f32x4*)(w + d) = y;
+        *(f32x4*)(w + n + d) = z;
+      }
   }
 }
 

@@ -212,12 +212,15 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   lsum += __shfl_xor(lsum, 32, 64);
   // a sum of zero: nothing seen, the row is zero; a NaN stays one
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-  if (qok) {
-    bf16* op = a.o + b * a.osb + (long)qi * a.ost + (long)h * a.D;
-    bf16* lo =
-        a.olo ? a.olo + (((long)b * a.Tq + qi) * a.H + h) * a.D : nullptr;
-    attn_store_t<DB>(op, o, inv, a.D, half, lo);
-  }
+  __syncthreads();  // the tiles' LDS is free
+  const unsigned box = wave * 64 * D;
+  attn_store_rows<DB, false>(sm, box, o, inv,
+                             a.o + b * a.osb + (long)h * a.D, a.ost, q0,
+                             a.Tq, a.D, lane);
+  if (a.olo)
+    attn_store_rows<DB, true>(sm, box, o, inv,
+                              a.olo + ((long)b * a.Tq * a.H + h) * a.D,
+                              (long)a.H * a.D, q0, a.Tq, a.D, lane);
   if (a.lse && half == 0 && qi < a.TqP)
     a.lse[((long)b * a.H + h) * a.TqP + qi] =
         qok && lsum != 0.f ? mrow + __log2f(lsum) : MXA_INF;
