@@ -469,8 +469,9 @@ DEVINL f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 
 // Writes a wave's transposed accumulator (32 rows from row0 on, those below
 // row_end) as rows of bf16.  They pass through 64 D bytes of LDS of the
-// wave's own at `box`: a lane has four columns of a row at a time, and
-// stores of 8 bytes to 32 rows took a third of a short block's time.
+// wave's own at `box`: a lane has four columns of a row at a time, and with
+// stores of 8 bytes to 32 rows 128 short sequences took 64 us forward, not
+// 60.
 // REST writes what the rounding takes instead.
 template <int DB, bool REST>
 DEVINL void attn_store_rows(lds_char* sm, unsigned box, const f32x16* acc,
