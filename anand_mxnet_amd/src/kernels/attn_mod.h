@@ -286,14 +286,10 @@ DEVINL bool attn_tile_any(const SeqMask& m, const RowSpan& s, int j0,
   return ok;
 }
 
-// Does every query of s see every one of them?
-DEVINL bool attn_tile_all(const SeqMask& m, const RowSpan& s, int j0,
-                          int2 r) {
-  bool ok = j0 + 64 <= attn_limit(m, s.pmin);
-  if (m.has_seg)
-    ok = ok && s.smin >= 0 && s.smin == s.smax && r.x == s.smin &&
-         r.y == s.smin;
-  return ok;
+// Do all queries of s and all of these keys have one id?
+DEVINL bool attn_tile_one(const SeqMask& m, const RowSpan& s, int2 r) {
+  return !m.has_seg || (s.smin >= 0 && s.smin == s.smax && r.x == s.smin &&
+                        r.y == s.smin);
 }
 
 DEVINL int2 attn_join(int2 x, int2 y) {
@@ -303,7 +299,8 @@ DEVINL int2 attn_join(int2 x, int2 y) {
 struct Tile {
   int t;      // index of 64 keys; negative: no more
   bool work;  // this wave has pairs in it
-  bool full;  // all its pairs are visible
+  bool ids;   // its queries' and keys' ids are not all the same
+  bool ends;  // some queries' last visible key lies in it
   bool neg;   // some ids are negative: stage with care
 };
 
@@ -311,18 +308,18 @@ struct Tile {
 // tile to a lane, and the verdicts are kept as bits.
 struct TileWalk {
   int base, nt;
-  u64 act, wact, wful, neg;
+  u64 act, wact, wone, wend, neg;
 
   DEVINL void start(int first, int ntiles) {
     base = first - 64;
     nt = ntiles;
-    act = wact = wful = neg = 0;
+    act = wact = wone = wend = neg = 0;
   }
   DEVINL Tile next(const SeqMask& m, const RowSpan& blk, const RowSpan& wav,
                    const int2* rng, int lane) {
     while (act == 0) {
       base += 64;
-      if (base >= nt) return Tile{-1, false, false, false};
+      if (base >= nt) return Tile{-1, false, false, false, false};
       int t = base + lane;
       int2 r = make_int2(0, 0);
       bool in = t < nt;
@@ -330,13 +327,14 @@ struct TileWalk {
       act = __ballot(in && attn_tile_any(m, blk, t * 64, r));
       wact = __ballot(in && wav.pmax != -0x7fffffff &&
                       attn_tile_any(m, wav, t * 64, r));
-      wful = __ballot(in && attn_tile_all(m, wav, t * 64, r));
+      wone = __ballot(in && attn_tile_one(m, wav, r));
+      wend = __ballot(in && t * 64 + 64 > attn_limit(m, wav.pmin));
       neg = __ballot(in && m.has_seg && r.x < 0);
     }
     int i = __builtin_ctzll(act);
     act &= act - 1;
-    return Tile{base + i, (bool)((wact >> i) & 1), (bool)((wful >> i) & 1),
-                (bool)((neg >> i) & 1)};
+    return Tile{base + i, (bool)((wact >> i) & 1), !((wone >> i) & 1),
+                (bool)((wend >> i) & 1), (bool)((neg >> i) & 1)};
   }
 };
 
@@ -366,21 +364,22 @@ DEVINL void attn_spans(const AttnArgs& a, const SeqMask& m, int b, int qb,
 
 // Masks 16 scores of one query (C order): ids at LDS address ksg, the first
 // `lim` keys are seen.  A masked score becomes `gone`.
-DEVINL void attn_mask_keys(float* x, int has_seg, lds_char* sm, unsigned ksg,
-                           int sq, int lim, float gone) {
-  if (has_seg) {
+DEVINL void attn_mask_keys(float* x, bool ids, bool ends, lds_char* sm,
+                           unsigned ksg, int sq, int lim, float gone) {
+  if (ids) {
 #pragma unroll
     for (int ii = 0; ii < 4; ++ii) {
       const i32x4 k4 = attn_lds<i32x4>(sm, ksg + 32 * ii);
-      x[ii * 4 + 0] = k4.x == sq ? x[ii * 4 + 0] : gone;
-      x[ii * 4 + 1] = k4.y == sq ? x[ii * 4 + 1] : gone;
-      x[ii * 4 + 2] = k4.z == sq ? x[ii * 4 + 2] : gone;
-      x[ii * 4 + 3] = k4.w == sq ? x[ii * 4 + 3] : gone;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[ii * 4 + i] = k4[i] == sq ? x[ii * 4 + i] : gone;
     }
   }
+  if (ends) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    x[i] = 8 * (i >> 2) + (i & 3) < lim ? x[i] : gone;
+    for (int i = 0; i < 16; ++i)
+      x[i] = 8 * (i >> 2) + (i & 3) < lim ? x[i] : gone;
+  }
 }
 
 // Constants of the score function.  The sign of the scale goes to the

@@ -123,8 +123,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = attn_z<CAP>(f, s[i]);
-        if (!cur.full)
-          attn_mask_keys(x, m.has_seg, sm,
+        if (cur.ids || cur.ends)
+          attn_mask_keys(x, cur.ids, cur.ends, sm,
                          ID0 + buf * 256 + nb * 128 + 16 * half, sq,
                          limit - j0, attn_gone<CAP>());
         bf16x8 df[2];

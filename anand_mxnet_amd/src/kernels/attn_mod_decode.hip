@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = attn_z<CAP>(f, s[i]);
     if (t * 32 + 32 > full_end)
-      attn_mask_keys(x, 0, sm, 0, 0, limit - j0, -MXA_INF);
+      attn_mask_keys(x, false, true, sm, 0, 0, limit - j0, -MXA_INF);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int dj = 8 * (i >> 2) + (i & 3);

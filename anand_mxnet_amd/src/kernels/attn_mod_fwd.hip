@@ -139,10 +139,11 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         x[i] = attn_z<CAP>(f, s[i >> 4][i & 15]);
-      if (!cur.full) {
-        attn_mask_keys(x, m.has_seg, sm, ids, sq, limit - j0, -MXA_INF);
-        attn_mask_keys(x + 16, m.has_seg, sm, ids + 128, sq, limit - j0 - 32,
+      if (cur.ids || cur.ends) {
+        attn_mask_keys(x, cur.ids, cur.ends, sm, ids, sq, limit - j0,
                        -MXA_INF);
+        attn_mask_keys(x + 16, cur.ids, cur.ends, sm, ids + 128, sq,
+                       limit - j0 - 32, -MXA_INF);
       }
       // with a bias, x[i] + base + (i >> 2) * step becomes the score.  The
       // bias is linear in j where all keys of the tile lie before the wave's
