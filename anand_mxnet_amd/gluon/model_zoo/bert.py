@@ -36,31 +36,57 @@ class PositionwiseFFN(HybridBlock):
 
 
 class MultiHeadAttentionCell(HybridBlock):
+    """Projections around nd.multi_head_attention.  num_kv_heads, logit_cap
+    and distance_bias (slopes 2 ** (-8 (h + 1) / num_heads)) and the masks
+    that forward takes by name shape the scores as documented there; such a
+    cell trains with dropout=0 only."""
+
     def __init__(self, units, num_heads, dropout=0.1, causal=False,
+                 num_kv_heads=None, logit_cap=None, distance_bias=False,
                  **kwargs):
         super().__init__(**kwargs)
         self._units = units
         self._num_heads = num_heads
         self._dropout = dropout
         self._causal = causal
+        self._num_kv_heads = num_kv_heads
+        self._logit_cap = logit_cap
+        self._distance_bias = distance_bias
+        self._slopes = {}
+        kv_units = units // num_heads * (num_kv_heads or num_heads)
         with self.name_scope():
             self.proj_query = nn.Dense(units, flatten=False, in_units=units,
                                        prefix="query_")
-            self.proj_key = nn.Dense(units, flatten=False, in_units=units,
+            self.proj_key = nn.Dense(kv_units, flatten=False, in_units=units,
                                      prefix="key_")
-            self.proj_value = nn.Dense(units, flatten=False, in_units=units,
-                                       prefix="value_")
+            self.proj_value = nn.Dense(kv_units, flatten=False,
+                                       in_units=units, prefix="value_")
             self.proj_out = nn.Dense(units, flatten=False, in_units=units,
                                      prefix="out_")
 
-    def forward(self, q_in, kv_in=None, mask=None):
+    def _distance_slopes(self, ctx):
+        if not self._distance_bias:
+            return None
+        if ctx not in self._slopes:  # a constant, laid out once a device
+            H = self._num_heads
+            self._slopes[ctx] = nd.array(
+                [2.0 ** (-8.0 * (h + 1) / H) for h in range(H)], ctx=ctx,
+                dtype="float32")
+        return self._slopes[ctx]
+
+    def forward(self, q_in, kv_in=None, mask=None, segment_ids=None,
+                prefix_length=None, kv_length=None, query_offset=None):
         kv_in = kv_in if kv_in is not None else q_in
         q = self.proj_query(q_in)
         k = self.proj_key(kv_in)
         v = self.proj_value(kv_in)
-        out = nd.multi_head_attention(q, k, v, self._num_heads, mask=mask,
-                                      dropout_p=self._dropout,
-                                      causal=self._causal)
+        out = nd.multi_head_attention(
+            q, k, v, self._num_heads, mask=mask, dropout_p=self._dropout,
+            causal=self._causal, num_kv_heads=self._num_kv_heads,
+            logit_cap=self._logit_cap,
+            distance_slopes=self._distance_slopes(q.context),
+            segment_ids=segment_ids, prefix_length=prefix_length,
+            kv_length=kv_length, query_offset=query_offset)
         return self.proj_out(out)
 
     hybrid_forward = None
@@ -68,18 +94,22 @@ class MultiHeadAttentionCell(HybridBlock):
 
 class TransformerEncoderCell(HybridBlock):
     def __init__(self, units, hidden_size, num_heads, dropout=0.1,
-                 causal=False, **kwargs):
+                 causal=False, num_kv_heads=None, logit_cap=None,
+                 distance_bias=False, **kwargs):
         super().__init__(**kwargs)
         with self.name_scope():
             self.attention_cell = MultiHeadAttentionCell(
-                units, num_heads, dropout, causal=causal, prefix="attn_")
+                units, num_heads, dropout, causal=causal,
+                num_kv_heads=num_kv_heads, logit_cap=logit_cap,
+                distance_bias=distance_bias, prefix="attn_")
             self.proj_dropout = nn.Dropout(dropout)
             self.layer_norm = nn.LayerNorm(in_channels=units)
             self.ffn = PositionwiseFFN(units, hidden_size, dropout,
                                        prefix="ffn_")
 
-    def forward(self, x, mask=None):
-        attn = self.attention_cell(x, mask=mask)
+    def forward(self, x, mask=None, segment_ids=None, prefix_length=None):
+        attn = self.attention_cell(x, mask=mask, segment_ids=segment_ids,
+                                   prefix_length=prefix_length)
         x = self.layer_norm(x + self.proj_dropout(attn))
         return self.ffn(x)
 

@@ -937,9 +937,14 @@ class _ShapedMha(torch.autograd.Function):
         return tuple(grads) + (None,) * (11 - len(grads))
 
 
-# Up to this many rows (query tokens times heads of a group) the form that
-# splits the keys is taken; above, that of 128 queries a block.
-_DECODE_ROWS = 64
+def _split_keys(B, Tq, H, G):
+    """Whether the form that divides the keys over the chip is taken, rather
+    than 128 queries a block: for few rows (query tokens times heads of a
+    group), and where the blocks would leave half of the chip idle.  One
+    sequence of 32768 keys, 16 heads of 128: 256 queries take 158 us in that
+    form and 778 us in blocks, 1024 queries 804 and 791; 16 sequences of 4096
+    keys, 16 heads over 4: 16 queries 53 and 99, 64 queries 172 and 103."""
+    return Tq * G <= 64 or B * H * ((Tq + 127) // 128) < 128
 
 
 @register_gpu("shaped_mha")
@@ -954,8 +959,8 @@ def shaped_mha(q, k, v, num_heads, num_kv_heads, scale, cap, causal, slopes,
                                     or v.requires_grad):
         return _ShapedMha.apply(q, k, v, conf, slopes, seg_q, seg_k, prefix,
                                 kv_len, q_off, off0)
-    if seg_q is None and q.shape[1] * (num_heads // num_kv_heads) \
-            <= _DECODE_ROWS:
+    if seg_q is None and _split_keys(q.shape[0], q.shape[1], num_heads,
+                                     num_heads // num_kv_heads):
         return _C.attn_decode(q, k, v, *conf, slopes, prefix, kv_len, q_off,
                               off0)
     return _C.attn_mod_fwd(q, k, v, *conf, slopes, seg_q, seg_k, prefix,

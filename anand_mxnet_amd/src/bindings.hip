@@ -1307,6 +1307,7 @@ at::Tensor attn_decode(const at::Tensor& q, const at::Tensor& k,
   a.o = bfp_mut(out);
   a.osb = out.stride(0);
   a.ost = out.stride(1);
+  TORCH_CHECK((long)a.Tq * a.G < (1L << 30), "attention: too large");
   const int R = a.Tq * a.G;
   a.nsplit = mxa::attn_decode_splits(a.B, a.Hkv, R, a.Tk);
   TORCH_CHECK((long)a.B * a.Hkv * ((R + 31) / 32) * a.nsplit < (1L << 31),

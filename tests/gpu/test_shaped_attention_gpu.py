@@ -157,6 +157,24 @@ def test_infer(i):
     check("out", _infer(c), _ref(c, grads=False)["out"])
 
 
+@pytest.mark.parametrize(
+    "i", [i for i in range(len(TRAIN)) if not TRAIN[i].get("docs")])
+def test_both_forms(i):
+    """Few queries and many take different kernels; each takes any number."""
+    from anand_mxnet_amd import _C
+    c = _case(100 + i, **TRAIN[i])
+    want = _ref(c, grads=False)["out"]
+    q, k, v = c["q"].cuda(), c["k"].cuda(), c["v"].cuda()
+    D = q.shape[2] // c["H"]
+    conf = (c["H"], c["Hkv"], c["scale"] or D ** -0.5, c["cap"] or 0.0,
+            c["causal"])
+    opt = [None if c[n] is None else torch.as_tensor(c[n]).cuda()
+           for n in ("slopes", "prefix", "kv_len", "off")]
+    check("split", _C.attn_decode(q, k, v, *conf, *opt, 0), want)
+    check("blocks", _C.attn_mod_fwd(q, k, v, *conf, opt[0], None, None,
+                                    *opt[1:], 0, False)[0], want)
+
+
 DECODE = [
     dict(B=1, Tq=1, Tk=1, H=1, Hkv=1, D=64, cap=20.0),
     dict(B=3, Tq=1, Tk=500, H=4, Hkv=4, D=64, kv_len=[500, 0, 33],
