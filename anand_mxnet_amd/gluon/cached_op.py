@@ -55,8 +55,14 @@ def maybe_cached_forward(block, args):
         return None
     if _ag.is_recording():
         return None  # training path stays eager (bench captures whole steps)
-    tensors = [a._t for a in args if isinstance(a, NDArray)]
-    if not tensors or not all(t.is_cuda for t in tensors):
+    # an argument left out at the end keeps its default; one left out before
+    # another would put that one in its place
+    while args and args[-1] is None:
+        args = args[:-1]
+    if not args or not all(isinstance(a, NDArray) for a in args):
+        return None
+    tensors = [a._t for a in args]
+    if not all(t.is_cuda for t in tensors):
         return None
     cg = getattr(block, "_cached_graph_obj", None)
     if cg is None:

@@ -731,6 +731,10 @@ _NATIVE_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 @register_gpu("embedding")
 def embedding(idx, W, scale=1.0):
+    if idx.device != W.device:
+        from ...base import MXNetError
+        raise MXNetError(f"Embedding: the indices are on {idx.device}, the "
+                         f"table is on {W.device}")
     if W.dtype not in _NATIVE_FLOATS:
         out = torch.nn.functional.embedding(idx.long(), W)
         return out if scale == 1.0 else out * scale

@@ -609,7 +609,8 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
                     between 1e-3 and 1e3
     distance_slopes (H,) floats: s -> s - slope_h * |P - j|, after the cap
     segment_ids     (B, Tq) integers: a query sees the keys with its own id;
-                    negative ids are padding that sees and shows nothing
+                    negative ids are padding that sees and shows nothing;
+                    ids are compared in 32 bits
     kv_segment_ids  (B, Tk), the keys' ids; segment_ids if not given
     prefix_length   (B,) integers: with causal, keys below it are seen by all
     kv_length       (B,) integers: keys from there on (a cache's unwritten

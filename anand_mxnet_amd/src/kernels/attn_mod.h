@@ -135,7 +135,7 @@ DEVINL T attn_lds(lds_char* sm, unsigned at) {
 // Whoever reads the tile waits with attn_wait_copies and a barrier.
 DEVINL void copy_lds16(const void* g, unsigned dst) {
   asm volatile(
-      "s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
       :
       : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory");
@@ -143,14 +143,14 @@ DEVINL void copy_lds16(const void* g, unsigned dst) {
 // the same from base + off
 DEVINL void copy_lds16(const void* base, unsigned off, unsigned dst) {
   asm volatile(
-      "s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+      "s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
       :
       : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory");
 }
 DEVINL void copy_lds4(const void* g, unsigned dst) {
   asm volatile(
-      "s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
       :
       : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory");
