@@ -520,9 +520,6 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
         seg_q = _attn_ints(seg_q, (B, Tq), "segment_ids", q)
         seg_k = seg_q if same else _attn_ints(seg_k, (B, Tk),
                                               "kv_segment_ids", q)
-    if prefix is not None and not causal:
-        bad("prefix_length opens a causal mask; without causal=True it has "
-            "no meaning")
     prefix = _attn_ints(prefix, (B,), "prefix_length", q)
     kv_len = _attn_ints(kv_len, (B,), "kv_length", q)
     off0 = 0
@@ -612,7 +609,8 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
                     negative ids are padding that sees and shows nothing;
                     ids are compared in 32 bits
     kv_segment_ids  (B, Tk), the keys' ids; segment_ids if not given
-    prefix_length   (B,) integers: with causal, keys below it are seen by all
+    prefix_length   (B,) integers: with causal, keys below it are seen by
+                    all; without, it changes nothing
     kv_length       (B,) integers: keys from there on (a cache's unwritten
                     part) are not seen and may hold anything
     query_offset    integer or (B,) integers, 0 if not given: the position

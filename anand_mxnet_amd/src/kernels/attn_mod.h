@@ -438,6 +438,15 @@ DEVINL bf16x8 pack8(const float* x) {
   return y;
 }
 
+// x as a bf16 and the bf16 of what that rounding takes: 16 bits of it.
+DEVINL void split8(const float* x, bf16x8& hi, bf16x8& lo) {
+  hi = pack8(x);
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i] - (float)hi[i];
+  lo = pack8(r);
+}
+
 // acc + sum of a[i] * b[i], in 32 bits
 DEVINL float dot8(bf16x8 a, bf16x8 b, float acc) {
 #pragma unroll

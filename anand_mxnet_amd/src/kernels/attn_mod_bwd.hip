@@ -3,6 +3,11 @@
 // With t = tanh(s / cap), P the probabilities and dP = dO V^T:
 //   dS = scale * P * (dP - delta) * (1 - t^2),  delta_i = sum_d dO_i O_i
 //   dV = P^T dO,   dK = dS^T Q,   dQ = dS K
+// P goes into dV rounded to bf16, as it went into O.  dS goes into dQ and dK
+// as the sum of two bf16 numbers: rounded to one, its error is as large as
+// that of rounding dQ and dK themselves, and both products have their other
+// operand in registers already.
+//
 // Two kernels, each of which recomputes the scores: one walks the keys for
 // 128 queries and keeps dQ in registers, the other walks the queries for 128
 // keys and keeps dK and dV.  That is 7 matrix products where one kernel would
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
           attn_mask_keys(x, cur.ids, cur.ends, sm,
                          ID0 + buf * 256 + nb * 128 + 16 * half, sq,
                          limit - j0, attn_gone<CAP>());
-        bf16x8 df[2];
+        bf16x8 df[2], dl[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           float ds[8];
@@ -139,15 +144,17 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
             ds[k] = fexp2(fmaf(x[i], f.mu, off)) * (dp[i] - delta);
             if (CAP) ds[k] *= attn_dtanh(x[i]);
           }
-          df[w] = pack8(ds);
+          split8(ds, df[w], dl[w]);
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int db = 0; db < DB; ++db)
-            dq[db] = mfma32(
-                attn_tr_frag<D>(sm, ktr, db, (nb * 2 + w) * 32 * D), df[w],
-                dq[db]);
+          for (int db = 0; db < DB; ++db) {
+            const bf16x8 kt =
+                attn_tr_frag<D>(sm, ktr, db, (nb * 2 + w) * 32 * D);
+            dq[db] = mfma32(kt, df[w], dq[db]);
+            dq[db] = mfma32(kt, dl[w], dq[db]);
+          }
       }
     }
     cur = nxt;
@@ -365,7 +372,7 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
         const int r0 = nb * 32 + 4 * half;  // this lane's first tile row
         const int p0 = cur.t * 64 + r0 + m.off;
         const float d0 = BIAS ? (float)(p0 - kj) : 0.f;
-        bf16x8 pf[2], df[2];
+        bf16x8 pf[2], df[2], dl[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           float p[8], ds[8];
@@ -405,7 +412,7 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
             }
           }
           pf[w] = pack8(p);
-          df[w] = pack8(ds);
+          split8(ds, df[w], dl[w]);
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w)
@@ -413,8 +420,9 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
           for (int db = 0; db < DB; ++db) {
             dv[db] = mfma32(attn_tr_frag<D>(sm, qtr, db, G0 + w * 32 * D),
                             pf[w], dv[db]);
-            dk[db] = mfma32(attn_tr_frag<D>(sm, qtr, db, w * 32 * D), df[w],
-                            dk[db]);
+            const bf16x8 qt = attn_tr_frag<D>(sm, qtr, db, w * 32 * D);
+            dk[db] = mfma32(qt, df[w], dk[db]);
+            dk[db] = mfma32(qt, dl[w], dk[db]);
           }
       }
     }

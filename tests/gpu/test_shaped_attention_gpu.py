@@ -112,6 +112,7 @@ TRAIN = [
          prefix=[0, 70, 400], slopes=True),
     dict(B=2, Tq=140, Tk=140, H=2, Hkv=2, D=128, causal=True,
          prefix=[5, 100], docs=3, pad=20, cap=10.0),
+    dict(B=2, Tq=100, Tk=100, H=2, Hkv=2, D=64, prefix=[5, 80], cap=10.0),
     # other head sizes
     dict(B=1, Tq=70, Tk=70, H=2, Hkv=2, D=8, causal=True, cap=4.0),
     dict(B=1, Tq=70, Tk=70, H=2, Hkv=1, D=32, causal=True, docs=2, pad=9),

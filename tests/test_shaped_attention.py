@@ -24,6 +24,7 @@ CASES = [
     dict(kv_length=np.array([0, 5]), query_offset=np.array([-1, 3]),
          causal=True),
     dict(query_offset=2, causal=True),
+    dict(prefix_length=np.array([3, 8])),
 ]
 
 
@@ -125,8 +126,7 @@ def _i(*s):
     dict(distance_slopes=_x(3)),
     dict(segment_ids=_x(2, 5)), dict(segment_ids=_i(2, 4)),
     dict(kv_segment_ids=_i(2, 5)),
-    dict(prefix_length=_i(2)),                       # not causal
-    dict(prefix_length=_i(3), causal=True),
+    dict(prefix_length=_i(3), causal=True), dict(prefix_length=_x(2)),
     dict(kv_length=_i(1)), dict(kv_length=7.0),
     dict(query_offset=_i(2, 1)), dict(query_offset=1 << 40),
     dict(logit_cap=5.0, mask=_x(2, 2, 5, 5)),
