@@ -956,7 +956,8 @@ def shaped_mha(q, k, v, num_heads, num_kv_heads, scale, cap, causal, slopes,
                seg_q, seg_k, prefix, kv_len, q_off, off0):
     if q.numel() == 0 or k.shape[1] == 0:
         # nothing to see: zero rows that still belong to the graph
-        return q * 0 + (k.sum() + v.sum()) * 0
+        return (q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0.0)
+                + (k.sum() + v.sum()) * 0)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     conf = (num_heads, num_kv_heads, scale, cap, causal)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad

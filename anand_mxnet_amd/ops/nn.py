@@ -482,7 +482,7 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
     B, Tq, HD = q.shape
     Bk, Tk, KD = k.shape
     H, Hkv = int(num_heads), int(num_kv_heads or num_heads)
-    if H <= 0 or HD % H:
+    if H <= 0 or HD == 0 or HD % H:
         bad(f"{HD} columns do not divide into {H} heads")
     if Hkv <= 0 or H % Hkv:
         bad(f"{H} heads cannot share {Hkv} key heads")
@@ -556,8 +556,9 @@ def _shaped_mha_oracle(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
         if prefix is not None:
             see = see | (j < prefix[:, None].long())[:, None, :]
         ok = ok & see
+        live = live & see.any(1)
     if kv_len is not None:
-        live = j < kv_len[:, None].long()
+        live = live & (j < kv_len[:, None].long())
     if seg_q is not None:
         ok = ok & (seg_q[:, :, None] == seg_k[:, None, :])
         live = live & (seg_k >= 0)
@@ -612,7 +613,9 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
     prefix_length   (B,) integers: with causal, keys below it are seen by
                     all; without, it changes nothing
     kv_length       (B,) integers: keys from there on (a cache's unwritten
-                    part) are not seen and may hold anything
+                    part) are not seen and may hold anything, as may keys
+                    with negative ids and, with causal, those that lie
+                    behind the last query and the prefix
     query_offset    integer or (B,) integers, 0 if not given: the position
                     of the first query among the keys, kv_length - Tq for
                     new tokens at the end of a cache

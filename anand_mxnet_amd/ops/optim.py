@@ -244,6 +244,8 @@ def multi_clip_global_norm(arrays, max_norm, out=None):
             need(isinstance(o, torch.Tensor) and o.shape == a.shape
                  and o.dtype == a.dtype and o.device == a.device,
                  "an output is unlike its array")
+            need(all(n <= 1 or st > 0 for n, st in zip(o.shape, o.stride())),
+                 "an output must not repeat its elements")
         _check_clip_overlap(arrays, out, need)
         if _maybe_hip("multi_clip_global_norm", arrays[0]):
             need(all(a.dtype in (torch.bfloat16, torch.float16,

@@ -60,12 +60,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
   Stager<D, 64, 4> ks, vs;
   ks.init(a.kst, wave, lane);
   vs.init(a.vst, wave, lane);
+  // keys that no query of the block sees may hold anything
+  const int kend = max(attn_limit(m, blk.pmax), 0);
   auto stage = [&](int buf, const Tile& t) {
     const int* sg = t.neg ? skb : nullptr;
     const int r = t.t * 64;
-    ks.copy(kb, a.kst, r, m.kv_len, a.D, sg, lds0 + buf * TILE, wave, lane);
-    vs.copy(vb, a.vst, r, m.kv_len, a.D, sg, lds0 + V0 + buf * TILE, wave,
-            lane);
+    ks.copy(kb, a.kst, r, kend, a.D, sg, lds0 + buf * TILE, wave, lane);
+    vs.copy(vb, a.vst, r, kend, a.D, sg, lds0 + V0 + buf * TILE, wave, lane);
     if (m.has_seg && wave == 0)
       attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
   };
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 
   const LaneAddr la = attn_lane_addr<D>(lane);
   TileWalk walk;
-  walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
+  walk.start(0, cdiv(kend, 64));
   Tile cur = walk.next(m, blk, wav, rng, lane);
   if (cur.t >= 0) stage(0, cur);
   // queries, their output gradients and delta
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
   const int kj = k0 + col;
   int sk = 0;
   if (m.has_seg) sk = kj < a.Tk ? a.seg_k[(long)b * a.Tk + kj] : -1;
-  const bool kok = kj < m.kv_len && sk >= 0;
+  const bool kok = kj < m.kv_len && sk >= 0 &&
+                   (!m.causal || kj < m.prefix || kj < a.Tq + m.off);
   // first position that sees this key (documents aside)
   const int NEVER = 0x7fffffff;
   const int first =

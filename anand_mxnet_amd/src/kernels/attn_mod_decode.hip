@@ -51,7 +51,8 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
   ScoreFn f;
   f.set<CAP>(a.scale, a.cap, BIAS && ok ? a.slopes[h] : 0.f);
   // this block's tiles: an equal share of what the sequence has
-  const int nt = cdiv(max(attn_limit(m, pmax), 0), 32);
+  const int kend = max(attn_limit(m, pmax), 0);  // nobody sees the rest
+  const int nt = cdiv(kend, 32);
   const int share = cdiv(nt, a.nsplit);
   const int t1 = min(nt, (sp + 1) * share);
   int t = sp * share + wave;
@@ -65,13 +66,11 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
   // the wave's own reads of a tile end before the next one is copied over it
   auto stage_k = [&](int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    ks.copy(kb, a.kst, tile * 32, m.kv_len, a.D, nullptr, lds0 + kat, 0,
-            lane);
+    ks.copy(kb, a.kst, tile * 32, kend, a.D, nullptr, lds0 + kat, 0, lane);
   };
   auto stage_v = [&](int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    vs.copy(vb, a.vst, tile * 32, m.kv_len, a.D, nullptr, lds0 + vat, 0,
-            lane);
+    vs.copy(vb, a.vst, tile * 32, kend, a.D, nullptr, lds0 + vat, 0, lane);
   };
 
   f32x16 o[DB];

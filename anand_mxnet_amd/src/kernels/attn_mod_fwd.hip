@@ -87,12 +87,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
   Stager<D, 64, 4> ks, vs;
   ks.init(a.kst, wave, lane);
   vs.init(a.vst, wave, lane);
+  // keys that no query of the block sees may hold anything
+  const int kend = max(attn_limit(m, blk.pmax), 0);
   auto stage = [&](int buf, const Tile& t) {
     const int* sg = t.neg ? skb : nullptr;
     const int r = t.t * 64;
-    ks.copy(kb, a.kst, r, m.kv_len, a.D, sg, lds0 + buf * TILE, wave, lane);
-    vs.copy(vb, a.vst, r, m.kv_len, a.D, sg, lds0 + V0 + buf * TILE, wave,
-            lane);
+    ks.copy(kb, a.kst, r, kend, a.D, sg, lds0 + buf * TILE, wave, lane);
+    vs.copy(vb, a.vst, r, kend, a.D, sg, lds0 + V0 + buf * TILE, wave, lane);
     if (m.has_seg && wave == 0)
       attn_stage64(skb, t.t * 64, a.Tk, lds0 + ID0 + buf * 256, lane);
   };
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
 
   const LaneAddr la = attn_lane_addr<D>(lane);
   TileWalk walk;
-  walk.start(0, cdiv(max(attn_limit(m, blk.pmax), 0), 64));
+  walk.start(0, cdiv(kend, 64));
   Tile cur = walk.next(m, blk, wav, rng, lane);
   if (cur.t >= 0) stage(0, cur);
   bf16x8 qf[KK];

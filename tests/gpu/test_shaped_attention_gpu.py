@@ -224,6 +224,32 @@ def test_unseen_places_may_hold_anything():
     check("decode", _infer(c), ref["out"])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Tq,off", [(3, 50), (70, 41), (150, 3)])
+def test_keys_behind_the_last_query(D, Tq, off):
+    """A cache without kv_length whose rest was never written."""
+    from anand_mxnet_amd import _C
+    last = off + Tq
+    for prefix in (None, [last + 7, 0]):
+        c = _case(9, 2, Tq, 230, 4, 2, D, causal=True, cap=10.0,
+                  prefix=prefix, off=[off, off - 2])
+        ref = _ref(c)
+        for key in ("k", "v"):
+            c[key][0, last + (7 if prefix else 0):] = float("nan")
+            c[key][1, last - 2:] = float("inf")
+        got = _train(c)
+        for name in ref:
+            check(name, got[name], ref[name])
+        check("infer", _infer(c), ref["out"])
+        pre = None if prefix is None else _nd(c["prefix"])._t
+        args = (_nd(c["q"])._t, _nd(c["k"])._t, _nd(c["v"])._t, 4, 2,
+                D ** -0.5, 10.0, True, None)
+        opts = (pre, None, _nd(c["off"])._t, 0)
+        check("split", _C.attn_decode(*args, *opts), ref["out"])
+        check("blocks", _C.attn_mod_fwd(*args, None, None, *opts, False)[0],
+              ref["out"])
+
+
 def test_strided_operands():
     """Slices of one fused projection, a transposed batch, odd offsets."""
     import anand_mxnet_amd as mx
@@ -338,6 +364,11 @@ def test_empty():
         for t in got.values():
             assert not t.any()
         assert not _infer(c).any()
+    c = _case(12, 2, 4, 0, 2, 2, 64, cap=5.0)
+    c["q"][:, 1] = float("nan")   # sees nothing all the same
+    assert not _infer(c).any()
+    for t in _train(c).values():
+        assert not t.any()
 
 
 def test_refuses_on_gpu():

@@ -1,13 +1,16 @@
 """Attention with shaped scores in 64 bits, with elementwise bounds on what a
-kernel that holds P and dS in bfloat16 and sums in 32 bits may be off.
+kernel that holds P in bfloat16 and sums in 32 bits may be off.
 
 A rounding to bfloat16 is off by at most h = 2**-8 of the value.  With
 absolute sums S(x) of the terms of a product:
   out    P is rounded once, the result once:   h P|V| + h |out|
   dV     P is rounded, the result:             h P^T|dO| + h |dV|
-  delta  sum of dO * (rounded out):            e_d = sum_d |dO| err(out)
-  dS     P (dP - delta) u, rounded:            e_s = u P e_d + h |dS|
+  delta  sum of dO * out:                      e_d = sum_d |dO| err(out)
+  dS     P (dP - delta) u:                     e_s = u P e_d + h |dS|
   dQ     scale (e_s |K|) + h |dQ|              dK: scale (e_s^T |Q|) + h |dK|
+The kernels divide by the sum of the rounded P, whose mean rounding m <= h
+they keep in the log-sum as well: dS is off by m |dS|, which is the term
+h |dS| (dS itself goes on as two bfloat16, 2**-16 of it).
 The 32-bit sums add n * 2**-24 of the absolute sum, the hardware's exp2 and
 reciprocal and the tanh 2e-5 of a probability at these sizes: both are covered
 by 10 per cent on every bound (0.1 * 2**-8 = 4e-4) and 1e-6 for sums that

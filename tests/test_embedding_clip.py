@@ -67,6 +67,7 @@ def test_clip_refuses():
     for arrays, kw in [
             ([], {}), ([w(x), w(x)], {}), ([w(x[:6]), w(x[5:])], {}),
             ([w(x)], dict(out=[])), ([w(x.int())], {}),
+            ([w(torch.ones(1).expand(10))], {}),
             ([w(x)], dict(out=[w(torch.ones(9))])),
             ([w(x)], dict(out=[w(torch.ones(10).double())])),
             ([w(x[:5]), w(x[5:])], dict(out=[w(x[5:]), w(x[:5])]))]:

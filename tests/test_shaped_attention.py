@@ -108,6 +108,10 @@ def test_nan_in_unseen_places():
         nd.from_torch(q), nd.from_torch(k), nd.from_torch(k), 2,
         kv_length=nd.from_torch(torch.tensor([3])))
     assert torch.isfinite(out._t).all()
+    out = nd.multi_head_attention(      # two queries before the last key
+        nd.from_torch(q[:, :2]), nd.from_torch(k), nd.from_torch(k), 2,
+        causal=True, query_offset=1)
+    assert torch.isfinite(out._t).all()
 
 
 def _x(*s):
@@ -148,6 +152,8 @@ def test_refuses_more():
         f(q, _x(3, 5, 16), _x(3, 5, 16), 2, logit_cap=1.0)
     with pytest.raises(MXNetError):
         f(_x(2, 5, 15), q, q, 2, logit_cap=1.0)
+    with pytest.raises(MXNetError):                  # heads of no columns
+        f(_x(2, 5, 0), _x(2, 5, 0), _x(2, 5, 0), 2, logit_cap=1.0)
     s = nd.from_torch(torch.zeros(2))
     s.attach_grad()
     with pytest.raises(MXNetError):
