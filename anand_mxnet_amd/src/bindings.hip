@@ -1241,10 +1241,10 @@ std::vector<at::Tensor> attn_mod_fwd(
 std::vector<at::Tensor> attn_mod_bwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& out, const at::Tensor& dout, const at::Tensor& lse,
-    const at::Tensor& lo, const OptT& rng_q, const OptT& rng_k, long H, long Hkv, double scale,
-    double cap, bool causal, const OptT& slopes, const OptT& seg_q,
-    const OptT& seg_k, const OptT& prefix, const OptT& kv_len,
-    const OptT& q_off, long off0, bool need_kv) {
+    const at::Tensor& lo, const OptT& rng_q, const OptT& rng_k, long H,
+    long Hkv, double scale, double cap, bool causal, const OptT& slopes,
+    const OptT& seg_q, const OptT& seg_k, const OptT& prefix,
+    const OptT& kv_len, const OptT& q_off, long off0, bool need_kv) {
   c10::DeviceGuard guard(q.device());
   auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
                      seg_k, prefix, kv_len, q_off, off0);
@@ -1501,7 +1501,8 @@ at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
   const long ntok = ix.numel(), D = dy.size(-1);
   TORCH_CHECK(dy.numel() == ntok * D,
               "embedding: one gradient row for each index");
-  TORCH_CHECK(vocab < 0x7fffffff && ntok < 0x7fffff00 && D < 0x7fffffff,
+  // places are 32 bits wide, and a batch of tokens may reach past the last
+  TORCH_CHECK(vocab < 0x7fffffff && ntok < 0x7ffff000 && D < 0x7fffffff,
               "embedding: too large");
   if (ntok == 0) return at::zeros({vocab, D}, dy.options());
   auto dW = at::empty({vocab, D}, dy.options());

@@ -154,6 +154,15 @@ def test_embedding_graph_replays():
         assert torch.equal(dw, _C.embedding_bwd(s[0], s[2], 800, 2.0))
 
 
+def test_embedding_refuses_too_many_tokens():
+    """Places in the order of the tokens are 32 bits wide."""
+    from anand_mxnet_amd import _C
+    idx = torch.empty(0x7ffff000, dtype=torch.int32, device="cuda")
+    dy = torch.empty(0x7ffff000, 0, device="cuda")
+    with pytest.raises(RuntimeError, match="too large"):
+        _C.embedding_bwd(idx, dy, 10, 1.0)
+
+
 # ------------------------------------------------------------------ clip
 
 def _shapes(n, rng):
@@ -248,6 +257,19 @@ def test_clip_extremes():
     assert not o.any()
     e = [nd(torch.zeros(0, device="cuda")), nd(torch.ones(4, device="cuda"))]
     assert float(f(e, 10.0)._t) == 2.0
+
+
+def test_clip_more_elements_than_32_bits():
+    import anand_mxnet_amd as mx
+    n = (1 << 32) + 1003
+    x = torch.full((n,), 0.25, dtype=torch.bfloat16, device="cuda")
+    norm = mx.nd.multi_clip_global_norm([mx.nd.from_torch(x)], 1e6)
+    assert abs(float(norm._t) / (0.25 * n ** 0.5) - 1) < 2.0 ** -23
+    assert float(x[0]) == float(x[-1]) == 0.25
+    max_norm = float(norm._t) / 2        # the factor is 1/2 within 2**-23
+    mx.nd.multi_clip_global_norm([mx.nd.from_torch(x)], max_norm)
+    lo, hi = torch.aminmax(x)
+    assert float(lo) == float(hi) == 0.125
 
 
 def test_clip_graph_replays():
