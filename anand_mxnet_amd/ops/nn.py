@@ -19,6 +19,7 @@ import torch.nn.functional as F
 
 from .registry import register, gpu_impl, has_gpu_impl
 from .. import autograd as _ag
+from ..base import MXNetError
 
 
 def _allow_fallback() -> bool:
@@ -456,7 +457,6 @@ def _attn_ints(x, shape, what, q):
     device."""
     if x is None:
         return None
-    from ..base import MXNetError
     if not isinstance(x, torch.Tensor) or x.dtype.is_floating_point \
             or x.dtype.is_complex or x.dtype == torch.bool:
         raise MXNetError(f"multi_head_attention: {what} must be an integer "
@@ -467,6 +467,8 @@ def _attn_ints(x, shape, what, q):
     if x.device != q.device:
         raise MXNetError(f"multi_head_attention: {what} is on {x.device}, "
                          f"the queries are on {q.device}")
+    if x.dtype is torch.int32 and x.is_contiguous():
+        return x
     return x.to(torch.int32).contiguous()
 
 
@@ -474,7 +476,6 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
                 causal, seg_q, seg_k, prefix, kv_len, q_off):
     """Checks and dispatch of the shaped forms of multi_head_attention."""
     def bad(what):
-        from ..base import MXNetError
         raise MXNetError("multi_head_attention: " + what)
 
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
@@ -624,12 +625,12 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
     queries outside autograd.record() take the form that splits the keys
     over the chip.  Positions count exactly up to 2**24.  These forms take
     neither a dense mask nor dropout."""
-    shaped = any(x is not None for x in (
-        logit_cap, distance_slopes, segment_ids, kv_segment_ids,
-        prefix_length, kv_length, query_offset)) or (
-        num_kv_heads is not None and int(num_kv_heads) != int(num_heads))
-    if shaped:
-        from ..base import MXNetError
+    if (kv_length is not None or segment_ids is not None
+            or logit_cap is not None or distance_slopes is not None
+            or prefix_length is not None or query_offset is not None
+            or kv_segment_ids is not None
+            or num_kv_heads is not None
+            and int(num_kv_heads) != int(num_heads)):
         if mask is not None:
             raise MXNetError("multi_head_attention: a dense mask cannot be "
                              "combined with shaped scores")

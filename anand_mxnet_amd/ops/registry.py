@@ -41,9 +41,12 @@ def _unwrap(x):
 
 
 def _wrap_out(out):
+    global _NDArray
     if isinstance(out, torch.Tensor):
-        from ..ndarray.ndarray import NDArray
-        return NDArray(out)
+        if _NDArray is None:
+            from ..ndarray.ndarray import NDArray
+            _NDArray = NDArray
+        return _NDArray(out)
     if isinstance(out, (list, tuple)):
         return [_wrap_out(o) for o in out]
     return out
