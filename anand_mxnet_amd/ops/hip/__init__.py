@@ -711,21 +711,6 @@ def dropout(x, p):
     return _Dropout.apply(x, p)
 
 
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, idx, W, scale):
-        ctx.save_for_backward(idx)
-        ctx.vocab = W.shape[0]
-        ctx.scale = scale
-        return _C.embedding_fwd(idx, W.contiguous(), scale)
-
-    @staticmethod
-    def backward(ctx, dy):
-        (idx,) = ctx.saved_tensors
-        return None, _C.embedding_bwd(idx, dy.contiguous(), ctx.vocab,
-                                      ctx.scale), None
-
-
 _NATIVE_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -738,7 +723,7 @@ def embedding(idx, W, scale=1.0):
     if W.dtype not in _NATIVE_FLOATS:
         out = torch.nn.functional.embedding(idx.long(), W)
         return out if scale == 1.0 else out * scale
-    return _Embedding.apply(idx, W, scale)
+    return _C.embedding(idx, W, scale)
 
 
 _ACT_IDS = {"relu": 0, "sigmoid": 1, "tanh": 2, "gelu": 3, "silu": 4,
@@ -905,42 +890,6 @@ class _FlashMha(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
-def _rows16(t):
-    """The tensor itself if the kernels can read its rows 16 bytes at a
-    time (any batch stride, rows up to 2**25 elements apart), else a packed
-    copy."""
-    if (t.stride(2) == 1 and t.stride(1) % 8 == 0 and t.stride(0) % 8 == 0
-            and 0 <= t.stride(1) < 1 << 25 and t.data_ptr() % 16 == 0):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-class _ShapedMha(torch.autograd.Function):
-    """Attention with shaped scores (attn_mod_fwd.hip, attn_mod_bwd.hip):
-    the backward recomputes the scores from the saved log-sums; nothing is
-    summed through atomics, so it gives the same bits every time."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, conf, slopes, seg_q, seg_k, prefix, kv_len,
-                q_off, off0):
-        opts = (slopes, seg_q, seg_k, prefix, kv_len, q_off)
-        out, lse, lo, *rng = _C.attn_mod_fwd(q, k, v, *conf, *opts, off0,
-                                             True)
-        ctx.save_for_backward(q, k, v, out, lse, lo, *opts, *rng)
-        ctx.conf = conf
-        ctx.off0 = off0
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        q, k, v, out, lse, lo, *rest = ctx.saved_tensors
-        opts, rng = rest[:6], (rest[6:] or [None, None])
-        need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        grads = _C.attn_mod_bwd(q, k, v, out, _rows16(dout), lse, lo, *rng,
-                                *ctx.conf, *opts, ctx.off0, need_kv)
-        return tuple(grads) + (None,) * (11 - len(grads))
-
-
 def _split_keys(B, Tq, H, G):
     """Whether the form that divides the keys over the chip is taken, rather
     than 128 queries a block: for few rows (query tokens times heads of a
@@ -958,12 +907,11 @@ def shaped_mha(q, k, v, num_heads, num_kv_heads, scale, cap, causal, slopes,
         # nothing to see: zero rows that still belong to the graph
         return (q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0.0)
                 + (k.sum() + v.sum()) * 0)
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
     conf = (num_heads, num_kv_heads, scale, cap, causal)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
                                     or v.requires_grad):
-        return _ShapedMha.apply(q, k, v, conf, slopes, seg_q, seg_k, prefix,
-                                kv_len, q_off, off0)
+        return _C.attn_mod(q, k, v, *conf, slopes, seg_q, seg_k, prefix,
+                           kv_len, q_off, off0)
     if seg_q is None and _split_keys(q.shape[0], q.shape[1], num_heads,
                                      num_heads // num_kv_heads):
         return _C.attn_decode(q, k, v, *conf, slopes, prefix, kv_len, q_off,

@@ -1186,6 +1186,16 @@ mxa::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k,
   return a;
 }
 
+// The tensor itself if the kernels can read its rows 16 bytes at a time (any
+// batch stride, rows up to 2**25 elements apart), else a packed copy.
+at::Tensor attn_rows(const at::Tensor& t) {
+  if (t.dim() == 3 && t.stride(2) == 1 && t.stride(1) % 8 == 0 &&
+      t.stride(0) % 8 == 0 && t.stride(1) >= 0 &&
+      t.stride(1) < (1L << 25) && (size_t)t.data_ptr() % 16 == 0)
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
 at::Tensor attn_ranges(const int* seg, long B, long T,
                        const at::Tensor& like) {
   auto r = at::empty({B, (T + 127) / 128 * 4, 2},
@@ -1200,11 +1210,12 @@ at::Tensor attn_ranges(const int* seg, long B, long T,
 // the log2 sums, what rounding took from the output, and (with ids) the id
 // ranges of queries and keys.
 std::vector<at::Tensor> attn_mod_fwd(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, long H,
+    const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, long H,
     long Hkv, double scale, double cap, bool causal, const OptT& slopes,
     const OptT& seg_q, const OptT& seg_k, const OptT& prefix,
     const OptT& kv_len, const OptT& q_off, long off0, bool with_stats) {
-  c10::DeviceGuard guard(q.device());
+  c10::DeviceGuard guard(q_.device());
+  const auto q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_);
   auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
                      seg_k, prefix, kv_len, q_off, off0);
   TORCH_CHECK(a.B > 0 && a.Tq > 0 && a.Tk > 0, "attention: empty");
@@ -1240,12 +1251,13 @@ std::vector<at::Tensor> attn_mod_fwd(
 
 std::vector<at::Tensor> attn_mod_bwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-    const at::Tensor& out, const at::Tensor& dout, const at::Tensor& lse,
+    const at::Tensor& out, const at::Tensor& dout_, const at::Tensor& lse,
     const at::Tensor& lo, const OptT& rng_q, const OptT& rng_k, long H,
     long Hkv, double scale, double cap, bool causal, const OptT& slopes,
     const OptT& seg_q, const OptT& seg_k, const OptT& prefix,
     const OptT& kv_len, const OptT& q_off, long off0, bool need_kv) {
   c10::DeviceGuard guard(q.device());
+  const auto dout = attn_rows(dout_);
   auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
                      seg_k, prefix, kv_len, q_off, off0);
   attn_operand(out, q, "output");
@@ -1294,12 +1306,68 @@ std::vector<at::Tensor> attn_mod_bwd(
   return res;
 }
 
-at::Tensor attn_decode(const at::Tensor& q, const at::Tensor& k,
-                       const at::Tensor& v, long H, long Hkv, double scale,
+// Differentiable form of attn_mod_fwd: the backward recomputes the scores
+// from the saved log-sums.  A native function rather than one in Python: a
+// short batch's time is the host's.
+class ShapedMha : public torch::autograd::Function<ShapedMha> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx,
+                            const at::Tensor& q_, const at::Tensor& k_,
+                            const at::Tensor& v_, long H, long Hkv,
+                            double scale, double cap, bool causal,
+                            const OptT& slopes, const OptT& seg_q,
+                            const OptT& seg_k, const OptT& prefix,
+                            const OptT& kv_len, const OptT& q_off,
+                            long off0) {
+    c10::DeviceGuard guard(q_.device());
+    const auto q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_);
+    auto r = attn_mod_fwd(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
+                          seg_k, prefix, kv_len, q_off, off0, true);
+    auto some = [](const OptT& t) { return t.value_or(at::Tensor()); };
+    ctx->save_for_backward({q, k, v, r[0], r[1], r[2], some(slopes),
+                            some(seg_q), some(seg_k), some(prefix),
+                            some(kv_len), some(q_off),
+                            r.size() > 3 ? r[3] : at::Tensor(),
+                            r.size() > 3 ? r[4] : at::Tensor()});
+    ctx->saved_data["conf"] = std::vector<int64_t>{H, Hkv, causal, off0};
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["cap"] = cap;
+    return r[0];
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grad) {
+    auto s = ctx->get_saved_variables();
+    auto opt = [&](int i) { return s[i].defined() ? OptT(s[i]) : OptT(); };
+    const auto c = ctx->saved_data["conf"].toIntVector();
+    auto g = attn_mod_bwd(
+        s[0], s[1], s[2], s[3], grad[0], s[4], s[5], opt(12), opt(13), c[0],
+        c[1], ctx->saved_data["scale"].toDouble(),
+        ctx->saved_data["cap"].toDouble(), c[2] != 0, opt(6), opt(7), opt(8),
+        opt(9), opt(10), opt(11), c[3],
+        ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+    g.resize(15);  // nothing for the other arguments
+    return g;
+  }
+};
+
+at::Tensor attn_mod(const at::Tensor& q, const at::Tensor& k,
+                    const at::Tensor& v, long H, long Hkv, double scale,
+                    double cap, bool causal, const OptT& slopes,
+                    const OptT& seg_q, const OptT& seg_k, const OptT& prefix,
+                    const OptT& kv_len, const OptT& q_off, long off0) {
+  return ShapedMha::apply(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
+                          seg_k, prefix, kv_len, q_off, off0);
+}
+
+at::Tensor attn_decode(const at::Tensor& q_, const at::Tensor& k_,
+                       const at::Tensor& v_, long H, long Hkv, double scale,
                        double cap, bool causal, const OptT& slopes,
                        const OptT& prefix, const OptT& kv_len,
                        const OptT& q_off, long off0) {
-  c10::DeviceGuard guard(q.device());
+  c10::DeviceGuard guard(q_.device());
+  const auto q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_);
   auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, {}, {},
                      prefix, kv_len, q_off, off0);
   TORCH_CHECK(a.B > 0 && a.Tq > 0 && a.Tk > 0, "attention: empty");
@@ -1518,6 +1586,35 @@ at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
                 (int2*)sorted.data_ptr<int>(), part.data_ptr<float>(),
                 (int)ntok, (int)D, (int)vocab, (float)scale, cur_stream());
   return dW;
+}
+
+// The differentiable lookup, native for the host's time of a small batch.
+class EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx,
+                            const at::Tensor& idx, const at::Tensor& W,
+                            double scale) {
+    ctx->save_for_backward({idx});
+    ctx->saved_data["vocab"] = W.size(0);
+    ctx->saved_data["scale"] = scale;
+    return embedding_fwd(idx, W.contiguous(), scale);
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grad) {
+    return {at::Tensor(),
+            embedding_bwd(ctx->get_saved_variables()[0],
+                          grad[0].contiguous(),
+                          ctx->saved_data["vocab"].toInt(),
+                          ctx->saved_data["scale"].toDouble()),
+            at::Tensor()};
+  }
+};
+
+at::Tensor embedding(const at::Tensor& idx, const at::Tensor& W,
+                     double scale) {
+  return EmbeddingFn::apply(idx, W, scale);
 }
 
 // Writes src[i] * min(1, max_norm / (norm + 1e-8)) to dst[i] (which may be
@@ -2002,6 +2099,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_wg", &attn_wg);
   m.def("attn_mod_fwd", &attn_mod_fwd);
   m.def("attn_mod_bwd", &attn_mod_bwd);
+  m.def("attn_mod", &attn_mod);
   m.def("attn_decode", &attn_decode);
   m.def("flash_fwd", &flash_fwd);
   m.def("flash_bwd", &flash_bwd);
@@ -2010,6 +2108,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("softmax_dropout_fwd", &softmax_dropout_fwd);
   m.def("softmax_dropout_bwd", &softmax_dropout_bwd);
   m.def("dropout_bwd", &dropout_bwd);
+  m.def("embedding", &embedding);
   m.def("embedding_fwd", &embedding_fwd, py::arg("idx"), py::arg("W"),
         py::arg("scale") = 1.0);
   m.def("embedding_bwd", &embedding_bwd, py::arg("idx"), py::arg("dy"),
