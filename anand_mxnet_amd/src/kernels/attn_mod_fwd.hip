@@ -134,6 +134,18 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
         for (int nb = 0; nb < 2; ++nb)
           s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
                          s[nb]);
+      if (D == 128) {
+        // eight reads of K ahead of the products: 16384 tokens, 16 heads
+        // of 128 took 631 us with the two to four that the compiler keeps
+        // in flight, 617 us like this, no less with twelve
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
+      }
 
       const int j0 = cur.t * 64 + 4 * half;
       float x[32];
