@@ -298,7 +298,7 @@ DEVINL int2 attn_join(int2 x, int2 y) {
 
 struct Tile {
   int t;      // index of 64 keys; negative: no more
-  bool work;  // this wave has pairs in it
+  int work;   // the halves of it in which this wave has pairs, as two bits
   bool ids;   // its queries' and keys' ids are not all the same
   bool ends;  // some queries' last visible key lies in it
   bool neg;   // some ids are negative: stage with care
@@ -308,32 +308,39 @@ struct Tile {
 // tile to a lane, and the verdicts are kept as bits.
 struct TileWalk {
   int base, nt;
-  u64 act, wact, wone, wend, neg;
+  u64 act, wact[2], wone, wend, neg;
 
   DEVINL void start(int first, int ntiles) {
     base = first - 64;
     nt = ntiles;
-    act = wact = wone = wend = neg = 0;
+    act = wact[0] = wact[1] = wone = wend = neg = 0;
   }
   DEVINL Tile next(const SeqMask& m, const RowSpan& blk, const RowSpan& wav,
                    const int2* rng, int lane) {
     while (act == 0) {
       base += 64;
-      if (base >= nt) return Tile{-1, false, false, false, false};
+      if (base >= nt) return Tile{-1, 0, false, false, false};
       int t = base + lane;
-      int2 r = make_int2(0, 0);
+      int2 r0 = make_int2(0, 0), r1 = r0;
       bool in = t < nt;
-      if (in && m.has_seg) r = attn_join(rng[2 * t], rng[2 * t + 1]);
+      if (in && m.has_seg) {
+        r0 = rng[2 * t];
+        r1 = rng[2 * t + 1];
+      }
+      const int2 r = attn_join(r0, r1);
       act = __ballot(in && attn_tile_any(m, blk, t * 64, r));
-      wact = __ballot(in && wav.pmax != -0x7fffffff &&
-                      attn_tile_any(m, wav, t * 64, r));
+      const bool some = in && wav.pmax != -0x7fffffff;
+      wact[0] = __ballot(some && attn_tile_any(m, wav, t * 64, r0));
+      wact[1] = __ballot(some && attn_tile_any(m, wav, t * 64 + 32, r1));
       wone = __ballot(in && attn_tile_one(m, wav, r));
       wend = __ballot(in && t * 64 + 64 > attn_limit(m, wav.pmin));
       neg = __ballot(in && m.has_seg && r.x < 0);
     }
     int i = __builtin_ctzll(act);
     act &= act - 1;
-    return Tile{base + i, (bool)((wact >> i) & 1), !((wone >> i) & 1),
+    return Tile{base + i,
+                (int)((wact[0] >> i) & 1) | (int)((wact[1] >> i) & 1) << 1,
+                !((wone >> i) & 1),
                 (bool)((wend >> i) & 1), (bool)((neg >> i) & 1)};
   }
 };

@@ -16,6 +16,8 @@
 // The running maximum moves only when some row's scores pass it by more
 // than 8 (a factor of 256, harmless in fp32 sums and bf16 probabilities), so
 // the rescaling of the accumulators is skipped for almost every tile.
+#include <type_traits>
+
 #include "attn_mod.h"
 
 namespace mxa {
@@ -47,8 +49,12 @@ void attn_seg_ranges(const int* seg, int2* out, int B, int T,
       seg, out, T, nr, total);
 }
 
-template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
+// SHORT: a wave takes the halves of a tile one by one, skips those that it
+// has no pairs in, and holds half as many scores: 116 registers, four blocks
+// on a compute unit.
+template <int D, bool CAP, bool BIAS, bool SHORT>
+__global__ __launch_bounds__(256, SHORT ? 4 : 2) void attn_mod_fwd_kernel(
+    AttnArgs a) {
   constexpr int KK = D / 16, DB = D / 32;
   // K and V tiles, two buffers of each; then the tiles' ids
   constexpr int TILE = 128 * D, V0 = 2 * TILE, ID0 = 4 * TILE;
@@ -118,106 +124,117 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) attn_settle(qf[kk]);
   }
+  // NH times 32 keys of a tile, from its half nb0 on
+  auto part = [&](auto nh, const Tile& cur, int buf, int nb0) {
+    constexpr int NH = decltype(nh)::value, N = 16 * NH;
+    const unsigned krow = la.row + buf * TILE + nb0 * 64 * D;
+    const unsigned vtr = la.tr + buf * TILE + nb0 * 64 * D;
+    const unsigned ids = ID0 + buf * 256 + 16 * half + nb0 * 128;
+    f32x16 s[NH];
+#pragma unroll
+    for (int nb = 0; nb < NH; ++nb) s[nb] = zero16();
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int nb = 0; nb < NH; ++nb)
+        s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
+                       s[nb]);
+    if (D == 128) {
+      // eight reads of K ahead of the products: 16384 tokens, 16 heads
+      // of 128 took 631 us with the two to four that the compiler keeps
+      // in flight, 617 us like this, no less with twelve
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
+    }
+
+    const int j0 = cur.t * 64 + nb0 * 32 + 4 * half;
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = attn_z<CAP>(f, s[i >> 4][i & 15]);
+    if (cur.ids || cur.ends) {
+#pragma unroll
+      for (int nb = 0; nb < NH; ++nb)
+        attn_mask_keys(x + 16 * nb, cur.ids, cur.ends, sm, ids + 128 * nb, sq,
+                       limit - j0 - 32 * nb, -MXA_INF);
+    }
+    // with a bias, x[i] + base + (i >> 2) * step becomes the score.  The
+    // bias is linear in j where all keys of the tile lie before the wave's
+    // queries: one addition for each four keys there.
+    float mx = -MXA_INF, base = 0.f, step = 0.f;
+    if (BIAS) {
+      const float d0 = (float)(pos - j0);
+      if (cur.t * 64 + 63 <= wav.pmin) {
+        base = f.slope * d0;
+        step = -8.f * f.slope;
+        const float e[4] = {0.f, -f.slope, -2.f * f.slope, -3.f * f.slope};
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], f.mu, e[i & 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          x[i] = fmaf(x[i], f.mu,
+                      f.slope * fabsf(d0 - (float)(8 * (i >> 2) + (i & 3))));
+      }
+#pragma unroll
+      for (int g = 0; g < N / 4; ++g)
+        mx = fmaxf(mx, fmaf((float)g, step,
+                            fmaxf(fmaxf(x[4 * g], x[4 * g + 1]),
+                                  fmaxf(x[4 * g + 2], x[4 * g + 3]))));
+      mx += base;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) mx = fmaxf(mx, x[i]);
+      mx *= f.mu;
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__ballot(mx > mrow + 8.f)) {
+      float mnew = fmaxf(mrow, mx);
+      float al = fexp2(mrow - mnew);
+      mrow = mnew;
+      lsum *= al;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] *= al;
+    }
+    bf16x8 pf[2 * NH];
+#pragma unroll
+    for (int st = 0; st < 2 * NH; ++st) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int g = 2 * st + (i >> 2);
+        p[i] = BIAS ? fexp2(x[8 * st + i] - (mrow - base - (float)g * step))
+                    : fexp2(fmaf(x[8 * st + i], f.mu, -mrow));
+      }
+      pf[st] = pack8(p);
+      lsum = dot8(pf[st], ones8(), lsum);
+    }
+#pragma unroll
+    for (int st = 0; st < 2 * NH; ++st)
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, V0 + st * 32 * D),
+                       pf[st], o[db]);
+  };
   int buf = 0;
   while (cur.t >= 0) {
     attn_wait_copies<0>();
     __syncthreads();  // this tile has landed, the other buffer is free
     Tile nxt = walk.next(m, blk, wav, rng, lane);
     if (nxt.t >= 0) stage(buf ^ 1, nxt);
-    if (cur.work) {
-      const unsigned krow = la.row + buf * TILE, vtr = la.tr + buf * TILE;
-      const unsigned ids = ID0 + buf * 256 + 16 * half;
-      f32x16 s[2] = {zero16(), zero16()};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-          s[nb] = mfma32(attn_row_frag(sm, krow, kk, nb * 64 * D), qf[kk],
-                         s[nb]);
-      if (D == 128) {
-        // eight reads of K ahead of the products: 16384 tokens, 16 heads
-        // of 128 took 631 us with the two to four that the compiler keeps
-        // in flight, 617 us like this, no less with twelve
-        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
-      }
-
-      const int j0 = cur.t * 64 + 4 * half;
-      float x[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        x[i] = attn_z<CAP>(f, s[i >> 4][i & 15]);
-      if (cur.ids || cur.ends) {
-        attn_mask_keys(x, cur.ids, cur.ends, sm, ids, sq, limit - j0,
-                       -MXA_INF);
-        attn_mask_keys(x + 16, cur.ids, cur.ends, sm, ids + 128, sq,
-                       limit - j0 - 32, -MXA_INF);
-      }
-      // with a bias, x[i] + base + (i >> 2) * step becomes the score.  The
-      // bias is linear in j where all keys of the tile lie before the wave's
-      // queries: one addition for each four keys there.
-      float mx = -MXA_INF, base = 0.f, step = 0.f;
-      if (BIAS) {
-        const float d0 = (float)(pos - j0);
-        if (cur.t * 64 + 63 <= wav.pmin) {
-          base = f.slope * d0;
-          step = -8.f * f.slope;
-          const float e[4] = {0.f, -f.slope, -2.f * f.slope, -3.f * f.slope};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], f.mu, e[i & 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            x[i] = fmaf(x[i], f.mu,
-                        f.slope *
-                            fabsf(d0 - (float)(8 * (i >> 2) + (i & 3))));
-        }
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-          mx = fmaxf(mx, fmaf((float)g, step,
-                              fmaxf(fmaxf(x[4 * g], x[4 * g + 1]),
-                                    fmaxf(x[4 * g + 2], x[4 * g + 3]))));
-        mx += base;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
-        mx *= f.mu;
-      }
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if (__ballot(mx > mrow + 8.f)) {
-        float mnew = fmaxf(mrow, mx);
-        float al = fexp2(mrow - mnew);
-        mrow = mnew;
-        lsum *= al;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[db][i] *= al;
-      }
-      bf16x8 pf[4];
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int g = 2 * st + (i >> 2);
-          p[i] = BIAS ? fexp2(x[8 * st + i] - (mrow - base - (float)g * step))
-                      : fexp2(fmaf(x[8 * st + i], f.mu, -mrow));
-        }
-        pf[st] = pack8(p);
-        lsum = dot8(pf[st], ones8(), lsum);
-      }
-#pragma unroll
-      for (int st = 0; st < 4; ++st)
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-          o[db] = mfma32(attn_tr_frag<D>(sm, vtr, db, V0 + st * 32 * D),
-                         pf[st], o[db]);
+    if constexpr (SHORT) {
+#pragma unroll 1
+      for (int nb = 0; nb < 2; ++nb)
+        if (cur.work >> nb & 1)
+          part(std::integral_constant<int, 1>(), cur, buf, nb);
+    } else if (cur.work) {
+      part(std::integral_constant<int, 2>(), cur, buf, 0);
     }
     cur = nxt;
     buf ^= 1;
@@ -243,22 +260,29 @@ __global__ __launch_bounds__(256, 2) void attn_mod_fwd_kernel(AttnArgs a) {
 void attn_mod_fwd(const AttnArgs& a, hipStream_t s) {
   dim3 g((unsigned)((long)a.B * a.H * cdiv_h(a.Tq, 128)));
   const bool c = a.cap != 0.f, w = a.slopes != nullptr;
-#define GO(D, C, W) attn_mod_fwd_kernel<D, C, W><<<g, 256, 0, s>>>(a)
-#define PICK(D)                       \
+#define GO(D, C, W, S) attn_mod_fwd_kernel<D, C, W, S><<<g, 256, 0, s>>>(a)
+#define PICK(D, S)                    \
   do {                                \
     if (c && w)                       \
-      GO(D, true, true);              \
+      GO(D, true, true, S);           \
     else if (c)                       \
-      GO(D, true, false);             \
+      GO(D, true, false, S);          \
     else if (w)                       \
-      GO(D, false, true);             \
+      GO(D, false, true, S);          \
     else                              \
-      GO(D, false, false);            \
+      GO(D, false, false, S);         \
   } while (0)
-  if (a.D <= 64)
-    PICK(64);
+  // 16384 tokens, 16 heads of 64, in us, whole tiles and halves: sequences
+  // of 256 36.3 and 33.0, of 1024 65 and 63, of 2048 119 and 120, of 8192
+  // 186 and 210; capped 41.2 and 38.2, 91 and 88, 154 and 150, 282 and 289;
+  // capped, sequences of 512 in four documents 57.8 and 53.2.  Heads of 128
+  // have no room for a third block either way.
+  if (a.D > 64)
+    PICK(128, false);
+  else if (a.Tk <= 2048)
+    PICK(64, true);
   else
-    PICK(128);
+    PICK(64, false);
 #undef PICK
 #undef GO
 }

@@ -140,6 +140,15 @@ TRAIN = [
     dict(B=1, Tq=4200, Tk=70, H=1, Hkv=1, D=64, cap=10.0),
     dict(B=1, Tq=70, Tk=4200, H=1, Hkv=1, D=128, docs=0, slopes=True,
          kv_len=[4161]),
+    # more than 2048 keys of heads of 64: whole tiles in the forward
+    dict(B=1, Tq=130, Tk=2200, H=2, Hkv=2, D=64, causal=True, cap=10.0,
+         off=[2050]),
+    dict(B=1, Tq=70, Tk=2100, H=2, Hkv=1, D=64, slopes=True,
+         kv_len=[2077]),
+    dict(B=1, Tq=2100, Tk=2100, H=1, Hkv=1, D=64, causal=True, docs=5,
+         pad=30),
+    dict(B=1, Tq=40, Tk=2050, H=2, Hkv=2, D=48, causal=True, cap=7.0,
+         slopes=True, off=[2000], prefix=[99]),
 ]
 
 
