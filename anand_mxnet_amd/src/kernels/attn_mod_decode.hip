@@ -1,10 +1,12 @@
 // Attention with shaped scores for a few queries over a long cache (see
 // attn_mod.h): the form that answers token by token.
 //
-// Bound by reading K and V once.  The queries of all heads that share a key
-// head form the 32 columns of one product (row r = token r / G, head r % G),
-// so a shared cache is read once for its whole group.  The keys of a
-// sequence are divided among `nsplit` blocks and, tile by tile of 32, among
+// Bound by reading K and V once: 64 sequences of up to 8192 keys, 16 heads of
+// 128 over 4, 102 us for 522 MB, 5.1 TB/s; 4 of up to 131071, three queries
+// each, 336 us for 1.95 GB, 5.8 TB/s (a copy moves 4.9, a sum reads 3.7).
+// The queries of all heads that share a key head form the 32 columns of one
+// product (row r = token r / G, head r % G), so a shared cache is read once
+// for its whole group.  The keys of a sequence are divided among `nsplit` blocks and, tile by tile of 32, among
 // the four waves of a block; a wave streams its tiles through LDS of its own
 // with counted waits and no barriers: the next K is on its way while this
 // tile's V is used, and the other way round.  Partial softmaxes are joined in

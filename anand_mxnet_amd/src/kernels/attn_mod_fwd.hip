@@ -16,6 +16,17 @@
 // The running maximum moves only when some row's scores pass it by more
 // than 8 (a factor of 256, harmless in fp32 sums and bf16 probabilities), so
 // the rescaling of the accumulators is skipped for almost every tile.
+//
+// Bound by the vector unit, with the matrix unit behind it: per score two
+// exp2 and a reciprocal under a cap.  16384 tokens in three documents, 16
+// heads of 128 over 8, capped: 605 us, 700 TFLOP/s; vector unit 54, matrix
+// unit 32 per cent busy at 2.05 GHz.  One document, uncapped: 976 TFLOP/s,
+// where a library product of 8192^3 reaches 1166.  Two groups of four waves
+// that took turns at products and softmax, 256 queries a block, were no
+// faster (640 us; prefixes of 4095 tokens 240, not 215).  Sequences of 512 in
+// four documents, 16384 tokens, heads of 64: 53 us, where moving the bytes
+// takes 34; a block has four tiles, and its first loads and its stores weigh
+// as much.
 #include <type_traits>
 
 #include "attn_mod.h"
