@@ -14,9 +14,9 @@
 //   3. emb_join    rows that cross chunks, their parts added in order
 // so a row that half of all tokens hit is spread over the chip like any
 // other, nothing is added by atomics and every run gives the same bits.
-// 16384 tokens, 32768 rows of 1024 in bf16: lookup 10 us (64 MB), order 18,
+// 16384 tokens, 32768 rows of 1024 in bf16: lookup 10 us (64 MB), order 14,
 // sums 20 (97 MB, 5 TB/s), rows that cross chunks 5; a table of two rows of
-// 768: 9, 17, 15 and 7.  The order is bound by the two passes that every block
+// 768: 9, 14, 15 and 7.  The order is bound by the two passes that every block
 // makes over all indices, from L2.
 #include <hip/hip_fp16.h>
 
@@ -96,15 +96,15 @@ __global__ __launch_bounds__(256) void emb_lookup_kernel(
 // tokens takes longer than all blocks' reading of the same indices from L2).
 // ---------------------------------------------------------------------------
 constexpr int EMB_WAVES = 16;
-constexpr int EMB_BATCH = 8;     // groups of 64 tokens that are read at once
 constexpr int EMB_ROWS = 512;    // rows of a block at most
 
-template <typename I>
+// BATCH: groups of 64 tokens that a wave reads at once.
+template <typename I, int BATCH>
 __global__ __launch_bounds__(1024) void emb_sort_kernel(
     const I* __restrict__ idx, int ntok, int vocab, int R, int rlog2,
     int* __restrict__ start, int2* __restrict__ sorted) {
   __shared__ int cnt[EMB_ROWS * EMB_WAVES];  // [row][wave]
-  __shared__ unsigned list[EMB_WAVES][64 * EMB_BATCH];
+  __shared__ unsigned list[EMB_WAVES][64 * BATCH];
   __shared__ int below[EMB_WAVES], tot[EMB_WAVES];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -114,16 +114,16 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
   for (int i = threadIdx.x; i < R * EMB_WAVES; i += 1024) cnt[i] = 0;
   __syncthreads();
 
-  constexpr int STEP = 64 * EMB_BATCH;
+  constexpr int STEP = 64 * BATCH;
   const int seg = (ntok + EMB_WAVES * 64 - 1) / (EMB_WAVES * 64) * 64;
   const int t0 = min(ntok, wave * seg), t1 = min(ntok, t0 + seg);
 
   // Tokens tb..tb + STEP - 1: a list of (row, place) of the block's own, in
   // order; returns how many.  low counts the tokens of lower rows.
   auto filter = [&](int tb, int& low) -> int {
-    unsigned r[EMB_BATCH];
+    unsigned r[BATCH];
 #pragma unroll
-    for (int u = 0; u < EMB_BATCH; ++u) {
+    for (int u = 0; u < BATCH; ++u) {
       const int t = tb + u * 64 + lane;
       r[u] = 0xffffffffu;  // outside the table: behind all rows
       if (t < t1) {
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
     }
     int n = 0;
 #pragma unroll
-    for (int u = 0; u < EMB_BATCH; ++u) {
+    for (int u = 0; u < BATCH; ++u) {
       low += __popcll(__ballot(r[u] < (unsigned)r0));
       const bool mine = r[u] - (unsigned)r0 < (unsigned)nr;
       const u64 m = __ballot(mine);
@@ -441,12 +441,23 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
   while ((1 << lg) < EMB_ROWS && (long)256 << lg < vocab) ++lg;
   const int R = 1 << lg;
   const unsigned nb = (unsigned)(((long)vocab + R - 1) / R);
-  if (idx64)
-    emb_sort_kernel<long><<<nb, 1024, 0, s>>>((const long*)idx, ntok,
-                                                vocab, R, lg, start, sorted);
+  // 16 groups at once keep the lists of 16384 tokens from the first pass to
+  // the second: 14.2 us, not 17.8 (32768 rows; 65536 tokens 48 and 51).  They
+  // gain nothing for few tokens (4096: 7.3 and 6.6) and leave room for one
+  // block on a compute unit (250000 rows: 25 and 23).
+  const bool wide = ntok > 8192 && nb <= 256;
+#define GO(I, N)                                                       \
+  emb_sort_kernel<I, N><<<nb, 1024, 0, s>>>((const I*)idx, ntok, vocab, \
+                                            R, lg, start, sorted)
+  if (idx64 && wide)
+    GO(long, 16);
+  else if (idx64)
+    GO(long, 8);
+  else if (wide)
+    GO(int, 16);
   else
-    emb_sort_kernel<int><<<nb, 1024, 0, s>>>((const int*)idx, ntok, vocab,
-                                               R, lg, start, sorted);
+    GO(int, 8);
+#undef GO
   const int nchunk = emb_chunks(ntok);
 #define GO(T, V)                                                            \
   do {                                                                      \

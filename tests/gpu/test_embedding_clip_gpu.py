@@ -68,6 +68,12 @@ CASES = [
     (50, 24, 1025, "float32", "int32", 1.0, "outside"),
     (3, 2056, 70, "bfloat16", "int64", 1.0, "uniform"),
     (40, 16, 64, "bfloat16", "int64", 1.0, "sorted"),
+    # one list of a wave's tokens and several, few rows and many
+    (900, 16, 8192, "bfloat16", "int32", 1.0, "zipf"),
+    (900, 16, 16384, "bfloat16", "int32", 1.0, "outside"),
+    (31, 8, 16385, "float32", "int64", 2.0, "uniform"),
+    (40000, 8, 40001, "bfloat16", "int32", 1.0, "zipf"),
+    (140000, 8, 20000, "bfloat16", "int64", 1.0, "uniform"),
 ]
 
 
