@@ -185,6 +185,44 @@ def test_both_forms(i):
                                     *opt[1:], 0, False)[0], want)
 
 
+def _drawn(seed):
+    r = np.random.default_rng(seed)
+    B, Hkv = int(r.integers(1, 4)), int(r.integers(1, 4))
+    big = int(r.choice([40, 140, 300, 600]))
+    Tk = int(r.integers(1, big))
+    docs = int(r.choice([0, 0, 1, 2, 6]))
+    kw = dict(B=B, Tq=Tk if docs else int(r.integers(1, big)), Tk=Tk,
+              H=Hkv * int(r.integers(1, 4)), Hkv=Hkv,
+              D=8 * int(r.integers(1, 17)), causal=bool(r.random() < 0.7),
+              cap=float(r.choice([1.0, 5.0, 30.0, 100.0])),
+              std=float(r.choice([0.3, 1.0, 2.5])))
+    if docs:
+        kw.update(docs=docs, pad=int(r.integers(0, Tk)))
+    if r.random() < 0.5:
+        kw["slopes"] = True
+        if r.random() < 0.5:
+            del kw["cap"]
+    if r.random() < 0.3:
+        kw["prefix"] = r.integers(-3, Tk + 10, B)
+    if r.random() < 0.4:
+        kw["kv_len"] = r.integers(0, Tk + 5, B)
+    if r.random() < 0.4:
+        kw["off"] = r.integers(-20, Tk + 20, B)
+    if r.random() < 0.2:
+        kw["scale"] = float(r.choice([-0.1, 0.3, 0.0]))
+    return kw
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_drawn(seed):
+    c = _case(1000 + seed, **_drawn(seed))
+    ref = _ref(c)
+    got = _train(c)
+    for name in ref:
+        check(name, got[name], ref[name])
+    check("infer", _infer(c), ref["out"])
+
+
 DECODE = [
     dict(B=1, Tq=1, Tk=1, H=1, Hkv=1, D=64, cap=20.0),
     dict(B=3, Tq=1, Tk=500, H=4, Hkv=4, D=64, kv_len=[500, 0, 33],

@@ -3,14 +3,18 @@ kernel that holds P in bfloat16 and sums in 32 bits may be off.
 
 A rounding to bfloat16 is off by at most h = 2**-8 of the value.  With
 absolute sums S(x) of the terms of a product:
-  out    P is rounded once, the result once:   h P|V| + h |out|
-  dV     P is rounded, the result:             h P^T|dO| + h |dV|
-  delta  sum of dO * out:                      e_d = sum_d |dO| err(out)
+  out    P is rounded, the result once:        e_o + h |out|
+         e_o = h P|V| + h |out|
+  dV     P is rounded, the result:             2 h P^T|dO| + h |dV|
+  delta  sum of dO * out and its remainder:    e_d = sum_d |dO| e_o
   dS     P (dP - delta) u:                     e_s = u P e_d + h |dS|
   dQ     scale (e_s |K|) + h |dQ|              dK: scale (e_s^T |Q|) + h |dK|
-The kernels divide by the sum of the rounded P, whose mean rounding m <= h
-they keep in the log-sum as well: dS is off by m |dS|, which is the term
-h |dS| (dS itself goes on as two bfloat16, 2**-16 of it).
+The kernels divide by the sum of the rounded terms p_j (1 + e_j), |e_j| <= h.
+That sum is (1 + m) sum p_j with the weighted mean m = sum p_j e_j / sum p_j,
+so |m| <= h too, and a weight of the values is P_j (1 + e_j) / (1 + m): off by
+h of each term and m of the whole, which is e_o.  The log-sum holds the same
+1 + m, so the backward's P is P_j / (1 + m): m more on top of its own rounding
+in dV, and m |dS| in dS, which goes on as two bfloat16 (2**-16 of it).
 The 32-bit sums add n * 2**-24 of the absolute sum, the hardware's exp2 and
 reciprocal and the tanh 2e-5 of a probability at these sizes: both are covered
 by 10 per cent on every bound (0.1 * 2**-8 = 4e-4) and 1e-6 for sums that
@@ -90,7 +94,8 @@ def reference(q, k, v, dout, H, Hkv, ok, pos, scale=None, cap=None,
         return x.reshape(B, Hkv, G, Tk, D).sum(2)
 
     out = p @ vh
-    out_b = 1.1 * (H8 * (p @ vh.abs()) + H8 * out.abs()) + 1e-6
+    e_o = H8 * (p @ vh.abs()) + H8 * out.abs()
+    out_b = 1.1 * (e_o + H8 * out.abs()) + 1e-6
     res = {"out": (merge(out), merge(out_b))}
     if dout is None:
         return res
@@ -100,7 +105,7 @@ def reference(q, k, v, dout, H, Hkv, ok, pos, scale=None, cap=None,
     dp = gh @ vh.transpose(-1, -2)
     delta = (gh * out).sum(-1, keepdim=True)
     ds = p * (dp - delta) * u
-    e_s = u * p * (gh.abs() * out_b).sum(-1, keepdim=True) + H8 * ds.abs()
+    e_s = u * p * (gh.abs() * e_o).sum(-1, keepdim=True) + H8 * ds.abs()
     dq = scale * ds @ kh
     dk = group(scale * ds.transpose(-1, -2) @ qh)
     dv = group(p.transpose(-1, -2) @ gh)
@@ -108,7 +113,7 @@ def reference(q, k, v, dout, H, Hkv, ok, pos, scale=None, cap=None,
     dq_b = 1.1 * (sc * e_s @ kh.abs() + H8 * dq.abs()) + 1e-6
     dk_b = 1.1 * (group(sc * e_s.transpose(-1, -2) @ qh.abs())
                   + H8 * dk.abs()) + 1e-6
-    dv_b = 1.1 * (group(H8 * p.transpose(-1, -2) @ gh.abs())
+    dv_b = 1.1 * (group(2 * H8 * p.transpose(-1, -2) @ gh.abs())
                   + H8 * dv.abs()) + 1e-6
     res.update(dq=(merge(dq), merge(dq_b)), dk=(merge(dk), merge(dk_b)),
                dv=(merge(dv), merge(dv_b)))
