@@ -42,7 +42,7 @@ struct AttnArgs {
   bf16* olo;   // what rounding took from o, [B, Tq, H, D]; may be null
   float* lse;  // [B, H, TqP] log2 of the softmax sum; +inf: row sees nothing
   const bf16* dout;
-  float* delta;  // [B, H, TqP] sum_d dout * out
+  float* delta;  // [B, H, TqP] minus sum_d dout * out
   bf16 *dq, *dk, *dv;
   float* ws;     // partial results of a split launch
   long qsb, ksb, vsb, osb, gsb;  // batch strides, elements

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
       delta = dot8(gf[kk], attn_load_row(lp, kk * 2 + half, a.D, ok), delta);
     }
     delta += __shfl_xor(delta, 32, 64);
-    if (half == 0 && qi < a.TqP) a.delta[row] = delta;
+    if (half == 0 && qi < a.TqP) a.delta[row] = -delta;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       attn_settle(qf[kk]);
@@ -368,7 +368,14 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
         const unsigned qrow = la.row + at, qtr = la.tr + at;
         const unsigned krow = attn_here(la.row + wk * 64 * D);
         const unsigned st = ST0 + buf * 256 + nb * 128 + 16 * half;
-        f32x16 s = zero16(), dp = zero16();
+        f32x16 s = zero16(), dp;
+        // dp starts at -delta of its rows
+#pragma unroll
+        for (int ii = 0; ii < 4; ++ii) {
+          const f32x4 e4 = attn_lds<f32x4>(sm, st + 32 * ii + 512);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dp[4 * ii + i] = e4[i];
+        }
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           bf16x8 kx, vx;
@@ -394,7 +401,6 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
             const int pr = p0 + 16 * w + 8 * ii;  // of four rows, pr..pr+3
             const unsigned sr = st + 64 * w + 32 * ii;
             const f32x4 l4 = attn_lds<f32x4>(sm, sr);
-            const f32x4 e4 = attn_lds<f32x4>(sm, sr + 512);
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -418,7 +424,7 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
                               fabsf(d0 + (float)(16 * w + 8 * ii + i)), -l4[i])
                        : -l4[i];
               const float pi = fexp2(fmaf(x[i], f.mu, off));
-              float di = pi * (dp[8 * w + 4 * ii + i] - e4[i]);
+              float di = pi * dp[8 * w + 4 * ii + i];
               if (CAP) di *= attn_dtanh(x[i]);
               p[4 * ii + i] = pi;
               ds[4 * ii + i] = di;
