@@ -137,7 +137,7 @@ void attn_wg_bf16(const bf16*, const bf16*, bf16*, int, int, int, int,
 void attn_seg_ranges(const int*, int2*, int, int, hipStream_t);
 void attn_mod_fwd(const AttnArgs&, hipStream_t);
 void attn_mod_bwd(const AttnArgs&, bool, hipStream_t);
-int attn_dkv_splits(int, int, int, int, int);
+int attn_dkv_splits(int, int, int, int, int, int);
 int attn_decode_splits(int, int, int, int);
 long attn_decode_ws(int, int, int, int, int);
 void attn_decode(const AttnArgs&, hipStream_t);
@@ -1289,7 +1289,7 @@ std::vector<at::Tensor> attn_mod_bwd(
   at::Tensor ws;
   a.nsplit = 1;
   if (need_kv) {
-    a.nsplit = mxa::attn_dkv_splits(a.B, a.Hkv, a.G, a.Tq, a.Tk);
+    a.nsplit = mxa::attn_dkv_splits(a.B, a.Hkv, a.G, a.Tq, a.Tk, a.D);
     if (a.nsplit > 1) {
       ws = at::empty({(long)a.nsplit * 2 * a.B * a.Tk * k.size(2)},
                      q.options().dtype(at::kFloat));

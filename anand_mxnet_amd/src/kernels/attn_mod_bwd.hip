@@ -19,7 +19,7 @@
 // capped: dQ 930 us, 910 TFLOP/s, matrix unit 44 and vector unit 57 per cent
 // busy; dK and dV 1300 us, 815 TFLOP/s, 38 and 45 per cent (a library
 // product of 8192^3: 1166 TFLOP/s).  dS as one bf16 number took 743 and 1140.
-// Sequences of 512 in four documents, 16384 tokens, heads of 64: 77 and 103
+// Sequences of 512 in four documents, 16384 tokens, heads of 64: 77 and 93
 // us, where moving the bytes takes 47 and 41.
 #include "attn_mod.h"
 
@@ -183,7 +183,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 // dK, dV: block = 128 keys of one key head, 32 of them along the lanes of a
 // wave; the queries of every head that shares them pass by in tiles of 64.
 //
-// D = 64: four waves that hold their K and V as operands in registers.
+// D = 64: four waves that hold V as operands in registers and K in LDS: with
+// K in registers as well, 193 of them, there is room for two blocks on a
+// compute unit, not three (sequences of 512 in four documents 103 and 93 us).
 // D = 128: those 64 registers beside 128 of accumulators would leave room
 // for one wave on a SIMD only, and nothing to overlap its phases with.  K
 // and V lie in LDS instead, and eight waves share the keys: one half takes
@@ -195,15 +197,16 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 // chip evenly.
 // ---------------------------------------------------------------------------
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
-    AttnArgs a) {
+__global__
+__launch_bounds__(D == 64 ? 256 : 512, D == 64 ? 3 : 2) void
+attn_mod_dkv_kernel(AttnArgs a) {
   constexpr bool WIDE = D == 128;
   constexpr int KK = D / 16, DB = D / 32, NW = WIDE ? 8 : 4;
-  // query and output-gradient tiles, two buffers of each; K and V where
-  // they lie here; log-sums, deltas and ids of the tiles
+  // query and output-gradient tiles, two buffers of each; K, and V where it
+  // lies here; log-sums, deltas and ids of the tiles
   constexpr int TILE = 128 * D, G0 = 2 * TILE, K0 = 4 * TILE;
   constexpr int V0 = K0 + 256 * D;
-  constexpr int ST0 = WIDE ? V0 + 256 * D : K0;
+  constexpr int ST0 = WIDE ? V0 + 256 * D : V0;
   __shared__ __align__(1024) char smem[ST0 + 6 * 256];
   lds_char* const sm = (lds_char*)smem;
   const unsigned lds0 = (unsigned)(size_t)sm;
@@ -325,32 +328,25 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
   ScoreFn f;
   QTile cur = next();
   if (cur.g >= 0) stage(0, cur);
-  bf16x8 kf[WIDE ? 1 : KK], vf[WIDE ? 1 : KK];
+  bf16x8 vf[WIDE ? 1 : KK];
   {
     const bf16* kp = a.k + b * a.ksb + (long)kj * a.kst + (long)hk * a.D;
     const bf16* vp = a.v + b * a.vsb + (long)kj * a.vst + (long)hk * a.D;
-    if constexpr (WIDE) {
-      // a wave writes the chunks that it would hold, K or V
-      const bool isv = wave >= 4;
-      bf16* img = (bf16*)(smem + (isv ? V0 : K0));
+    // WIDE: a wave writes K or V of its keys, else K
+    const bool isv = WIDE && wave >= 4;
+    const int row = wk * 32 + col;
+    bf16* img = (bf16*)(smem + (isv ? V0 : K0)) + row * D;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int ch = kk * 2 + half, row = wk * 32 + col;
-        bf16x8 x = isv ? attn_load_row(vp, ch, a.D, kok)
-                       : attn_load_q(kp, ch, a.D, kok, a.scale);
-        *(bf16x8*)&img[row * D + ((ch ^ attn_key<D>(row)) << 3)] = x;
-      }
-    } else {
+    for (int kk = 0; kk < KK; ++kk) {
+      const int ch = kk * 2 + half;
+      bf16x8 x = isv ? attn_load_row(vp, ch, a.D, kok)
+                     : attn_load_q(kp, ch, a.D, kok, a.scale);
+      *(bf16x8*)&img[(ch ^ attn_key<D>(row)) << 3] = x;
+      if constexpr (!WIDE) vf[kk] = attn_load_row(vp, ch, a.D, kok);
+    }
+    if constexpr (!WIDE) {
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        kf[kk] = attn_load_q(kp, kk * 2 + half, a.D, kok, a.scale);
-        vf[kk] = attn_load_row(vp, kk * 2 + half, a.D, kok);
-      }
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        attn_settle(kf[kk]);
-        attn_settle(vf[kk]);
-      }
+      for (int kk = 0; kk < KK; ++kk) attn_settle(vf[kk]);
     }
   }
   int buf = 0;
@@ -378,14 +374,12 @@ __global__ __launch_bounds__(D == 64 ? 256 : 512, 2) void attn_mod_dkv_kernel(
         }
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-          bf16x8 kx, vx;
-          if constexpr (WIDE) {
-            kx = attn_row_frag(sm, krow, kk, K0);
+          const bf16x8 kx = attn_row_frag(sm, krow, kk, K0);
+          bf16x8 vx;
+          if constexpr (WIDE)
             vx = attn_row_frag(sm, krow, kk, V0);
-          } else {
-            kx = kf[kk];
+          else
             vx = vf[kk];
-          }
           s = mfma32(attn_row_frag(sm, qrow, kk, 0), kx, s);
           dp = mfma32(attn_row_frag(sm, qrow, kk, G0), vx, dp);
         }
@@ -531,11 +525,15 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(
 }
 
 // Blocks of 128 keys are the unit of work and differ a lot under a causal
-// mask.  Fewer than 512 of them leave compute units idle at the end: their
-// queries are divided, as long as a part keeps some 16 tiles.
-int attn_dkv_splits(int B, int Hkv, int G, int Tq, int Tk) {
+// mask.  Few of them leave compute units idle at the end: their queries are
+// divided, as long as a part keeps some 16 tiles.  Heads of 64, three blocks
+// on a compute unit, 8192 tokens of 16 heads over 8 without a cap: 579 us
+// with 512 blocks, 395 with 1024, 425 with 1536, the join counted; 2 x 4096
+// of 16 over 4: 322, 231, 245.  Heads of 128, one block on a compute unit,
+// 2 x 4095: 475, 476 and 507.
+int attn_dkv_splits(int B, int Hkv, int G, int Tq, int Tk, int D) {
   const long base = (long)B * Hkv * cdiv_h(Tk, 128);
-  const long want = (511 + base) / base;
+  const long want = ((D <= 64 ? 1023 : 511) + base) / base;
   const long most = (long)cdiv_h(Tq, 64) * G / 16;
   const long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
