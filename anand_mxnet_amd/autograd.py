@@ -92,7 +92,12 @@ def _register_attached(arr):
 
 def backward(heads, head_grads=None, retain_graph: bool = False,
              train_mode: bool = True):
-    """Compute gradients of heads w.r.t. all attached variables."""
+    """Compute gradients of heads w.r.t. all attached variables.
+
+    Before a backward is captured into a graph, let go of the outputs and
+    losses of eager steps on the same variables: while they live, a gradient
+    is accumulated on the stream of that step, which a capture must not wait
+    for."""
     from .ndarray.ndarray import NDArray
 
     if isinstance(heads, NDArray):
