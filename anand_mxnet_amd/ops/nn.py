@@ -452,9 +452,10 @@ class _ScaledLookup(torch.autograd.Function):
 
 # ---------------- attention (contrib/transformer parity) ----------------
 
-def _attn_ints(x, shape, what, q):
-    """An optional integer tensor of the given shape, as int32 on q's
-    device."""
+def _attn_ints(x, shape, what, q, lo=None, hi=None):
+    """An optional integer tensor of the given shape, as int32 on q's device.
+    Where wider integers come, values outside [lo, hi] are taken as the
+    border."""
     if x is None:
         return None
     if not isinstance(x, torch.Tensor) or x.dtype.is_floating_point \
@@ -469,6 +470,8 @@ def _attn_ints(x, shape, what, q):
                          f"the queries are on {q.device}")
     if x.dtype is torch.int32 and x.is_contiguous():
         return x
+    if x.dtype is torch.int64 and lo is not None:
+        x = x.clamp(lo, hi)
     return x.to(torch.int32).contiguous()
 
 
@@ -521,14 +524,15 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
         seg_q = _attn_ints(seg_q, (B, Tq), "segment_ids", q)
         seg_k = seg_q if same else _attn_ints(seg_k, (B, Tk),
                                               "kv_segment_ids", q)
-    prefix = _attn_ints(prefix, (B,), "prefix_length", q)
-    kv_len = _attn_ints(kv_len, (B,), "kv_length", q)
+    prefix = _attn_ints(prefix, (B,), "prefix_length", q, 0, Tk)
+    kv_len = _attn_ints(kv_len, (B,), "kv_length", q, 0, Tk)
     off0 = 0
     if q_off is not None and not isinstance(q_off, torch.Tensor):
         off0, q_off = int(q_off), None
         if abs(off0) >= 1 << 30:
             bad("query_offset is out of range")
-    q_off = _attn_ints(q_off, (B,), "query_offset", q)
+    far = (1 << 30) - 1  # behind every key, or before it
+    q_off = _attn_ints(q_off, (B,), "query_offset", q, -far, far)
     args = (H, Hkv, float(scale if scale is not None else D ** -0.5), cap,
             bool(causal), slopes, seg_q, seg_k, prefix, kv_len, q_off, off0)
     if _use_hip(q, "shaped_mha", _BF16):
@@ -620,6 +624,9 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
     query_offset    integer or (B,) integers, 0 if not given: the position
                     of the first query among the keys, kv_length - Tq for
                     new tokens at the end of a cache
+
+    Lengths and offsets in arrays may be of any size: those past the keys on
+    either side count as the border (32-bit integers take no extra launch).
 
     A query that sees no key gives a row of zeros and no gradient.  Few
     queries outside autograd.record() take the form that splits the keys

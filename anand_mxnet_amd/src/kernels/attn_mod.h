@@ -267,7 +267,11 @@ DEVINL SeqMask attn_seq_mask(const AttnArgs& a, int b) {
   SeqMask m;
   m.kv_len = a.kv_len ? min(max(a.kv_len[b], 0), a.Tk) : a.Tk;
   m.prefix = a.prefix ? a.prefix[b] : 0;
-  m.off = a.off0 + (a.q_off ? a.q_off[b] : 0);
+  // positions and the ones behind them stay within 32 bits; Tq and Tk are
+  // below 2**30, so an offset cut to that sees the same keys
+  const long far = (1l << 30) - 1;
+  const long off = (long)a.off0 + (a.q_off ? a.q_off[b] : 0);
+  m.off = (int)min(max(off, -far), far);
   m.causal = a.causal;
   m.has_seg = a.seg_q != nullptr;
   return m;

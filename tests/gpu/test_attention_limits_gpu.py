@@ -1,0 +1,46 @@
+"""Attention with shaped scores at the borders of its arguments (GPU)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FAR = [2 ** 31 - 1, 2 ** 31 - 200, 2 ** 30 - 1, 2 ** 30]
+
+
+def _args(Tq, Tk):
+    g = torch.Generator().manual_seed(5)
+    return [torch.randn((2, T, 2 * 64), generator=g).bfloat16().cuda()
+            for T in (Tq, Tk, Tk)]
+
+
+def _run(ts, train, **kw):
+    import anand_mxnet_amd as mx
+    a = [mx.nd.from_torch(t.clone()) for t in ts]
+    kw = {k: mx.nd.from_torch(v.cuda()) if isinstance(v, torch.Tensor) else v
+          for k, v in kw.items()}
+    if not train:
+        return [mx.nd.multi_head_attention(*a, 2, num_kv_heads=2, **kw)._t]
+    for x in a:
+        x.attach_grad()
+    with mx.autograd.record():
+        out = mx.nd.multi_head_attention(*a, 2, num_kv_heads=2, **kw)
+    out.backward(mx.nd.from_torch(torch.ones_like(ts[0])))
+    return [out._t.detach()] + [x.grad._t for x in a]
+
+
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("Tq,train", [(1, False), (130, False), (130, True)])
+def test_offsets_near_the_end_of_32_bits(far, Tq, train):
+    """A query behind every key sees them all, one before every key none,
+    whatever the offset: no position overflows."""
+    ts = _args(Tq, 150)
+    ids = torch.zeros(2, Tq, dtype=torch.int32), \
+        torch.zeros(2, 150, dtype=torch.int32)
+    for seg in (False, True):  # with ids, single queries take blocks too
+        kw = dict(segment_ids=ids[0], kv_segment_ids=ids[1]) if seg else {}
+        want = _run(ts, train, kv_length=torch.tensor([150, 150]), **kw)
+        for sign in (1, -1):
+            off = torch.tensor([sign * far] * 2, dtype=torch.int32)
+            got = _run(ts, train, causal=True, query_offset=off, **kw)
+            for x, y in zip(got, want):
+                assert torch.equal(x, y if sign > 0 else torch.zeros_like(y))

@@ -163,3 +163,26 @@ def test_refuses_more():
             f(q, q, q, 2, logit_cap=1.0, dropout_p=0.1)
     # outside training dropout does nothing
     f(q, q, q, 2, logit_cap=1.0, dropout_p=0.1)
+
+
+@pytest.mark.parametrize("far", [2 ** 31, 2 ** 32, 2 ** 40 + 1, 2 ** 63 - 1])
+def test_integers_past_32_bits(far):
+    """Lengths and positions behind every key see all of them, whatever
+    their size; those before the first see none."""
+    q, k = torch.randn(2, 3, 16), torch.randn(2, 7, 16)
+    v = torch.randn(2, 7, 16)
+    a = [nd.from_torch(t) for t in (q, k, v)]
+    f = nd.multi_head_attention
+
+    def ints(*x):
+        return nd.from_torch(torch.tensor(x, dtype=torch.int64))
+
+    want = f(*a, 2, kv_length=ints(7, 0))._t
+    assert want[0].any() and not want[1].any()
+    got = f(*a, 2, kv_length=ints(far, -far))._t
+    assert torch.equal(got, want)
+    got = f(*a, 2, causal=True, query_offset=ints(far, -far))._t
+    assert torch.equal(got, want)
+    want = f(*a, 2, causal=True, prefix_length=ints(7, 0))._t
+    got = f(*a, 2, causal=True, prefix_length=ints(far, -far))._t
+    assert torch.equal(got, want)
