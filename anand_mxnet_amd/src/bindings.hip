@@ -7,6 +7,7 @@
 
 #include <hip/hip_runtime.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/hip/HIPException.h>
 
 #include <algorithm>
 #include <unordered_map>
@@ -1104,6 +1105,13 @@ std::vector<at::Tensor> flash_bwd(const at::Tensor& q,
 using OptT = c10::optional<at::Tensor>;
 
 namespace {
+// A launch of blocks blocks: the runtime takes less than 2**32 threads a
+// dimension.
+void attn_grid(long blocks, int threads) {
+  TORCH_CHECK(blocks < (1L << 32) / threads,
+              "attention: too large, a launch of ", blocks, " blocks");
+}
+
 const int* attn_index(const OptT& t, const at::Tensor& like, long n,
                       const char* what) {
   if (!t.has_value()) return nullptr;
@@ -1151,9 +1159,8 @@ mxa::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k,
                   v.sizes() == k.sizes(),
               "attention: key and value must be [batch, keys, kv_heads * ",
               a.D, "]");
-  TORCH_CHECK(q.size(1) < (1L << 30) && k.size(1) < (1L << 30) &&
-                  a.B * H * ((a.Tq + 127) / 128 + 1) < (1L << 30) &&
-                  (long)a.B * Hkv * ((a.Tk + 127) / 128 + 1) < (1L << 30),
+  TORCH_CHECK(q.size(0) < (1L << 30) && q.size(1) < (1L << 30) &&
+                  k.size(1) < (1L << 30),
               "attention: too large");
   a.TqP = (a.Tq + 63) / 64 * 64;
   a.q = bfp(q);
@@ -1200,8 +1207,10 @@ at::Tensor attn_ranges(const int* seg, long B, long T,
                        const at::Tensor& like) {
   auto r = at::empty({B, (T + 127) / 128 * 4, 2},
                      like.options().dtype(at::kInt));
+  attn_grid((B * ((T + 127) / 128) * 4 + 7) / 8, 256);
   mxa::attn_seg_ranges(seg, (int2*)r.data_ptr<int>(), (int)B, (int)T,
                        cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return r;
 }
 }  // namespace
@@ -1219,6 +1228,9 @@ std::vector<at::Tensor> attn_mod_fwd(
   auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
                      seg_k, prefix, kv_len, q_off, off0);
   TORCH_CHECK(a.B > 0 && a.Tq > 0 && a.Tk > 0, "attention: empty");
+  attn_grid(a.B * H * ((a.Tq + 127) / 128), 256);
+  if (with_stats)  // the backward's over the keys, undivided at such sizes
+    attn_grid(a.B * Hkv * ((a.Tk + 127) / 128), a.D > 64 ? 512 : 256);
   auto out = at::empty({a.B, a.Tq, q.size(2)}, q.options());
   a.o = bfp_mut(out);
   a.osb = out.stride(0);
@@ -1246,6 +1258,7 @@ std::vector<at::Tensor> attn_mod_fwd(
     }
   }
   mxa::attn_mod_fwd(a, cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return res;
 }
 
@@ -1290,6 +1303,8 @@ std::vector<at::Tensor> attn_mod_bwd(
   a.nsplit = 1;
   if (need_kv) {
     a.nsplit = mxa::attn_dkv_splits(a.B, a.Hkv, a.G, a.Tq, a.Tk, a.D);
+    attn_grid(a.B * Hkv * ((a.Tk + 127) / 128) * a.nsplit,
+              a.D > 64 ? 512 : 256);
     if (a.nsplit > 1) {
       ws = at::empty({(long)a.nsplit * 2 * a.B * a.Tk * k.size(2)},
                      q.options().dtype(at::kFloat));
@@ -1303,6 +1318,7 @@ std::vector<at::Tensor> attn_mod_bwd(
     res.push_back(dv);
   }
   mxa::attn_mod_bwd(a, need_kv, cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return res;
 }
 
@@ -1371,21 +1387,22 @@ at::Tensor attn_decode(const at::Tensor& q_, const at::Tensor& k_,
   auto a = attn_args(q, k, v, H, Hkv, scale, cap, causal, slopes, {}, {},
                      prefix, kv_len, q_off, off0);
   TORCH_CHECK(a.B > 0 && a.Tq > 0 && a.Tk > 0, "attention: empty");
+  TORCH_CHECK((long)a.Tq * a.G < (1L << 30), "attention: too large");
+  const int R = a.Tq * a.G;
+  a.nsplit = mxa::attn_decode_splits(a.B, a.Hkv, R, a.Tk);
+  attn_grid(a.B * Hkv * ((R + 31) / 32) * a.nsplit, 256);
+  if (a.nsplit > 1) attn_grid((a.B * Hkv * R + 3) / 4, 256);  // the join
   auto out = at::empty({a.B, a.Tq, q.size(2)}, q.options());
   a.o = bfp_mut(out);
   a.osb = out.stride(0);
   a.ost = out.stride(1);
-  TORCH_CHECK((long)a.Tq * a.G < (1L << 30), "attention: too large");
-  const int R = a.Tq * a.G;
-  a.nsplit = mxa::attn_decode_splits(a.B, a.Hkv, R, a.Tk);
-  TORCH_CHECK((long)a.B * a.Hkv * ((R + 31) / 32) * a.nsplit < (1L << 31),
-              "attention: too large");
   at::Tensor ws;
   if (long n = mxa::attn_decode_ws(a.B, a.Hkv, R, a.D, a.nsplit)) {
     ws = at::empty({n}, q.options().dtype(at::kFloat));
     a.ws = ws.data_ptr<float>();
   }
   mxa::attn_decode(a, cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return out;
 }
 

@@ -44,3 +44,51 @@ def test_offsets_near_the_end_of_32_bits(far, Tq, train):
             got = _run(ts, train, causal=True, query_offset=off, **kw)
             for x, y in zip(got, want):
                 assert torch.equal(x, y if sign > 0 else torch.zeros_like(y))
+
+
+def _wide(B, H, Tq, Tk):
+    """B equal sequences of H heads of 8, one sequence's memory."""
+    g = torch.Generator().manual_seed(6)
+    return [torch.randn((1, T, H * 8), generator=g).bfloat16().cuda()
+            .expand(B, T, H * 8) for T in (Tq, Tk, Tk)]
+
+
+@pytest.mark.parametrize("B,Tq,Tk,ids", [
+    (1 << 21, 1, 1, False),            # 2**24 blocks of single queries
+    (1 << 21, 1, 1, True),             # the same in blocks of 128
+    (1 << 19, 1 << 10, 1, False),      # 2**25 blocks of 128 queries
+])
+def test_launches_past_2_to_the_32_threads_are_refused(B, Tq, Tk, ids):
+    import anand_mxnet_amd as mx
+    a = [mx.nd.from_torch(t) for t in _wide(B, 8, Tq, Tk)]
+    kw = dict(num_kv_heads=8, logit_cap=30.0)
+    if ids:
+        kw.update(segment_ids=mx.nd.from_torch(torch.zeros(
+            (B, Tq), dtype=torch.int32, device="cuda")))
+    with pytest.raises(RuntimeError, match="too large"):
+        mx.nd.multi_head_attention(*a, 8, **kw)
+
+
+def test_backward_past_2_to_the_32_threads_is_refused_forward():
+    """Heads above 64 columns: the keys' gradients take blocks of 512."""
+    import anand_mxnet_amd as mx
+    t = torch.zeros(1, 1, 8 * 72, dtype=torch.bfloat16, device="cuda")
+    a = [mx.nd.from_torch(t.expand(1 << 20, 1, 8 * 72)) for _ in range(3)]
+    a[1].attach_grad()
+    with mx.autograd.record():
+        with pytest.raises(RuntimeError, match="too large"):
+            mx.nd.multi_head_attention(*a, 8, num_kv_heads=8, logit_cap=30.0)
+
+
+@pytest.mark.parametrize("ids", [False, True])
+def test_largest_launch(ids):
+    import anand_mxnet_amd as mx
+    B = (1 << 21) - 1
+    ts = _wide(B, 8, 1, 1)
+    kw = dict(num_kv_heads=8, logit_cap=30.0)
+    if ids:
+        kw.update(segment_ids=mx.nd.from_torch(torch.zeros(
+            (B, 1), dtype=torch.int32, device="cuda")))
+    out = mx.nd.multi_head_attention(*[mx.nd.from_torch(t) for t in ts], 8,
+                                     **kw)._t
+    assert torch.equal(out, ts[2])  # one key: its value
