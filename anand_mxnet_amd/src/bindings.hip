@@ -1570,6 +1570,7 @@ at::Tensor embedding_fwd(const at::Tensor& idx, const at::Tensor& W,
                   ix.scalar_type() == at::kLong, ix.data_ptr(), W.data_ptr(),
                   out.data_ptr(), ntok, (int)D, W.size(0), (float)scale,
                   cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return out;
 }
 
@@ -1602,6 +1603,7 @@ at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
                 dW.data_ptr(), start.data_ptr<int>(),
                 (int2*)sorted.data_ptr<int>(), part.data_ptr<float>(),
                 (int)ntok, (int)D, (int)vocab, (float)scale, cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return dW;
 }
 
@@ -1699,6 +1701,7 @@ at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
   mxa::clip_norm(sp.data(), dp.data(), n.data(), dt.data(), (long)sp.size(),
                  max_norm, ws.data_ptr<double>(), norm.data_ptr<float>(),
                  cur_stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return norm;
 }
 

@@ -101,7 +101,7 @@ constexpr int EMB_ROWS = 512;    // rows of a block at most
 // BATCH: groups of 64 tokens that a wave reads at once.
 template <typename I, int BATCH>
 __global__ __launch_bounds__(1024) void emb_sort_kernel(
-    const I* __restrict__ idx, int ntok, int vocab, int R, int rlog2,
+    const I* __restrict__ idx, int ntok, int vocab, int R, int rlog2, int p0,
     int* __restrict__ start, int2* __restrict__ sorted) {
   __shared__ int cnt[EMB_ROWS * EMB_WAVES];  // [row][wave]
   __shared__ unsigned list[EMB_WAVES][64 * BATCH];
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const u64 lower = (1ull << lane) - 1;
-  const int r0 = blockIdx.x * R;
+  const int r0 = (p0 + (int)blockIdx.x) * R;
   const int nr = min(R, vocab - r0);
   for (int i = threadIdx.x; i < R * EMB_WAVES; i += 1024) cnt[i] = 0;
   __syncthreads();
@@ -233,8 +233,8 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// 2. Sums.  Waves [0, nchunk * ns) take a chunk and a slice of 64 V columns;
-// the rest of the grid clears rows that no token hits.
+// 2. Sums.  Waves [0, nchunk * ns) take a chunk (from chunk0 on) and a slice
+// of 64 V columns; the rest of the grid clears rows that no token hits.
 // part: [nchunk][2][D], the sums of a chunk's first row where it began in an
 // earlier chunk, and of its last row where it goes on in the next.
 // ---------------------------------------------------------------------------
@@ -242,7 +242,8 @@ template <typename T, int V>
 __global__ __launch_bounds__(256) void emb_reduce_kernel(
     const int2* __restrict__ sorted, const int* __restrict__ start,
     const T* __restrict__ dy, T* __restrict__ dW, float* __restrict__ part,
-    int vocab, int D, float scale, int nchunk, int ns, int sumblocks) {
+    int vocab, int D, float scale, int chunk0, int nchunk, int ns,
+    int sumblocks) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x >= sumblocks) {
@@ -258,9 +259,10 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
   }
   const int n = start[vocab];  // tokens inside the table
   const long w = (long)blockIdx.x * 4 + wave;
-  const int chunk = (int)(w / ns), slice = (int)(w % ns);
+  if (w >= (long)nchunk * ns) return;
+  const int chunk = chunk0 + (int)(w / ns), slice = (int)(w % ns);
   const int p0 = chunk * EMB_CHUNK, p1 = min(n, p0 + EMB_CHUNK);
-  if (chunk >= nchunk || p0 >= p1) return;
+  if (p0 >= p1) return;
   const int c = (slice * 64 + lane) * V;
   const bool on = c < D;
 
@@ -329,10 +331,10 @@ template <typename T, int PV>
 __global__ __launch_bounds__(256) void emb_join_kernel(
     const int2* __restrict__ sorted, const int* __restrict__ start,
     const float* __restrict__ part, T* __restrict__ dW, int vocab, int D,
-    float scale) {
+    float scale, int chunk0) {
   __shared__ float sums[8][32][PV];
   const int n = start[vocab];
-  const int chunk = blockIdx.x;
+  const int chunk = chunk0 + (int)blockIdx.x;
   const int end = (chunk + 1) * EMB_CHUNK;
   if (end >= n) return;  // nothing follows this chunk
   const int key = sorted[end - 1].x;
@@ -394,6 +396,10 @@ __global__ __launch_bounds__(256) void emb_join_kernel(
 // host
 // ---------------------------------------------------------------------------
 
+// Blocks of a launch at most: the runtime takes less than 2**32 threads a
+// dimension.
+constexpr unsigned EMB_LAUNCH = 1u << 21;
+
 // dtype: 0 bf16, 1 fp16, 2 fp32
 #define EMB_TYPES(dtype, F)                 \
   switch (dtype) {                          \
@@ -446,9 +452,10 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
   // gain nothing for few tokens (4096: 7.3 and 6.6) and leave room for one
   // block on a compute unit (250000 rows: 25 and 23).
   const bool wide = ntok > 8192 && nb <= 256;
-#define GO(I, N)                                                       \
-  emb_sort_kernel<I, N><<<nb, 1024, 0, s>>>((const I*)idx, ntok, vocab, \
-                                            R, lg, start, sorted)
+#define GO(I, N)                                                         \
+  for (unsigned p = 0; p < nb; p += EMB_LAUNCH)                          \
+  emb_sort_kernel<I, N><<<min(EMB_LAUNCH, nb - p), 1024, 0, s>>>(        \
+      (const I*)idx, ntok, vocab, R, lg, (int)p, start, sorted)
   if (idx64 && wide)
     GO(long, 16);
   else if (idx64)
@@ -459,19 +466,24 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
     GO(int, 8);
 #undef GO
   const int nchunk = emb_chunks(ntok);
-#define GO(T, V)                                                            \
-  do {                                                                      \
-    int ns = (D / (V) + 63) / 64;                                           \
-    unsigned sb = (unsigned)(((long)nchunk * ns + 3) / 4);                  \
-    unsigned zb = (unsigned)(vocab < 8192 ? (vocab + 3) / 4 : 2048);        \
-    emb_reduce_kernel<T, V><<<sb + zb, 256, 0, s>>>(                        \
-        sorted, start, (const T*)dy, (T*)dW, part, vocab, D, scale, nchunk, \
-        ns, (int)sb);                                                       \
-    constexpr int PV = (V) == 1 ? 1 : 4;                                    \
-    dim3 jg(nchunk - 1, EMB_JOIN);                                          \
-    if (nchunk > 1)                                                         \
-      emb_join_kernel<T, PV><<<jg, 256, 0, s>>>(sorted, start, part,        \
-                                                (T*)dW, vocab, D, scale);   \
+#define GO(T, V)                                                             \
+  do {                                                                       \
+    const int ns = (D / (V) + 63) / 64;                                      \
+    const int most = max(1, (int)(EMB_LAUNCH * 4l / ns));                    \
+    for (int c0 = 0; c0 < nchunk; c0 += most) {                              \
+      const int nc = min(most, nchunk - c0);                                 \
+      unsigned sb = (unsigned)(((long)nc * ns + 3) / 4);                     \
+      unsigned zb = (unsigned)(vocab < 8192 ? (vocab + 3) / 4 : 2048);       \
+      if (c0 > 0) zb = 0;                                                    \
+      emb_reduce_kernel<T, V><<<sb + zb, 256, 0, s>>>(                       \
+          sorted, start, (const T*)dy, (T*)dW, part, vocab, D, scale, c0,    \
+          nc, ns, (int)sb);                                                  \
+    }                                                                        \
+    constexpr int PV = (V) == 1 ? 1 : 4;                                     \
+    for (int c0 = 0; c0 < nchunk - 1; c0 += EMB_LAUNCH)                      \
+      emb_join_kernel<T, PV>                                                 \
+          <<<dim3(min((int)EMB_LAUNCH, nchunk - 1 - c0), EMB_JOIN), 256, 0,  \
+             s>>>(sorted, start, part, (T*)dW, vocab, D, scale, c0);         \
   } while (0)
 #define F(T, V) \
   if (vec)      \
