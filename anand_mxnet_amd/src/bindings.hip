@@ -1561,7 +1561,7 @@ at::Tensor embedding_fwd(const at::Tensor& idx, const at::Tensor& W,
   auto ix = idx.scalar_type() == at::kInt ? idx.contiguous()
                                           : idx.to(at::kLong).contiguous();
   const long ntok = ix.numel(), D = W.size(1);
-  TORCH_CHECK(D < (1L << 31), "embedding: rows are too long");
+  TORCH_CHECK(D < 0x7ffff000, "embedding: rows are too long");
   auto sizes = idx.sizes().vec();
   sizes.push_back(D);
   auto out = at::empty(sizes, W.options());
@@ -1587,8 +1587,9 @@ at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
   const long ntok = ix.numel(), D = dy.size(-1);
   TORCH_CHECK(dy.numel() == ntok * D,
               "embedding: one gradient row for each index");
-  // places are 32 bits wide, and a batch of tokens may reach past the last
-  TORCH_CHECK(vocab < 0x7fffffff && ntok < 0x7ffff000 && D < 0x7fffffff,
+  // places are 32 bits wide, and a batch of tokens or columns may reach past
+  // the last
+  TORCH_CHECK(vocab < 0x7fffffff && ntok < 0x7ffff000 && D < 0x7ffff000,
               "embedding: too large");
   if (ntok == 0) return at::zeros({vocab, D}, dy.options());
   auto dW = at::empty({vocab, D}, dy.options());

@@ -249,11 +249,11 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
   if ((int)blockIdx.x >= sumblocks) {
     const int nv = D / V;
     const float z[V] = {};
-    for (int r = (blockIdx.x - sumblocks) * 4 + wave; r < vocab;
+    for (long r = (blockIdx.x - sumblocks) * 4 + wave; r < vocab;
          r += (gridDim.x - sumblocks) * 4) {
       if (start[r] != start[r + 1]) continue;
       for (int c = lane; c < nv; c += 64)
-        emb_store<T, V>(dW + (long)r * D + c * V, z, 1.f);
+        emb_store<T, V>(dW + r * D + (long)c * V, z, 1.f);
     }
     return;
   }
