@@ -10,6 +10,7 @@ graph compiler to pass over — dispatch IS the graph)."""
 from __future__ import annotations
 
 import functools
+import inspect
 
 import torch
 
@@ -23,12 +24,22 @@ _initialized = False
 _target_dtype = torch.bfloat16
 
 
-def _cast_args(args, kwargs, dtype):
-    def c(x):
-        if isinstance(x, torch.Tensor) and x.is_floating_point():
+def _cast_args(args, kwargs, dtype, keep=()):
+    """The arguments in dtype, but for those that keep names or numbers."""
+    def c(x, key):
+        if isinstance(x, torch.Tensor) and x.is_floating_point() \
+                and key not in keep:
             return x.to(dtype)
         return x
-    return [c(a) for a in args], {k: c(v) for k, v in kwargs.items()}
+    return [c(a, i) for i, a in enumerate(args)], \
+        {k: c(v, k) for k, v in kwargs.items()}
+
+
+def _kept(name, raw):
+    """Names and positions of the arguments that keep their type."""
+    names = lists.LP16_KEEP_ARGS.get(name, ())
+    order = list(inspect.signature(raw).parameters) if names else []
+    return frozenset(names) | {order.index(n) for n in names}
 
 
 def init(target_dtype="bfloat16"):
@@ -44,8 +55,8 @@ def init(target_dtype="bfloat16"):
         raw = _reg.RAW[name]
 
         @functools.wraps(raw)
-        def lp(*args, __raw=raw, **kwargs):
-            a, k = _cast_args(args, kwargs, _target_dtype)
+        def lp(*args, __raw=raw, __keep=_kept(name, raw), **kwargs):
+            a, k = _cast_args(args, kwargs, _target_dtype, __keep)
             return __raw(*a, **k)
 
         _reg.RAW[name] = lp

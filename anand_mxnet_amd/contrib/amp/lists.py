@@ -9,6 +9,12 @@ LP16_FUNCS = [
     "gelu", "silu", "Pooling", "Embedding",
 ]
 
+# arguments of LP16_FUNCS that keep their type: constants that the op itself
+# holds in fp32 (a slope's rounding would grow with the distance)
+LP16_KEEP_ARGS = {
+    "multi_head_attention": ("distance_slopes",),
+}
+
 # ops forced to fp32 (reductions / losses / normalization statistics)
 FP32_FUNCS = [
     "softmax", "log_softmax", "SoftmaxOutput", "softmax_cross_entropy",
