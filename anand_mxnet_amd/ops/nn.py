@@ -425,29 +425,10 @@ def embedding_impl(data, weight, scale=1.0):
     out = F.embedding(data.long(), weight)
     if scale == 1.0:
         return out
-    if weight.dtype in (torch.bfloat16, torch.float16):
-        return _ScaledLookup.apply(data.long(), weight, float(scale))
-    return out * scale
-
-
-class _ScaledLookup(torch.autograd.Function):
-    """CPU oracle of the scaled lookup for 16-bit tables: the gradient is
-    summed and scaled in 32 bits and rounded once, as the kernels do."""
-
-    @staticmethod
-    def forward(ctx, idx, weight, scale):
-        ctx.save_for_backward(idx)
-        ctx.conf = (weight.shape, weight.dtype, scale)
-        return (F.embedding(idx, weight).float() * scale).to(weight.dtype)
-
-    @staticmethod
-    def backward(ctx, dy):
-        (idx,) = ctx.saved_tensors
-        shape, dtype, scale = ctx.conf
-        g = torch.zeros(shape, dtype=torch.float32)
-        g.index_add_(0, idx.flatten(),
-                     dy.float().reshape(-1, shape[1]))
-        return None, (g * scale).to(dtype), None
+    # a 16-bit table's gradient is summed in 32 bits and rounded once, as the
+    # kernels do
+    ct = torch.promote_types(weight.dtype, torch.float32)
+    return (F.embedding(data.long(), weight.to(ct)) * scale).to(weight.dtype)
 
 
 # ---------------- attention (contrib/transformer parity) ----------------

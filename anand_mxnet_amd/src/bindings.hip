@@ -1608,7 +1608,9 @@ at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
   return dW;
 }
 
-// The differentiable lookup, native for the host's time of a small batch.
+// The differentiable lookup, native for the host's time of a small batch, and
+// the gradient of its table.  Each is the other's backward, so derivatives of
+// any order come out.
 class EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx,
@@ -1622,15 +1624,42 @@ class EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
 
   static torch::autograd::variable_list backward(
       torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grad);
+};
+
+class EmbeddingGradFn : public torch::autograd::Function<EmbeddingGradFn> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx,
+                            const at::Tensor& idx, const at::Tensor& dy,
+                            long vocab, double scale) {
+    ctx->save_for_backward({idx});
+    ctx->saved_data["scale"] = scale;
+    return embedding_bwd(idx, dy.contiguous(), vocab, scale);
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
       torch::autograd::variable_list grad) {
     return {at::Tensor(),
-            embedding_bwd(ctx->get_saved_variables()[0],
-                          grad[0].contiguous(),
-                          ctx->saved_data["vocab"].toInt(),
-                          ctx->saved_data["scale"].toDouble()),
-            at::Tensor()};
+            EmbeddingFn::apply(ctx->get_saved_variables()[0], grad[0],
+                               ctx->saved_data["scale"].toDouble()),
+            at::Tensor(), at::Tensor()};
   }
 };
+
+torch::autograd::variable_list EmbeddingFn::backward(
+    torch::autograd::AutogradContext* ctx,
+    torch::autograd::variable_list grad) {
+  const auto idx = ctx->get_saved_variables()[0];
+  const long vocab = ctx->saved_data["vocab"].toInt();
+  const double scale = ctx->saved_data["scale"].toDouble();
+  // the tape of a second order costs time that others need not spend
+  return {at::Tensor(),
+          at::GradMode::is_enabled()
+              ? EmbeddingGradFn::apply(idx, grad[0], vocab, scale)
+              : embedding_bwd(idx, grad[0].contiguous(), vocab, scale),
+          at::Tensor()};
+}
 
 at::Tensor embedding(const at::Tensor& idx, const at::Tensor& W,
                      double scale) {

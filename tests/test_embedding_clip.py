@@ -78,3 +78,33 @@ def test_clip_refuses():
     with pytest.raises(MXNetError):
         f([w(x)], float("nan"))
     assert x.eq(1).all()
+
+
+def second_order(idx, w, scale):
+    """Gradient of the squared norm of the table's gradient."""
+    from anand_mxnet_amd.ops.registry import RAW
+    w = w.detach().requires_grad_()
+    out = RAW["Embedding"](idx, w, scale=scale)
+    g, = torch.autograd.grad((out ** 3).sum(), w, create_graph=True)
+    second, = torch.autograd.grad((g ** 2).sum(), w)
+    return g.detach(), second
+
+
+def check_second_order(dt, scale, dev):
+    """(x -> scale x[idx]) cubed: with c the count of a row's tokens the
+    gradient is 3 c s^3 w^2, and that of its squared norm 36 c^2 s^6 w^3."""
+    w = torch.randint(-2, 3, (5, 8)).to(dt)   # small whole numbers: exact
+    idx = torch.tensor([[3, 3, 0], [4, 3, 1]])
+    c = torch.tensor([1, 1, 0, 3, 1], dtype=torch.float64)[:, None]
+    g, second = second_order(idx.to(dev), w.to(dev), scale)
+    x = w.double()
+    assert torch.equal(g.double().cpu(), 3 * c * scale ** 3 * x ** 2)
+    assert torch.equal(second.double().cpu(),
+                       36 * c ** 2 * scale ** 6 * x ** 3)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float64, torch.bfloat16,
+                                torch.float16])
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+def test_embedding_twice(dt, scale):
+    check_second_order(dt, scale, "cpu")
