@@ -1322,21 +1322,36 @@ std::vector<at::Tensor> attn_mod_bwd(
   return res;
 }
 
+// A gradient whose own derivative is not there: whoever asks for it gets an
+// error, not a sum without this term.
+class AttnFirstOrder : public torch::autograd::Function<AttnFirstOrder> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext*,
+                            const at::Tensor& g, const at::Tensor& q,
+                            const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& dout) {
+    return g.detach();
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "attention: shaped scores have no second derivative "
+                       "on the GPU");
+  }
+};
+
 // Differentiable form of attn_mod_fwd: the backward recomputes the scores
 // from the saved log-sums.  A native function rather than one in Python: a
 // short batch's time is the host's.
 class ShapedMha : public torch::autograd::Function<ShapedMha> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx,
-                            const at::Tensor& q_, const at::Tensor& k_,
-                            const at::Tensor& v_, long H, long Hkv,
+                            const at::Tensor& q, const at::Tensor& k,
+                            const at::Tensor& v, long H, long Hkv,
                             double scale, double cap, bool causal,
                             const OptT& slopes, const OptT& seg_q,
                             const OptT& seg_k, const OptT& prefix,
                             const OptT& kv_len, const OptT& q_off,
                             long off0) {
-    c10::DeviceGuard guard(q_.device());
-    const auto q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_);
     auto r = attn_mod_fwd(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
                           seg_k, prefix, kv_len, q_off, off0, true);
     auto some = [](const OptT& t) { return t.value_or(at::Tensor()); };
@@ -1363,6 +1378,9 @@ class ShapedMha : public torch::autograd::Function<ShapedMha> {
         ctx->saved_data["cap"].toDouble(), c[2] != 0, opt(6), opt(7), opt(8),
         opt(9), opt(10), opt(11), c[3],
         ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+    if (at::GradMode::is_enabled())
+      for (auto& x : g)
+        x = AttnFirstOrder::apply(x, s[0], s[1], s[2], grad[0]);
     g.resize(15);  // nothing for the other arguments
     return g;
   }
@@ -1373,8 +1391,10 @@ at::Tensor attn_mod(const at::Tensor& q, const at::Tensor& k,
                     double cap, bool causal, const OptT& slopes,
                     const OptT& seg_q, const OptT& seg_k, const OptT& prefix,
                     const OptT& kv_len, const OptT& q_off, long off0) {
-  return ShapedMha::apply(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
-                          seg_k, prefix, kv_len, q_off, off0);
+  c10::DeviceGuard guard(q.device());
+  return ShapedMha::apply(attn_rows(q), attn_rows(k), attn_rows(v), H, Hkv,
+                          scale, cap, causal, slopes, seg_q, seg_k, prefix,
+                          kv_len, q_off, off0);
 }
 
 at::Tensor attn_decode(const at::Tensor& q_, const at::Tensor& k_,

@@ -25,3 +25,25 @@ def test_embedding_forward_mode_raises():
     with torch.enable_grad(), pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: RAW["Embedding"](idx, t), (w,),
                        (torch.ones_like(w),))
+
+
+def test_attention_twice_raises():
+    """The first derivative is the same under create_graph; the second one
+    raises, also where the queries had to be copied for the kernels."""
+    from anand_mxnet_amd.ops.registry import RAW
+    for odd in (0, 1):
+        t = [torch.randn(2, 5, 2 * 16 + odd, device="cuda").bfloat16()
+             .requires_grad_() for _ in range(3)]
+
+        def f():
+            return RAW["multi_head_attention"](
+                *[x[..., :32] for x in t], 2, num_kv_heads=2, logit_cap=5.0)
+
+        plain = torch.autograd.grad(f().sum(), t)
+        g = torch.autograd.grad(f().sum(), t, create_graph=True)
+        for x, y in zip(plain, g):
+            assert torch.equal(x, y.detach())
+        for y in g:
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad((y.float() ** 2).sum(), t,
+                                    retain_graph=True, allow_unused=True)

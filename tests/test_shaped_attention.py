@@ -186,3 +186,13 @@ def test_integers_past_32_bits(far):
     want = f(*a, 2, causal=True, prefix_length=ints(7, 0))._t
     got = f(*a, 2, causal=True, prefix_length=ints(far, -far))._t
     assert torch.equal(got, want)
+
+
+def test_second_derivative():
+    """The composition on the CPU has one."""
+    from anand_mxnet_amd.ops.registry import RAW
+    t = [torch.randn(1, 3, 8, dtype=torch.float64).requires_grad_()
+         for _ in range(3)]
+    assert torch.autograd.gradgradcheck(
+        lambda *x: RAW["multi_head_attention"](*x, 2, num_kv_heads=2,
+                                               logit_cap=5.0, causal=True), t)
