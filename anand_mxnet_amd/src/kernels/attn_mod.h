@@ -132,28 +132,32 @@ DEVINL T attn_lds(lds_char* sm, unsigned at) {
 // dst + 16 (4) * lane.  Written as assembly because the compiler waits for
 // every copy in flight before any LDS read that follows a builtin one, which
 // would undo the double buffering; it names no register that a load fills.
+// M0 is read one state after it is written, and declared, so that a value that
+// the compiler puts there itself is not taken as still in place.
 // Whoever reads the tile waits with attn_wait_copies and a barrier.
 DEVINL void copy_lds16(const void* g, unsigned dst) {
   asm volatile(
       "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
       :
       : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
-      : "memory");
+      : "memory", "m0");
 }
-// the same from base + off
+// the same from base + off.  The compiler does not see that a load reads the
+// pair that holds base: five states after a vector instruction wrote it (a
+// move of a spilled pair may do so right before) are waited for here.
 DEVINL void copy_lds16(const void* base, unsigned off, unsigned dst) {
   asm volatile(
-      "s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+      "s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
       :
       : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst))
-      : "memory");
+      : "memory", "m0");
 }
 DEVINL void copy_lds4(const void* g, unsigned dst) {
   asm volatile(
       "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
       :
       : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
-      : "memory");
+      : "memory", "m0");
 }
 // All but the last N copies have landed.
 template <int N>

@@ -60,8 +60,11 @@ if __name__ == "__main__":
                     "cxx": ["-O3", "-std=c++17"],
                     # packed fp32 instructions stay off: some of their forms
                     # have given wrong results on this hardware
+                    # and assembly that names M0, which the compiler does
+                    # not allocate, is no cause for a remark
                     "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
-                             "-Xclang", "-packed-fp32-ops"],
+                             "-Xclang", "-packed-fp32-ops",
+                             "-Wno-inline-asm"],
                 },
             )
         ],
