@@ -106,8 +106,9 @@ void dropout_bwd_bf16(const bf16*, const unsigned char*, bf16*, long, float,
 void emb_lookup(int, bool, bool, const void*, const void*, void*, long, int,
                 long, float, hipStream_t);
 int emb_chunks(long);
+long emb_ws(long, long);
 void emb_grad(int, bool, bool, const void*, const void*, void*, int*, int2*,
-              float*, int, int, int, float, hipStream_t);
+              float*, int*, int, int, int, float, hipStream_t);
 // clip_norm.hip
 long clip_entries(long);
 long clip_ws(long);
@@ -1619,11 +1620,13 @@ at::Tensor embedding_bwd(const at::Tensor& idx, const at::Tensor& dy,
   auto sorted = at::empty({ntok, 2}, iopt);
   auto part = at::empty({(long)mxa::emb_chunks(ntok), 2, D},
                         dy.options().dtype(at::kFloat));
+  at::Tensor ws;
+  if (long n = mxa::emb_ws(ntok, vocab)) ws = at::empty({n}, iopt);
   mxa::emb_grad(dt, rows16(dy.data_ptr(), D, dy.element_size()),
                 ix.scalar_type() == at::kLong, ix.data_ptr(), dy.data_ptr(),
                 dW.data_ptr(), start.data_ptr<int>(),
                 (int2*)sorted.data_ptr<int>(), part.data_ptr<float>(),
-                (int)ntok, (int)D, (int)vocab, (float)scale, cur_stream());
+                ws.defined() ? ws.data_ptr<int>() : nullptr, (int)ntok, (int)D, (int)vocab, (float)scale, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return dW;
 }

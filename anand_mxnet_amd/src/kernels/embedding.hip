@@ -6,8 +6,9 @@
 //
 // An index outside [0, vocab) gives a row of zeros and adds to nothing.
 // Both directions are bound by memory.  The gradient is summed in 32 bits in
-// the order of the tokens and rounded once, by three launches:
-//   1. emb_sort    tokens ordered by row (stable), and where each row starts
+// the order of the tokens and rounded once:
+//   1. emb_sort    tokens ordered by row (stable), and where each row starts;
+//                  for many tokens or rows a sort by digits instead
 //   2. emb_reduce  EMB_CHUNK sorted tokens to a wave: rows that lie inside a
 //                  chunk are final, the two at its ends may be partial; rows
 //                  without a token are cleared by further blocks
@@ -19,6 +20,8 @@
 // 768: 9, 14, 15 and 7.  The order is bound by the two passes that every block
 // makes over all indices, from L2.
 #include <hip/hip_fp16.h>
+
+#include <algorithm>
 
 #include "common.h"
 
@@ -101,7 +104,7 @@ constexpr int EMB_ROWS = 512;    // rows of a block at most
 // BATCH: groups of 64 tokens that a wave reads at once.
 template <typename I, int BATCH>
 __global__ __launch_bounds__(1024) void emb_sort_kernel(
-    const I* __restrict__ idx, int ntok, int vocab, int R, int rlog2, int p0,
+    const I* __restrict__ idx, int ntok, int vocab, int R, int rlog2,
     int* __restrict__ start, int2* __restrict__ sorted) {
   __shared__ int cnt[EMB_ROWS * EMB_WAVES];  // [row][wave]
   __shared__ unsigned list[EMB_WAVES][64 * BATCH];
@@ -109,7 +112,7 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const u64 lower = (1ull << lane) - 1;
-  const int r0 = (p0 + (int)blockIdx.x) * R;
+  const int r0 = blockIdx.x * R;
   const int nr = min(R, vocab - r0);
   for (int i = threadIdx.x; i < R * EMB_WAVES; i += 1024) cnt[i] = 0;
   __syncthreads();
@@ -233,6 +236,186 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
 }
 
 // ---------------------------------------------------------------------------
+// 1 for many tokens or rows: the work above is blocks times tokens.  A stable
+// sort by digits of the row, lowest first, takes a few passes over the tokens
+// instead.  Each pass divides them into segments of a block each:
+//   emb_digits   counts every digit of a segment
+//   emb_scan     sums a digit's counts over the segments before each
+//   emb_scatter  counts once more by wave, which gives every wave its places,
+//                and writes (row, token) there; equal digits within 64 tokens
+//                are ranked by lane
+// Tokens outside the table count as of one row behind it.  The last pass knows
+// where each value of the highest digit begins; emb_start finds the rows from
+// there by halving.  262144 tokens in 2 ** 22 rows, three passes: 52 us, the
+// starts 39, bound by the passes' launches and the reads that follow one
+// another in the halving; 2 ** 20 tokens in 10 ** 7 rows 70 and 96.
+// ---------------------------------------------------------------------------
+constexpr int EMB_BITS = 11;      // of a digit at most: 32 KB of counters
+constexpr int EMB_SEG = 2048;     // tokens of a segment at least
+constexpr int EMB_SEGS = 1024;    // segments at most
+
+template <typename I>
+struct EmbIndices {
+  const I* idx;
+  int vocab;
+  DEVINL int2 at(int t) const {
+    const I x = idx[t];
+    const bool in = sizeof(I) == 8 ? (u64)x < (u64)(unsigned)vocab
+                                   : (unsigned)x < (unsigned)vocab;
+    return make_int2(in ? (int)x : vocab, t);
+  }
+};
+
+struct EmbPairs {
+  const int2* pair;
+  DEVINL int2 at(int t) const { return pair[t]; }
+};
+
+template <typename S>
+__global__ __launch_bounds__(256) void emb_digits_kernel(
+    S src, int ntok, int len, int shift, int bits, int* __restrict__ cnt) {
+  __shared__ int h[1 << EMB_BITS];
+  const int nd = 1 << bits;
+  for (int i = threadIdx.x; i < nd; i += 256) h[i] = 0;
+  __syncthreads();
+  const int t0 = blockIdx.x * len;
+  const int t1 = ntok - t0 < len ? ntok : t0 + len;
+#pragma unroll 4
+  for (int t = t0 + (int)threadIdx.x; t < t1; t += 256)
+    atomicAdd(&h[(src.at(t).x >> shift) & (nd - 1)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i < nd; i += 256)
+    cnt[(long)blockIdx.x * nd + i] = h[i];
+}
+
+// cnt: [nseg][nd], every entry becomes the sum of those before it; total: [nd]
+__global__ __launch_bounds__(256) void emb_scan_kernel(
+    int* __restrict__ cnt, int* __restrict__ total, int nseg, int nd) {
+  __shared__ int part[16][16];
+  const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
+  int* const p = cnt + blockIdx.x * 16 + l;
+  const int per = (nseg + 15) / 16;
+  const int a = min(nseg, g * per), e = min(nseg, a + per);
+  int sum = 0;
+#pragma unroll 8
+  for (int i = a; i < e; ++i) sum += p[(long)i * nd];
+  part[g][l] = sum;
+  __syncthreads();
+  int run = 0;
+  for (int i = 0; i < g; ++i) run += part[i][l];
+  if (g == 15) total[blockIdx.x * 16 + l] = run + sum;
+#pragma unroll 8
+  for (int i = a; i < e; ++i) {
+    const int c = p[(long)i * nd];
+    p[(long)i * nd] = run;
+    run += c;
+  }
+}
+
+// first: [nd + 1], where each digit begins; null but in the last pass
+template <typename S>
+__global__ __launch_bounds__(256) void emb_scatter_kernel(
+    S src, int ntok, int len, int shift, int bits,
+    const int* __restrict__ cnt, const int* __restrict__ total,
+    int* __restrict__ first, int2* __restrict__ out) {
+  __shared__ int place[4][1 << EMB_BITS];
+  __shared__ int tot[4];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u64 lower = (1ull << lane) - 1;
+  const int nd = 1 << bits;
+  for (int i = threadIdx.x; i < nd; i += 256)
+    place[0][i] = place[1][i] = place[2][i] = place[3][i] = 0;
+  __syncthreads();
+  const int t0 = blockIdx.x * len;
+  const int t1 = ntok - t0 < len ? ntok : t0 + len;
+  // a quarter to a wave, groups of 64 tokens whole
+  const int quarter = (t1 - t0 + 255) / 256 * 64;
+  const int w0 = min(t1, t0 + wave * quarter), w1 = min(t1, w0 + quarter);
+#pragma unroll 4
+  for (int t = w0 + lane; t < w1; t += 64)
+    atomicAdd(&place[wave][(src.at(t).x >> shift) & (nd - 1)], 1);
+
+  // a thread takes a run of the digits
+  const int per = (nd + 255) / 256;
+  const int a = min(nd, (int)threadIdx.x * per), e = min(nd, a + per);
+  int sum = 0;
+  for (int i = a; i < e; ++i) sum += total[i];
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 63) tot[wave] = inc;
+  __syncthreads();
+  int run = inc - sum;
+  for (int w = 0; w < wave; ++w) run += tot[w];
+  for (int i = a; i < e; ++i) {
+    if (first && blockIdx.x == 0) first[i] = run;
+    int at = run + cnt[(long)blockIdx.x * nd + i];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int c = place[w][i];
+      place[w][i] = at;
+      at += c;
+    }
+    run += total[i];
+  }
+  if (first && blockIdx.x == 0 && threadIdx.x == 0) first[nd] = ntok;
+  __syncthreads();
+
+  // a wave's counters are its own, and its LDS accesses stay in order
+  constexpr int U = 4;
+  for (int tb = w0; tb < w1; tb += 64 * U) {
+    int2 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = tb + u * 64 + lane;
+      x[u] = t < w1 ? src.at(t) : make_int2(0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = tb + u * 64 + lane < w1;
+      const int digit = (x[u].x >> shift) & (nd - 1);
+      u64 same = __ballot(on);
+      for (int bit = 0; bit < bits; ++bit) {
+        const bool one = (digit >> bit) & 1;
+        const u64 bal = __ballot(one);
+        same &= one ? bal : ~bal;
+      }
+      if (on) {
+        const int rank = __popcll(same & lower);
+        const int pos = place[wave][digit] + rank;
+        out[pos] = x[u];
+        // the last lane of a digit moves its counter on
+        if (rank == __popcll(same) - 1) place[wave][digit] = pos + 1;
+      }
+    }
+  }
+}
+
+// start[r]: the first place whose row is r or higher
+__global__ __launch_bounds__(256) void emb_start_kernel(
+    const int2* __restrict__ sorted, const int* __restrict__ first, int vocab,
+    int shift, int* __restrict__ start) {
+  for (long r = (long)blockIdx.x * 256 + threadIdx.x; r <= vocab;
+       r += (long)gridDim.x * 256) {
+    int lo = first[r >> shift], hi = first[(r >> shift) + 1];
+    if (shift > 0) {
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (sorted[mid].x < (int)r)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+    }
+    start[r] = lo;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // 2. Sums.  Waves [0, nchunk * ns) take a chunk (from chunk0 on) and a slice
 // of 64 V columns; the rest of the grid clears rows that no token hits.
 // part: [nchunk][2][D], the sums of a chunk's first row where it began in an
@@ -243,17 +426,27 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
     const int2* __restrict__ sorted, const int* __restrict__ start,
     const T* __restrict__ dy, T* __restrict__ dW, float* __restrict__ part,
     int vocab, int D, float scale, int chunk0, int nchunk, int ns,
-    int sumblocks) {
+    int sumblocks, int zrows, int zlog2) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x >= sumblocks) {
+    // zrows rows of a wave at a time, 1 << zlog2 lanes to each
     const int nv = D / V;
     const float z[V] = {};
-    for (long r = (blockIdx.x - sumblocks) * 4 + wave; r < vocab;
-         r += (gridDim.x - sumblocks) * 4) {
-      if (start[r] != start[r + 1]) continue;
-      for (int c = lane; c < nv; c += 64)
-        emb_store<T, V>(dW + r * D + (long)c * V, z, 1.f);
+    const int sub = lane >> zlog2, l = lane & ((1 << zlog2) - 1);
+    const long step = (long)(gridDim.x - sumblocks) * 4 * zrows;
+    for (long r0 = ((long)(blockIdx.x - sumblocks) * 4 + wave) * zrows;
+         r0 < vocab; r0 += step) {
+      const long r = r0 + lane;
+      const u64 empty = __ballot(lane < zrows && r < vocab &&
+                                 start[min(r, (long)vocab)] ==
+                                     start[min(r + 1, (long)vocab)]);
+      if (empty == 0) continue;
+      for (int k = sub; k < zrows; k += 64 >> zlog2) {
+        if (!(empty >> k & 1)) continue;
+        for (int c = l; c < nv; c += 1 << zlog2)
+          emb_store<T, V>(dW + (r0 + k) * D + (long)c * V, z, 1.f);
+      }
     }
     return;
   }
@@ -319,8 +512,8 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// 3. Rows that cross chunks.  A block looks at the last row of one chunk; if
-// it began there and goes on, the block adds its parts.  Few parts: the
+// 3. Rows that cross chunks.  A block looks at the last rows of per chunks; if
+// one began there and goes on, the block adds its parts.  Few parts: the
 // first of EMB_JOIN blocks of the chunk adds them for all columns.  Many:
 // each block takes a share of the columns, and 8 groups of 32 threads a
 // share of the parts each, joined in order.
@@ -331,64 +524,80 @@ template <typename T, int PV>
 __global__ __launch_bounds__(256) void emb_join_kernel(
     const int2* __restrict__ sorted, const int* __restrict__ start,
     const float* __restrict__ part, T* __restrict__ dW, int vocab, int D,
-    float scale, int chunk0) {
+    float scale, int chunk0, int nchunk, int per) {
   __shared__ float sums[8][32][PV];
+  __shared__ u64 todo;
   const int n = start[vocab];
-  const int chunk = chunk0 + (int)blockIdx.x;
-  const int end = (chunk + 1) * EMB_CHUNK;
-  if (end >= n) return;  // nothing follows this chunk
-  const int key = sorted[end - 1].x;
-  const int s0 = start[key], s1 = start[key + 1];
-  if (s1 <= end || s0 < chunk * EMB_CHUNK) return;
-  const int parts = (s1 - 1) / EMB_CHUNK - chunk + 1;
-  const int nv = D / PV;
-  const float* p0 = part + ((long)chunk * 2 + 1) * D;  // first part
-  const float* p1 = part + ((long)chunk * 2) * D;      // others: + 2 D i
-  T* out = dW + (long)key * D;
-  if (parts <= 32) {
-    if (blockIdx.y != 0) return;
-    for (int v = threadIdx.x; v < nv; v += 256) {
-      float y[PV], x[PV];
-      emb_load<float, PV>(p0 + v * PV, y);
-#pragma unroll 4
-      for (int i = 1; i < parts; ++i) {
-        emb_load<float, PV>(p1 + (long)i * 2 * D + v * PV, x);
-#pragma unroll
-        for (int k = 0; k < PV; ++k) y[k] += x[k];
-      }
-      emb_store<T, PV>(out + v * PV, y, scale);
+  const int first = chunk0 + (int)blockIdx.x * per;
+  if (threadIdx.x < 64) {  // per is 64 at most
+    const int chunk = first + (int)threadIdx.x;
+    bool on = (int)threadIdx.x < per && chunk < nchunk - 1;
+    const long end = ((long)chunk + 1) * EMB_CHUNK;
+    on = on && end < n;  // else nothing follows this chunk
+    if (on) {
+      const int key = sorted[end - 1].x;
+      on = start[key + 1] > end && start[key] >= chunk * EMB_CHUNK;
     }
-    return;
+    const u64 all = __ballot(on);
+    if (threadIdx.x == 0) todo = all;
   }
-  const int lo = (int)((long)nv * blockIdx.y / EMB_JOIN);
-  const int hi = (int)((long)nv * (blockIdx.y + 1) / EMB_JOIN);
-  const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
-  const int share = (parts + 7) / 8;
-  const int a = g * share, e = min(parts, a + share);
-  for (int vb = lo; vb < hi; vb += 32) {
-    const int v = vb + l;
-    float y[PV] = {};
-    if (v < hi) {
-#pragma unroll 8
-      for (int i = a; i < e; ++i) {
-        float x[PV];
-        emb_load<float, PV>(
-            (i == 0 ? p0 : p1 + (long)i * 2 * D) + v * PV, x);
+  __syncthreads();
+  const u64 all = todo;
+  for (u64 left = all; left; left &= left - 1) {
+    const int chunk = first + __builtin_ctzll(left);
+    const int end = (chunk + 1) * EMB_CHUNK;
+    const int key = sorted[end - 1].x;
+    const int s1 = start[key + 1];
+    const int parts = (s1 - 1) / EMB_CHUNK - chunk + 1;
+    const int nv = D / PV;
+    const float* p0 = part + ((long)chunk * 2 + 1) * D;  // first part
+    const float* p1 = part + ((long)chunk * 2) * D;      // others: + 2 D i
+    T* out = dW + (long)key * D;
+    if (parts <= 32) {
+      if (blockIdx.y != 0) continue;
+      for (int v = threadIdx.x; v < nv; v += 256) {
+        float y[PV], x[PV];
+        emb_load<float, PV>(p0 + v * PV, y);
+#pragma unroll 4
+        for (int i = 1; i < parts; ++i) {
+          emb_load<float, PV>(p1 + (long)i * 2 * D + v * PV, x);
 #pragma unroll
-        for (int k = 0; k < PV; ++k) y[k] += x[k];
+          for (int k = 0; k < PV; ++k) y[k] += x[k];
+        }
+        emb_store<T, PV>(out + v * PV, y, scale);
       }
+      continue;
     }
+    const int lo = (int)((long)nv * blockIdx.y / EMB_JOIN);
+    const int hi = (int)((long)nv * (blockIdx.y + 1) / EMB_JOIN);
+    const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int share = (parts + 7) / 8;
+    const int a = g * share, e = min(parts, a + share);
+    for (int vb = lo; vb < hi; vb += 32) {
+      const int v = vb + l;
+      float y[PV] = {};
+      if (v < hi) {
+#pragma unroll 8
+        for (int i = a; i < e; ++i) {
+          float x[PV];
+          emb_load<float, PV>(
+              (i == 0 ? p0 : p1 + (long)i * 2 * D) + v * PV, x);
 #pragma unroll
-    for (int k = 0; k < PV; ++k) sums[g][l][k] = y[k];
-    __syncthreads();
-    if (g == 0 && v < hi) {
+          for (int k = 0; k < PV; ++k) y[k] += x[k];
+        }
+      }
 #pragma unroll
-      for (int w = 1; w < 8; ++w)
+      for (int k = 0; k < PV; ++k) sums[g][l][k] = y[k];
+      __syncthreads();
+      if (g == 0 && v < hi) {
 #pragma unroll
-        for (int k = 0; k < PV; ++k) y[k] += sums[w][l][k];
-      emb_store<T, PV>(out + v * PV, y, scale);
+        for (int w = 1; w < 8; ++w)
+#pragma unroll
+          for (int k = 0; k < PV; ++k) y[k] += sums[w][l][k];
+        emb_store<T, PV>(out + v * PV, y, scale);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -438,25 +647,94 @@ int emb_chunks(long ntok) {
   return (int)((ntok + EMB_CHUNK - 1) / EMB_CHUNK);
 }
 
-// start: [vocab + 1], sorted: [ntok], part: [emb_chunks][2][D]
+// How the tokens are ordered.  By blocks the time goes with tokens (and some
+// 4096 more for a block's start) times blocks beyond one for each compute
+// unit, by digits with the passes.  The whole gradient of rows of 64, in us by
+// blocks and by digits:
+//   1000 rows       16384 tokens 24 and 32,   65536 54 and 40
+//   32768 rows      32768 tokens 39 and 50,   65536 59 and 57,  262144 209, 100
+//   250000 rows     16384 tokens 44 and 56,   65536 79 and 64,  262144 221, 97
+//   2 ** 20 rows    512 tokens   64 and 59,   65536 186 and 79
+//   10 ** 7 rows    512 tokens   540 and 312, 16384 772 and 354
+struct EmbOrder {
+  int rlog2;        // rows of a block, as a power of two
+  unsigned blocks;
+  int bits, passes; // by digits: of this many bits; no passes: by blocks
+  int len, nseg;    // and segments of this many tokens
+  long ws;          // integers of workspace
+};
+
+static EmbOrder emb_order(long ntok, long vocab) {
+  EmbOrder o = {};
+  while ((1 << o.rlog2) < EMB_ROWS && (long)256 << o.rlog2 < vocab) ++o.rlog2;
+  o.blocks = (unsigned)((vocab + (1l << o.rlog2) - 1) >> o.rlog2);
+  int bits = 4;  // of the row behind the last one too
+  while (vocab >> bits) ++bits;
+  const int passes = (bits + EMB_BITS - 1) / EMB_BITS;
+  if ((ntok + 4096) * std::max(256l, (long)o.blocks) <=
+      16384l * 256 * (passes + 1))
+    return o;
+  o.passes = passes;
+  o.bits = (bits + o.passes - 1) / o.passes;
+  o.len = (int)std::max((long)EMB_SEG, (ntok + EMB_SEGS - 1) / EMB_SEGS);
+  o.nseg = (int)((ntok + o.len - 1) / o.len);
+  // the other buffer of (row, token); counts, totals and first places
+  o.ws = (o.passes > 1 ? 2 * ntok : 0) + ((o.nseg + 2l) << o.bits) + 1;
+  return o;
+}
+
+long emb_ws(long ntok, long vocab) { return emb_order(ntok, vocab).ws; }
+
+template <typename S>
+static void emb_pass(const EmbOrder& o, S src, int pass, int ntok, int* cnt,
+                     int2* out, hipStream_t s) {
+  const int nd = 1 << o.bits, shift = pass * o.bits;
+  int* total = cnt + (long)o.nseg * nd;
+  int* first = pass == o.passes - 1 ? total + nd : nullptr;
+  emb_digits_kernel<S><<<o.nseg, 256, 0, s>>>(src, ntok, o.len, shift, o.bits,
+                                              cnt);
+  emb_scan_kernel<<<nd / 16, 256, 0, s>>>(cnt, total, o.nseg, nd);
+  emb_scatter_kernel<S><<<o.nseg, 256, 0, s>>>(src, ntok, o.len, shift, o.bits,
+                                               cnt, total, first, out);
+}
+
+// start: [vocab + 1], sorted: [ntok], part: [emb_chunks][2][D], ws: [emb_ws]
 void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
               const void* dy, void* dW, int* start, int2* sorted,
-              float* part, int ntok, int D, int vocab, float scale,
+              float* part, int* ws, int ntok, int D, int vocab, float scale,
               hipStream_t s) {
-  int lg = 0;
-  while ((1 << lg) < EMB_ROWS && (long)256 << lg < vocab) ++lg;
-  const int R = 1 << lg;
-  const unsigned nb = (unsigned)(((long)vocab + R - 1) / R);
+  const EmbOrder o = emb_order(ntok, vocab);
+  const int R = 1 << o.rlog2, lg = o.rlog2;
+  const unsigned nb = o.blocks;
   // 16 groups at once keep the lists of 16384 tokens from the first pass to
-  // the second: 14.2 us, not 17.8 (32768 rows; 65536 tokens 48 and 51).  They
-  // gain nothing for few tokens (4096: 7.3 and 6.6) and leave room for one
-  // block on a compute unit (250000 rows: 25 and 23).
+  // the second: 14.2 us, not 17.8 (32768 rows).  They gain nothing for few
+  // tokens (4096: 7.3 and 6.6) and leave room for one block on a compute unit
+  // (250000 rows: 25 and 23).
   const bool wide = ntok > 8192 && nb <= 256;
-#define GO(I, N)                                                         \
-  for (unsigned p = 0; p < nb; p += EMB_LAUNCH)                          \
-  emb_sort_kernel<I, N><<<min(EMB_LAUNCH, nb - p), 1024, 0, s>>>(        \
-      (const I*)idx, ntok, vocab, R, lg, (int)p, start, sorted)
-  if (idx64 && wide)
+#define GO(I, N)                                                       \
+  emb_sort_kernel<I, N><<<nb, 1024, 0, s>>>((const I*)idx, ntok, vocab, \
+                                            R, lg, start, sorted)
+  if (o.passes) {
+    int2* other = (int2*)ws;
+    int* cnt = ws + (o.passes > 1 ? 2l * ntok : 0);
+    for (int p = 0; p < o.passes; ++p) {
+      // the last pass writes to sorted
+      int2* dst = (o.passes - 1 - p) % 2 ? other : sorted;
+      const int2* src = dst == sorted ? other : sorted;
+      if (p > 0)
+        emb_pass(o, EmbPairs{src}, p, ntok, cnt, dst, s);
+      else if (idx64)
+        emb_pass(o, EmbIndices<long>{(const long*)idx, vocab}, p, ntok, cnt,
+                 dst, s);
+      else
+        emb_pass(o, EmbIndices<int>{(const int*)idx, vocab}, p, ntok, cnt,
+                 dst, s);
+    }
+    const long rows = ((long)vocab + 256) / 256;
+    emb_start_kernel<<<(unsigned)std::min(rows, (long)EMB_LAUNCH), 256, 0,
+                       s>>>(sorted, cnt + ((o.nseg + 1l) << o.bits), vocab,
+                            (o.passes - 1) * o.bits, start);
+  } else if (idx64 && wide)
     GO(long, 16);
   else if (idx64)
     GO(long, 8);
@@ -470,6 +748,12 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
   do {                                                                       \
     const int ns = (D / (V) + 63) / 64;                                      \
     const int most = max(1, (int)(EMB_LAUNCH * 4l / ns));                    \
+    /* cleared by 8192 waves, whose lanes take as many rows as they cover */ \
+    int zlog2 = 0, zrows = 1;                                                \
+    while (zlog2 < 6 && (1 << zlog2) < D / (V)) ++zlog2;                     \
+    while (zrows < 64 &&                                                     \
+           (zrows < 64 >> zlog2 || 16384l * zrows <= vocab))                 \
+      zrows *= 2;                                                            \
     for (int c0 = 0; c0 < nchunk; c0 += most) {                              \
       const int nc = min(most, nchunk - c0);                                 \
       unsigned sb = (unsigned)(((long)nc * ns + 3) / 4);                     \
@@ -477,13 +761,17 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
       if (c0 > 0) zb = 0;                                                    \
       emb_reduce_kernel<T, V><<<sb + zb, 256, 0, s>>>(                       \
           sorted, start, (const T*)dy, (T*)dW, part, vocab, D, scale, c0,    \
-          nc, ns, (int)sb);                                                  \
+          nc, ns, (int)sb, zrows, zlog2);                                    \
     }                                                                        \
     constexpr int PV = (V) == 1 ? 1 : 4;                                     \
-    for (int c0 = 0; c0 < nchunk - 1; c0 += EMB_LAUNCH)                      \
+    /* chunks of a block: few blocks start for nothing */                    \
+    const int per = max(1, min(64, nchunk / 2048));                          \
+    const int jb = (nchunk - 2 + per) / per;                                 \
+    for (int j = 0; j < jb; j += EMB_LAUNCH)                                 \
       emb_join_kernel<T, PV>                                                 \
-          <<<dim3(min((int)EMB_LAUNCH, nchunk - 1 - c0), EMB_JOIN), 256, 0,  \
-             s>>>(sorted, start, part, (T*)dW, vocab, D, scale, c0);         \
+          <<<dim3(min((int)EMB_LAUNCH, jb - j), EMB_JOIN), 256, 0, s>>>(     \
+              sorted, start, part, (T*)dW, vocab, D, scale, j * per, nchunk, \
+              per);                                                          \
   } while (0)
 #define F(T, V) \
   if (vec)      \
