@@ -466,7 +466,8 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
         bad("query, key and value must be (batch, tokens, heads * size)")
     B, Tq, HD = q.shape
     Bk, Tk, KD = k.shape
-    H, Hkv = int(num_heads), int(num_kv_heads or num_heads)
+    H = int(num_heads)
+    Hkv = H if num_kv_heads is None else int(num_kv_heads)
     if H <= 0 or HD == 0 or HD % H:
         bad(f"{HD} columns do not divide into {H} heads")
     if Hkv <= 0 or H % Hkv:

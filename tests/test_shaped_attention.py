@@ -196,3 +196,9 @@ def test_second_derivative():
     assert torch.autograd.gradgradcheck(
         lambda *x: RAW["multi_head_attention"](*x, 2, num_kv_heads=2,
                                                logit_cap=5.0, causal=True), t)
+
+
+def test_refuses_no_kv_heads():
+    q = _x(2, 5, 16)
+    with pytest.raises(MXNetError):
+        nd.multi_head_attention(q, q, q, 2, num_kv_heads=0)
