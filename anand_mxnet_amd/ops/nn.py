@@ -13,6 +13,7 @@ the reference.  Dispatch contract (MI355X-first):
 """
 from __future__ import annotations
 
+import operator
 import os
 import torch
 import torch.nn.functional as F
@@ -510,7 +511,10 @@ def _shaped_mha(q, k, v, num_heads, num_kv_heads, scale, logit_cap, slopes,
     kv_len = _attn_ints(kv_len, (B,), "kv_length", q, 0, Tk)
     off0 = 0
     if q_off is not None and not isinstance(q_off, torch.Tensor):
-        off0, q_off = int(q_off), None
+        try:
+            off0, q_off = operator.index(q_off), None
+        except TypeError:
+            bad("query_offset must be an integer or an array of them")
         if abs(off0) >= 1 << 30:
             bad("query_offset is out of range")
     far = (1 << 30) - 1  # behind every key, or before it

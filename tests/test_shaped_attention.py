@@ -202,3 +202,11 @@ def test_refuses_no_kv_heads():
     q = _x(2, 5, 16)
     with pytest.raises(MXNetError):
         nd.multi_head_attention(q, q, q, 2, num_kv_heads=0)
+
+
+@pytest.mark.parametrize("off", [1.5, 2.0, "3", [1, 2], np.zeros(2, int)])
+def test_refuses_offsets_that_are_no_integers(off):
+    q = _x(2, 5, 16)
+    with pytest.raises(MXNetError):
+        nd.multi_head_attention(q, q, q, 2, query_offset=off)
+    nd.multi_head_attention(q, q, q, 2, query_offset=np.int64(2))
