@@ -43,14 +43,22 @@ def clip_global_norm(arrays, max_norm, check_isfinite=True):
     GPU path: nd.multi_clip_global_norm, which sums and scales all arrays in
     two kernels; call that one where the host need not wait for the norm."""
     assert len(arrays) > 0
+    from ..ops.optim import _clip_global_norm
     from ..ops.registry import RAW
     ts = [a._t for a in arrays]
     if ts[0].is_cuda:
         try:
-            norm = float(RAW["multi_clip_global_norm"](ts, max_norm))
+            norm = float(_clip_global_norm(ts, max_norm, mark=False))
         except MXNetError:
-            pass  # other types, several devices, shared memory: one by one
+            # other types or strides, several devices, shared memory: one by
+            # one
+            pass
         else:
+            # arrays below the limit stay as a backward saved them; the norm
+            # here is rounded to 32 bits
+            if max_norm < norm * (1 + 1e-6):
+                torch.autograd.graph.increment_version(
+                    [t for t in ts if not t.is_inference()])
             if check_isfinite and not math.isfinite(norm):
                 import warnings
                 warnings.warn("nan or inf is detected. Clipping results "

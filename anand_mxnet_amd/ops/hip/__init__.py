@@ -781,10 +781,10 @@ def multi_sumsq(blob, ntens, nchunks, bf16in):
 
 
 @register_gpu("multi_clip_global_norm")
-def multi_clip_global_norm(arrays, max_norm, out):
+def multi_clip_global_norm(arrays, max_norm, out, mark=True):
     """One norm over all arrays and their clipping (clip_norm.hip); the
-    factor stays on the device."""
-    return _C.clip_global_norm(arrays, out, max_norm)
+    factor stays on the device.  mark: out counts as written."""
+    return _C.clip_global_norm(arrays, out, max_norm, mark)
 
 
 # ---------------------------------------------------------------------------

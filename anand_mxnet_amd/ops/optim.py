@@ -208,6 +208,12 @@ def multi_clip_global_norm(arrays, max_norm, out=None):
     are.  GPU: bfloat16, float16 and float32, mixed as they come, two kernels
     (clip_norm.hip) for up to 164 arrays.  An array that is written must not
     overlap another one."""
+    return _clip_global_norm(arrays, max_norm, out)
+
+
+def _clip_global_norm(arrays, max_norm, out=None, mark=True):
+    """mark=False (contiguous arrays on the GPU): autograd is not told of the
+    write, the caller does so if there was one."""
     from ..base import MXNetError
 
     def need(ok, what):
@@ -228,9 +234,9 @@ def multi_clip_global_norm(arrays, max_norm, out=None):
             # the extension checks the rest: many arrays, little time
             try:
                 return gpu_impl("multi_clip_global_norm")(arrays, max_norm,
-                                                          out)
+                                                          out, mark)
             except (RuntimeError, TypeError) as e:
-                if "not contiguous" not in str(e):
+                if not mark or "not contiguous" not in str(e):
                     if isinstance(e, RuntimeError) \
                             and "clip_global_norm: " not in str(e):
                         raise

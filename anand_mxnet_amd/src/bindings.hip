@@ -1693,7 +1693,7 @@ at::Tensor embedding(const at::Tensor& idx, const at::Tensor& W,
 // src[i] itself), norm over all of src; returns the norm.
 at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
                             const std::vector<at::Tensor>& dst,
-                            double max_norm) {
+                            double max_norm, bool mark) {
   TORCH_CHECK(!src.empty() && src.size() == dst.size(),
               "clip_global_norm: one output for each array");
   const auto dev = src[0].device();
@@ -1746,7 +1746,7 @@ at::Tensor clip_global_norm(const std::vector<at::Tensor>& src,
     if (s.write) wend = std::max(wend, s.e);
   }
   for (const auto& t : dst)  // autograd must know of the write
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    if (mark && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   auto norm = at::empty({}, src[0].options().dtype(at::kFloat));
   if (sp.empty()) return norm.zero_();
   auto ws = at::empty({mxa::clip_ws((long)sp.size())},
@@ -2186,7 +2186,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale") = 1.0);
   m.def("embedding_bwd", &embedding_bwd, py::arg("idx"), py::arg("dy"),
         py::arg("vocab"), py::arg("scale") = 1.0);
-  m.def("clip_global_norm", &clip_global_norm);
+  m.def("clip_global_norm", &clip_global_norm, py::arg("src"),
+        py::arg("dst"), py::arg("max_norm"), py::arg("mark") = true);
   m.def("act_fwd", &act_fwd);
   m.def("act_bwd", &act_bwd);
   m.def("build_opt_descs", &build_opt_descs);
