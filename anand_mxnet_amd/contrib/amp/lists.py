@@ -10,8 +10,10 @@ LP16_FUNCS = [
 ]
 
 # arguments of LP16_FUNCS that keep their type: constants that the op itself
-# holds in fp32 (a slope's rounding would grow with the distance)
+# holds in fp32 (a slope's rounding would grow with the distance), and indices
+# that come as floats (above 256 bf16 holds every other one at most)
 LP16_KEEP_ARGS = {
+    "Embedding": ("data",),
     "multi_head_attention": ("distance_slopes",),
 }
 

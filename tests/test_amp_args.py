@@ -51,3 +51,12 @@ def test_distance_slopes_keep_their_bits(amp_on, monkeypatch, by_name):
                                 None, s)
     assert seen["q"].dtype == torch.bfloat16
     assert torch.equal(seen["slopes"], slopes)
+
+
+def test_float_indices_keep_their_rows(amp_on):
+    w = torch.arange(1000.0)[:, None].expand(1000, 4).contiguous()
+    idx = torch.tensor([255.0, 257.0, 511.0, 999.0])
+    out = nd.Embedding(nd.from_torch(idx), nd.from_torch(w), input_dim=1000,
+                       output_dim=4)._t
+    assert out.dtype == torch.bfloat16
+    assert torch.equal(out, w[idx.long()].bfloat16())
