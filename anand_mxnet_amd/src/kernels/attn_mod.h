@@ -142,15 +142,37 @@ DEVINL void copy_lds16(const void* g, unsigned dst) {
       : "v"(g), "s"(__builtin_amdgcn_readfirstlane(dst))
       : "memory", "m0");
 }
-// the same from base + off.  The compiler does not see that a load reads the
-// pair that holds base: five states after a vector instruction wrote it (a
-// move of a spilled pair may do so right before) are waited for here.
-DEVINL void copy_lds16(const void* base, unsigned off, unsigned dst) {
+// Two or four of them, from base + off[p] to places 1024 bytes apart.  The
+// compiler does not see that a load reads the pair that holds base: five
+// states after a vector instruction wrote it (a move of a spilled pair may do
+// so right before) are waited for here, once for all.
+DEVINL void copy_lds16x2(const void* base, const unsigned* off,
+                         unsigned dst) {
   asm volatile(
-      "s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
+      "s_mov_b32 m0, %1\n\ts_nop 3\n\t"
+      "global_load_lds_dwordx4 %2, %0\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %0"
       :
-      : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst))
-      : "memory", "m0");
+      : "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off[0]),
+        "v"(off[1])
+      : "memory", "m0", "scc");
+}
+DEVINL void copy_lds16x4(const void* base, const unsigned* off,
+                         unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\ts_nop 3\n\t"
+      "global_load_lds_dwordx4 %2, %0\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %0\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, %0\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %5, %0"
+      :
+      : "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off[0]),
+        "v"(off[1]), "v"(off[2]), "v"(off[3])
+      : "memory", "m0", "scc");
 }
 DEVINL void copy_lds4(const void* g, unsigned dst) {
   asm volatile(
@@ -212,8 +234,14 @@ struct Stager {
     const unsigned dst = img + wave * (N * 1024);
     const bf16* g0 = uniform_ptr(base + (long)row0 * stride);
     if (row0 + NROW <= row_end && Dact == D && seg == nullptr) {
+      static_assert(N == 2 || N % 4 == 0, "copies of a wave");
+      if constexpr (N == 2) {
+        copy_lds16x2(g0, off, dst);
+      } else {
 #pragma unroll
-      for (int p = 0; p < N; ++p) copy_lds16(g0, off[p], dst + p * 1024);
+        for (int p = 0; p < N; p += 4)
+          copy_lds16x4(g0, off + p, dst + p * 1024);
+      }
     } else {
 #pragma unroll 1  // rare: small code counts for more
       for (int p = 0; p < N; ++p) {

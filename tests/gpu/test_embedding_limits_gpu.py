@@ -81,7 +81,9 @@ def test_orders(vocab, D, n, dt):
     out = torch.rand(n, generator=g, device="cuda") < 0.1
     heap[out] = torch.randint(-3, 3, (int(out.sum()),), generator=g,
                               device="cuda") + vocab
-    for idx in (even, heap.to(torch.int32)):
+    wide = heap.clone()
+    wide[::97] += 2 ** 40
+    for idx in (even, heap.to(torch.int32), wide):
         want, bound = _sum64(idx, dy, vocab, 0.5)
         got = _C.embedding_bwd(idx, dy, vocab, 0.5)
         assert ((got.double() - want).abs() <= bound).all()
