@@ -554,12 +554,13 @@ def _shaped_mha_oracle(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
         ok = ok & (seg_q[:, :, None] == seg_k[:, None, :])
         live = live & (seg_k >= 0)
     ok = ok & live[:, None, :]
-    # keys and values that no query can see may hold anything
+    # keys and values that no query can see may hold anything, and so may
+    # queries that see none, and their gradients
     gone = ~live.reshape(B, Tk, 1)
     k = k.masked_fill(gone, 0.0)
     v = v.masked_fill(gone, 0.0)
-    if seg_q is not None:
-        q = q.masked_fill((seg_q < 0)[:, :, None], 0.0)
+    blind = ~ok.any(-1)[:, :, None]
+    q = q.masked_fill(blind, 0.0)
     qh = q.reshape(B, Tq, Hkv, G, D).permute(0, 2, 3, 1, 4).to(ct)
     kh = k.reshape(B, Tk, Hkv, 1, D).permute(0, 2, 3, 1, 4).to(ct)
     vh = v.reshape(B, Tk, Hkv, 1, D).permute(0, 2, 3, 1, 4).to(ct)
@@ -573,7 +574,8 @@ def _shaped_mha_oracle(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
     some = ok.any(-1)[:, None, None, :, None]
     p = F.softmax(s.masked_fill(~some, 0.0), dim=-1).masked_fill(~some, 0.0)
     out = torch.matmul(p, vh)
-    return out.permute(0, 3, 1, 2, 4).reshape(B, Tq, HD).to(q.dtype)
+    out = out.permute(0, 3, 1, 2, 4).reshape(B, Tq, HD).to(q.dtype)
+    return out.masked_fill(blind, 0.0)
 
 
 @register("multi_head_attention")
@@ -614,7 +616,8 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
     Lengths and offsets in arrays may be of any size: those past the keys on
     either side count as the border (32-bit integers take no extra launch).
 
-    A query that sees no key gives a row of zeros and no gradient.  Few
+    A query that sees no key gives a row of zeros and no gradient, whatever
+    it and the gradient of its row hold.  Few
     queries outside autograd.record() take the form that splits the keys
     over the chip.  Positions count exactly up to 2**24.  These forms take
     neither a dense mask nor dropout."""

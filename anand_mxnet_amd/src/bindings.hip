@@ -1293,6 +1293,9 @@ std::vector<at::Tensor> attn_mod_bwd(
   a.lse = lse.data_ptr<float>();
   auto delta = at::empty_like(lse);
   a.delta = delta.data_ptr<float>();
+  auto blind = at::empty({a.B, H, a.TqP / 32},
+                         q.options().dtype(at::kInt));
+  a.blind = blind.data_ptr<int>();
   if (a.seg_q) {
     a.rng_q = (const int2*)rng_q->data_ptr<int>();
     a.rng_k = (const int2*)rng_k->data_ptr<int>();

@@ -43,6 +43,7 @@ struct AttnArgs {
   float* lse;  // [B, H, TqP] log2 of the softmax sum; +inf: row sees nothing
   const bf16* dout;
   float* delta;  // [B, H, TqP] minus sum_d dout * out
+  int* blind;    // [B, H, TqP / 32] whether some of 32 queries see nothing
   bf16 *dq, *dk, *dv;
   float* ws;     // partial results of a split launch
   long qsb, ksb, vsb, osb, gsb;  // batch strides, elements
@@ -197,6 +198,16 @@ DEVINL unsigned attn_here(unsigned x) {
   return x;
 }
 
+// The kernel's arguments, read where this stands: what is needed now and then
+// takes no registers all the way from the kernel's start.  For kernels whose
+// only argument they are.
+typedef __attribute__((address_space(4))) const AttnArgs ConstArgs;
+DEVINL ConstArgs* attn_args_here() {
+  ConstArgs* a = (ConstArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
+}
+
 // A pointer that is the same in all lanes, where the compiler knows it.
 DEVINL const bf16* uniform_ptr(const bf16* p) {
   const size_t x = (size_t)p;
@@ -204,6 +215,10 @@ DEVINL const bf16* uniform_ptr(const bf16* p) {
   const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(x >> 32));
   return (const bf16*)((size_t)hi << 32 | lo);
 }
+
+// Whether a row counts: its id is not negative, or its query sees something.
+DEVINL bool attn_open(int id) { return id >= 0; }
+DEVINL bool attn_open(float lse) { return lse != MXA_INF; }
 
 // Copies NROW consecutive rows of a head into an image, by NW waves, each
 // lane 16 bytes of N instructions.  off holds where its chunks lie behind
@@ -226,14 +241,15 @@ struct Stager {
     }
   }
   // Rows row0 on; img is the image's LDS address.  Rows at or behind
-  // row_end, rows whose id in seg is negative (seg may be null) and chunks at
-  // or behind Dact read as zero.
+  // row_end, rows that gate (it may be null) shuts out and chunks at or behind
+  // Dact read as zero.
+  template <typename G>
   DEVINL void copy(const bf16* base, long stride, int row0, int row_end,
-                   int Dact, const int* seg, unsigned img, int wave,
+                   int Dact, const G* gate, unsigned img, int wave,
                    int lane) const {
     const unsigned dst = img + wave * (N * 1024);
     const bf16* g0 = uniform_ptr(base + (long)row0 * stride);
-    if (row0 + NROW <= row_end && Dact == D && seg == nullptr) {
+    if (row0 + NROW <= row_end && Dact == D && gate == nullptr) {
       static_assert(N == 2 || N % 4 == 0, "copies of a wave");
       if constexpr (N == 2) {
         copy_lds16x2(g0, off, dst);
@@ -249,7 +265,7 @@ struct Stager {
         const int ch = (lane % CPR) ^ attn_key<D>(r);
         const bf16* g = g0 + (long)r * stride + ch * 8;
         bool ok = row0 + r < row_end && ch * 8 < Dact;
-        if (ok && seg) ok = seg[row0 + r] >= 0;
+        if (ok && gate) ok = attn_open(gate[row0 + r]);
         if (!ok) g = (const bf16*)attn_zero16;
         copy_lds16(g, dst + p * 1024);
       }

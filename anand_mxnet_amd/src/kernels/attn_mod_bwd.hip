@@ -107,7 +107,15 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
       delta = dot8(gf[kk], attn_load_row(lp, kk * 2 + half, a.D, ok), delta);
     }
     delta += __shfl_xor(delta, 32, 64);
+    if (lse == MXA_INF) {  // sees nothing: its gradient may hold anything
+      delta = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) gf[kk] = bf16x8{};
+    }
     if (half == 0 && qi < a.TqP) a.delta[row] = -delta;
+    const bool blind = __ballot(qok && lse == MXA_INF) != 0;
+    if (lane == 0 && q0 < a.TqP)
+      a.blind[((long)b * a.H + h) * (a.TqP / 32) + q0 / 32] = blind;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       attn_settle(qf[kk]);
@@ -260,11 +268,14 @@ attn_mod_dkv_kernel(AttnArgs a) {
   const int2* rng = m.has_seg ? attn_ranges(a.rng_q, b, a.Tq) : nullptr;
   const int* sqb = m.has_seg ? a.seg_q + (long)b * a.Tq : nullptr;
 
-  // Verdict on query tile t: bit 0 block, bit 1 wave, bit 2 all pairs of the
-  // wave visible, bit 3 negative ids.
-  auto judge = [&](int t) {
+  // Verdict on query tile t of a head: bit 0 block, bit 1 wave, bit 2 all
+  // pairs of the wave visible, bit 3 queries that see nothing.
+  auto judge = [&](int t, int g) {
     int2 r = make_int2(0, 0);
     if (m.has_seg) r = attn_join(rng[2 * t], rng[2 * t + 1]);
+    ConstArgs* c = attn_args_here();
+    const int2 bl = ((const int2*)c->blind)[
+        ((long)b * c->H + hk * c->G + g) * ntq + t];
     const int p0 = t * 64 + m.off, p1 = min(t * 64 + 63, a.Tq - 1) + m.off;
     bool any = p1 >= blo && blo != NEVER, wany = p1 >= wlo && wlo != NEVER;
     bool all = p0 >= whi && whi != NEVER;
@@ -275,14 +286,14 @@ attn_mod_dkv_kernel(AttnArgs a) {
     }
     any = any && t % a.nsplit == split;
     return (any ? 1 : 0) | (wany ? 2 : 0) | (all ? 4 : 0) |
-           (m.has_seg && r.x < 0 ? 8 : 0);
+           (bl.x | bl.y ? 8 : 0);
   };
 
   int cg = 0, base = -64;
-  u64 act = 0, wact = 0, wful = 0, neg = 0;
+  u64 act = 0, wact = 0, wful = 0, blind = 0;
   struct QTile {
     int g, t;
-    bool work, full, neg;
+    bool work, full, blind;
   };
   auto next = [&]() -> QTile {
     while (act == 0) {
@@ -292,16 +303,16 @@ attn_mod_dkv_kernel(AttnArgs a) {
         if (++cg >= a.G) return QTile{-1, 0, false, false, false};
       }
       int t = base + lane;
-      int v = t < ntq ? judge(t) : 0;
+      int v = t < ntq ? judge(t, cg) : 0;
       act = __ballot(v & 1);
       wact = __ballot(v & 2);
       wful = __ballot(v & 4);
-      neg = __ballot(v & 8);
+      blind = __ballot(v & 8);
     }
     int i = __builtin_ctzll(act);
     act &= act - 1;
     return QTile{cg, base + i, (bool)((wact >> i) & 1),
-                 (bool)((wful >> i) & 1), (bool)((neg >> i) & 1)};
+                 (bool)((wful >> i) & 1), (bool)((blind >> i) & 1)};
   };
 
   Stager<D, 64, NW> qs, gs;
@@ -309,12 +320,14 @@ attn_mod_dkv_kernel(AttnArgs a) {
   gs.init(a.gst, wave, lane);
   auto stage = [&](int buf, const QTile& t) {
     const int h = hk * a.G + t.g, r = t.t * 64;
-    const int* sg = t.neg ? sqb : nullptr;
+    const long row = ((long)b * a.H + h) * a.TqP;
+    // queries that see nothing, and their gradients, may hold anything
+    const float* sg = nullptr;
+    if (t.blind) sg = attn_args_here()->lse + row;
     qs.copy(a.q + b * a.qsb + (long)h * a.D, a.qst, r, a.Tq, a.D, sg,
             lds0 + buf * TILE, wave, lane);
     gs.copy(a.dout + b * a.gsb + (long)h * a.D, a.gst, r, a.Tq, a.D, sg,
             lds0 + G0 + buf * TILE, wave, lane);
-    const long row = ((long)b * a.H + h) * a.TqP;
     if (wave == 0)
       attn_stage64(a.lse + row, r, a.TqP, lds0 + ST0 + buf * 256, lane);
     if (wave == 1)

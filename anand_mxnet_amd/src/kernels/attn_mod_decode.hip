@@ -68,11 +68,13 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
   // the wave's own reads of a tile end before the next one is copied over it
   auto stage_k = [&](int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    ks.copy(kb, a.kst, tile * 32, kend, a.D, nullptr, lds0 + kat, 0, lane);
+    ks.copy(kb, a.kst, tile * 32, kend, a.D, (const int*)nullptr, lds0 + kat,
+            0, lane);
   };
   auto stage_v = [&](int tile) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    vs.copy(vb, a.vst, tile * 32, kend, a.D, nullptr, lds0 + vat, 0, lane);
+    vs.copy(vb, a.vst, tile * 32, kend, a.D, (const int*)nullptr, lds0 + vat,
+            0, lane);
   };
 
   f32x16 o[DB];

@@ -1,6 +1,11 @@
 """Attention with shaped scores at the borders of its arguments (GPU)."""
+import os
+import sys
+
 import pytest
 import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(__file__)))
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +97,57 @@ def test_largest_launch(ids):
     out = mx.nd.multi_head_attention(*[mx.nd.from_torch(t) for t in ts], 8,
                                      **kw)._t
     assert torch.equal(out, ts[2])  # one key: its value
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_nan_in_blind_queries(i):
+    import anand_mxnet_amd as mx
+    from test_shaped_attention import blind_cases, check_blind
+
+    def same(x, y):
+        assert torch.equal(x, y)
+    check_blind(blind_cases()[i], torch.bfloat16,
+                lambda t: mx.nd.from_torch(t.cuda()), same)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [None, 8.0])
+def test_nan_in_blind_queries_of_long_sequences(D, cap):
+    """Several tiles, shared heads, rows at both ends of them."""
+    import anand_mxnet_amd as mx
+    g = torch.Generator().manual_seed(8)
+    T, H = 700, 4
+    q, g0 = [torch.randn((2, T, H * D), generator=g).bfloat16()
+             for _ in range(2)]
+    k, v = [torch.randn((2, T, 2 * D), generator=g).bfloat16()
+            for _ in range(2)]
+    seg = torch.randint(0, 3, (2, T), generator=g, dtype=torch.int32)
+    keys = seg.clone()
+    seg[:, [0, 63, 64, 200, 255, 256, T - 1]] = 8  # no key has that id
+    off = torch.tensor([-70, 0], dtype=torch.int32)
+    pos = torch.arange(T)[None] + off[:, None]
+    blind = (seg == 8) | (pos < 0)
+    for b in range(2):  # causal: an id that begins behind the query
+        for s in range(3):
+            first = int((keys[b] == s).nonzero()[0])
+            blind[b] |= (seg[b] == s) & (pos[b] < first)
+    got = []
+    for bad in (False, True):
+        q2, g2 = q.clone(), g0.clone()
+        if bad:
+            q2[blind], g2[blind] = float("nan"), float("inf")
+        a = [mx.nd.from_torch(t.cuda()) for t in (q2, k, v)]
+        for x in a:
+            x.attach_grad()
+        with mx.autograd.record():
+            out = mx.nd.multi_head_attention(
+                *a, H, num_kv_heads=2, causal=True, logit_cap=cap,
+                segment_ids=mx.nd.from_torch(seg.cuda()),
+                kv_segment_ids=mx.nd.from_torch(keys.cuda()),
+                query_offset=mx.nd.from_torch(off.cuda()))
+        out.backward(mx.nd.from_torch(g2.cuda()))
+        got.append([out._t.detach()] + [x.grad._t for x in a])
+    assert blind.sum() > 80
+    assert not got[0][0][blind].any() and not got[0][1][blind].any()
+    for x, y in zip(*got):
+        assert torch.isfinite(y).all() and torch.equal(x, y)

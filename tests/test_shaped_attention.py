@@ -210,3 +210,50 @@ def test_refuses_offsets_that_are_no_integers(off):
     with pytest.raises(MXNetError):
         nd.multi_head_attention(q, q, q, 2, query_offset=off)
     nd.multi_head_attention(q, q, q, 2, query_offset=np.int64(2))
+
+
+def blind_cases():
+    """Sizes, which queries see nothing, and the arguments that make it so."""
+    seg = np.array([[0, 0, 5, 1, 1, 7, 2, 2, 2]], np.int32)
+    keys = np.array([[0, 0, 0, 1, 1, 2, 2, 4, 4]], np.int32)
+    return [
+        (dict(causal=True, query_offset=np.array([-4], np.int32)),
+         [0, 1, 2, 3]),
+        (dict(segment_ids=seg, kv_segment_ids=keys), [2, 5]),
+        (dict(segment_ids=seg, kv_segment_ids=keys, causal=True,
+              logit_cap=4.0), [2, 5]),
+        (dict(kv_length=np.array([0], np.int32)), list(range(9))),
+    ]
+
+
+def check_blind(case, dtype, wrap, check):
+    """NaN in queries that see nothing and in the gradients of their rows
+    changes nothing anywhere."""
+    kw, rows = case
+    rng = np.random.default_rng(9)
+    q, k, v, g = [torch.from_numpy(rng.standard_normal((1, 9, 16))).to(dtype)
+                  for _ in range(4)]
+    kw = {n: wrap(torch.from_numpy(x)) if isinstance(x, np.ndarray) else x
+          for n, x in kw.items()}
+    got = []
+    for bad in (False, True):
+        q2, g2 = q.clone(), g.clone()
+        if bad:
+            q2[:, rows], g2[:, rows] = float("nan"), float("nan")
+        a = [wrap(t) for t in (q2, k, v)]
+        for x in a:
+            x.attach_grad()
+        with mx.autograd.record():
+            out = nd.multi_head_attention(*a, 2, num_kv_heads=2, **kw)
+        out.backward(wrap(g2))
+        got.append([out._t.detach()] + [x.grad._t for x in a])
+    assert not got[0][0][:, rows].any() and not got[0][1][:, rows].any()
+    for x, y in zip(*got):
+        check(x, y)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_nan_in_blind_queries(i):
+    def same(x, y):
+        assert torch.equal(x, y)
+    check_blind(blind_cases()[i], torch.float64, nd.from_torch, same)
