@@ -894,9 +894,9 @@ def _split_keys(B, Tq, H, G):
     """Whether the form that divides the keys over the chip is taken, rather
     than 128 queries a block: for few rows (query tokens times heads of a
     group), and where the blocks would leave half of the chip idle.  One
-    sequence of 32768 keys, 16 heads of 128: 256 queries take 158 us in that
-    form and 778 us in blocks, 1024 queries 804 and 791; 16 sequences of 4096
-    keys, 16 heads over 4: 16 queries 53 and 99, 64 queries 172 and 103."""
+    sequence of 32768 keys, 16 heads of 128: 256 queries take 142 us in that
+    form and 636 us in blocks, 1024 queries 804 and 656; 16 sequences of 4096
+    keys, 16 heads over 4: 16 queries 52 and 82, 64 queries 171 and 89."""
     return Tq * G <= 64 or B * H * ((Tq + 127) // 128) < 128
 
 

@@ -193,7 +193,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
 //
 // D = 64: four waves that hold V as operands in registers and K in LDS: with
 // K in registers as well, 193 of them, there is room for two blocks on a
-// compute unit, not three (sequences of 512 in four documents 103 and 93 us).
+// compute unit, not three (sequences of 512 in four documents 103 and 93 us,
+// though 1 to 5 registers and some 50 scalars are spilled for it).
 // D = 128: those 64 registers beside 128 of accumulators would leave room
 // for one wave on a SIMD only, and nothing to overlap its phases with.  K
 // and V lie in LDS instead, and eight waves share the keys: one half takes
@@ -539,7 +540,9 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(
 
 // Blocks of 128 keys are the unit of work and differ a lot under a causal
 // mask.  Few of them leave compute units idle at the end: their queries are
-// divided, as long as a part keeps some 16 tiles.  Heads of 64, three blocks
+// divided, as long as a part keeps some 16 tiles, those of all heads of a
+// group counted: with more than 16 heads to a key head there may be more parts
+// than tiles, and those without one add zeros.  Heads of 64, three blocks
 // on a compute unit, 8192 tokens of 16 heads over 8 without a cap: 579 us
 // with 512 blocks, 395 with 1024, 425 with 1536, the join counted; 2 x 4096
 // of 16 over 4: 322, 231, 245.  Heads of 128, one block on a compute unit,

@@ -275,7 +275,9 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
 }
 
 // Blocks a sequence's keys are divided among: enough to fill the chip twice
-// over, but no block with fewer than eight tiles (two a wave).
+// over, but no more than one for each 256 keys that the cache has room for:
+// eight tiles, two a wave, of a full one; the tiles that a shorter sequence
+// has are shared out evenly, and some blocks may get fewer or none.
 int attn_decode_splits(int B, int Hkv, int R, int Tk) {
   long base = (long)B * Hkv * cdiv_h(R, DEC_ROWS);
   long want = (1536 + base - 1) / base;
