@@ -1291,11 +1291,10 @@ std::vector<at::Tensor> attn_mod_bwd(
   a.gsb = dout.stride(0);
   a.gst = dout.stride(1);
   a.lse = lse.data_ptr<float>();
-  auto delta = at::empty_like(lse);
+  const long nd = lse.numel();  // a multiple of 64
+  auto delta = at::empty({nd + nd / 32}, lse.options());
   a.delta = delta.data_ptr<float>();
-  auto blind = at::empty({a.B, H, a.TqP / 32},
-                         q.options().dtype(at::kInt));
-  a.blind = blind.data_ptr<int>();
+  a.blind = (int*)(a.delta + nd);
   if (a.seg_q) {
     a.rng_q = (const int2*)rng_q->data_ptr<int>();
     a.rng_k = (const int2*)rng_k->data_ptr<int>();
