@@ -247,8 +247,8 @@ __global__ __launch_bounds__(1024) void emb_sort_kernel(
 // Tokens outside the table count as of one row behind it.  The last pass knows
 // where each value of the highest digit begins; emb_start finds the rows from
 // there by halving.  262144 tokens in 2 ** 22 rows, three passes: 52 us, the
-// starts 39, bound by the passes' launches and the reads that follow one
-// another in the halving; 2 ** 20 tokens in 10 ** 7 rows 70 and 96.
+// starts 21, bound by the passes' launches and the reads that follow one
+// another in the halving; 2 ** 20 tokens in 10 ** 7 rows 70 and 33.
 // ---------------------------------------------------------------------------
 constexpr int EMB_BITS = 11;      // of a digit at most: 32 KB of counters
 constexpr int EMB_SEG = 2048;     // tokens of a segment at least
@@ -395,23 +395,60 @@ __global__ __launch_bounds__(256) void emb_scatter_kernel(
   }
 }
 
-// start[r]: the first place whose row is r or higher
+// The first place in [lo, hi) whose row is r or higher; row(i) is the i-th.
+template <typename F>
+DEVINL int emb_first(F row, int lo, int hi, int r) {
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (row(mid) < r)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// start[r]: the first place whose row is r or higher.  A block takes 256 rows,
+// or EMB_SPAN of a large table, whose tokens it halves in LDS if they fit: the
+// halving in memory would be most of the time there (10 ** 7 rows 33 us, not
+// 96; 2 ** 22 21 and 39; 32768 rows 29 and 5, on 16 blocks).
+constexpr int EMB_SPAN = 2048, EMB_KEYS = 4096;
+
 __global__ __launch_bounds__(256) void emb_start_kernel(
-    const int2* __restrict__ sorted, const int* __restrict__ first, int vocab,
-    int shift, int* __restrict__ start) {
-  for (long r = (long)blockIdx.x * 256 + threadIdx.x; r <= vocab;
-       r += (long)gridDim.x * 256) {
-    int lo = first[r >> shift], hi = first[(r >> shift) + 1];
-    if (shift > 0) {
-      while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (sorted[mid].x < (int)r)
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-    }
-    start[r] = lo;
+    const int2* __restrict__ sorted, const int* __restrict__ first, int ntok,
+    int vocab, int shift, int span, int* __restrict__ start) {
+  __shared__ int keys[EMB_KEYS];
+  __shared__ int ends[2];
+  const long r0 = (long)blockIdx.x * span;
+  const long r1 = min(r0 + span, (long)vocab + 1);
+  if (span < EMB_SPAN) {
+    const long r = r0 + threadIdx.x;
+    if (r < r1)
+      start[r] = emb_first([&](int i) { return sorted[i].x; },
+                           first[r >> shift], first[(r >> shift) + 1],
+                           (int)r);
+    return;
+  }
+  if (threadIdx.x < 2) {
+    const long r = threadIdx.x ? r1 : r0;
+    int at = ntok;
+    if (r <= vocab)
+      at = emb_first([&](int i) { return sorted[i].x; }, first[r >> shift],
+                     first[(r >> shift) + 1], (int)r);
+    ends[threadIdx.x] = at;
+  }
+  __syncthreads();
+  const int lo = ends[0], n = ends[1] - lo;
+  if (n <= EMB_KEYS) {
+    for (int i = threadIdx.x; i < n; i += 256) keys[i] = sorted[lo + i].x;
+    __syncthreads();
+    for (long r = r0 + threadIdx.x; r < r1; r += 256)
+      start[r] = lo + emb_first([&](int i) { return keys[i]; }, 0, n, (int)r);
+  } else {
+    for (long r = r0 + threadIdx.x; r < r1; r += 256)
+      start[r] = emb_first([&](int i) { return sorted[i].x; },
+                           max(lo, first[r >> shift]),
+                           min(lo + n, first[(r >> shift) + 1]), (int)r);
   }
 }
 
@@ -730,10 +767,10 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
         emb_pass(o, EmbIndices<int>{(const int*)idx, vocab}, p, ntok, cnt,
                  dst, s);
     }
-    const long rows = ((long)vocab + 256) / 256;
-    emb_start_kernel<<<(unsigned)std::min(rows, (long)EMB_LAUNCH), 256, 0,
-                       s>>>(sorted, cnt + ((o.nseg + 1l) << o.bits), vocab,
-                            (o.passes - 1) * o.bits, start);
+    const int span = vocab >= 1 << 20 ? EMB_SPAN : 256;
+    emb_start_kernel<<<(unsigned)(vocab / span + 1), 256, 0, s>>>(
+        sorted, cnt + ((o.nseg + 1l) << o.bits), ntok, vocab,
+        (o.passes - 1) * o.bits, span, start);
   } else if (idx64 && wide)
     GO(long, 16);
   else if (idx64)
