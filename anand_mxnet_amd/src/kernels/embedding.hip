@@ -12,12 +12,12 @@
 //   2. emb_reduce  EMB_CHUNK sorted tokens to a wave: rows that lie inside a
 //                  chunk are final, the two at its ends may be partial; rows
 //                  without a token are cleared by further blocks
-//   3. emb_join    rows that cross chunks, their parts added in order
+//   3. emb_join    rows that cross chunks, their parts added in a fixed order
 // so a row that half of all tokens hit is spread over the chip like any
 // other, nothing is added by atomics and every run gives the same bits.
 // 16384 tokens, 32768 rows of 1024 in bf16: lookup 10 us (64 MB), order 14,
-// sums 20 (97 MB, 5 TB/s), rows that cross chunks 5; a table of two rows of
-// 768: 9, 14, 15 and 7.  The order is bound by the two passes that every block
+// sums 21 (97 MB, 4.6 TB/s), rows that cross chunks 6; a table of two rows of
+// 768: 9, 13, 16 and 7.  The order is bound by the two passes that every block
 // makes over all indices, from L2.
 #include <hip/hip_fp16.h>
 
@@ -551,9 +551,11 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
 // ---------------------------------------------------------------------------
 // 3. Rows that cross chunks.  A block looks at the last rows of per chunks; if
 // one began there and goes on, the block adds its parts.  Few parts: the
-// first of EMB_JOIN blocks of the chunk adds them for all columns.  Many:
-// each block takes a share of the columns, and 8 groups of 32 threads a
-// share of the parts each, joined in order.
+// first of EMB_JOIN blocks of the chunks adds them for all columns, 1 << jlog2
+// threads a chunk (262144 tokens, rows of 64 in bf16: 31 us with the block's
+// chunks one after another, 5 side by side).  Many: each block takes a share
+// of the columns, and groups of 1 << glog2 threads a share of the parts each,
+// joined in order.
 // ---------------------------------------------------------------------------
 constexpr int EMB_JOIN = 8;
 
@@ -561,9 +563,9 @@ template <typename T, int PV>
 __global__ __launch_bounds__(256) void emb_join_kernel(
     const int2* __restrict__ sorted, const int* __restrict__ start,
     const float* __restrict__ part, T* __restrict__ dW, int vocab, int D,
-    float scale, int chunk0, int nchunk, int per) {
-  __shared__ float sums[8][32][PV];
-  __shared__ u64 todo;
+    float scale, int chunk0, int nchunk, int per, int jlog2, int glog2) {
+  __shared__ float sums[256][PV];
+  __shared__ u64 todo[2];
   const int n = start[vocab];
   const int first = chunk0 + (int)blockIdx.x * per;
   if (threadIdx.x < 64) {  // per is 64 at most
@@ -571,46 +573,57 @@ __global__ __launch_bounds__(256) void emb_join_kernel(
     bool on = (int)threadIdx.x < per && chunk < nchunk - 1;
     const long end = ((long)chunk + 1) * EMB_CHUNK;
     on = on && end < n;  // else nothing follows this chunk
+    bool few = false;
     if (on) {
       const int key = sorted[end - 1].x;
-      on = start[key + 1] > end && start[key] >= chunk * EMB_CHUNK;
+      const int s1 = start[key + 1];
+      on = s1 > end && start[key] >= chunk * EMB_CHUNK;
+      few = (s1 - 1) / EMB_CHUNK - chunk + 1 <= 32;
     }
-    const u64 all = __ballot(on);
-    if (threadIdx.x == 0) todo = all;
+    const u64 f = __ballot(on && few), m = __ballot(on && !few);
+    if (threadIdx.x == 0) {
+      todo[0] = f;
+      todo[1] = m;
+    }
   }
   __syncthreads();
-  const u64 all = todo;
-  for (u64 left = all; left; left &= left - 1) {
-    const int chunk = first + __builtin_ctzll(left);
-    const int end = (chunk + 1) * EMB_CHUNK;
-    const int key = sorted[end - 1].x;
-    const int s1 = start[key + 1];
-    const int parts = (s1 - 1) / EMB_CHUNK - chunk + 1;
-    const int nv = D / PV;
+  const int nv = D / PV;
+  const u64 fews = blockIdx.y == 0 ? todo[0] : 0;
+  for (int k = threadIdx.x >> jlog2; fews && k < per; k += 256 >> jlog2) {
+    if (!(fews >> k & 1)) continue;
+    const int chunk = first + k;
+    const int key = sorted[(chunk + 1) * EMB_CHUNK - 1].x;
+    const int parts = (start[key + 1] - 1) / EMB_CHUNK - chunk + 1;
     const float* p0 = part + ((long)chunk * 2 + 1) * D;  // first part
     const float* p1 = part + ((long)chunk * 2) * D;      // others: + 2 D i
     T* out = dW + (long)key * D;
-    if (parts <= 32) {
-      if (blockIdx.y != 0) continue;
-      for (int v = threadIdx.x; v < nv; v += 256) {
-        float y[PV], x[PV];
-        emb_load<float, PV>(p0 + v * PV, y);
+    for (int v = threadIdx.x & ((1 << jlog2) - 1); v < nv; v += 1 << jlog2) {
+      float y[PV], x[PV];
+      emb_load<float, PV>(p0 + v * PV, y);
 #pragma unroll 4
-        for (int i = 1; i < parts; ++i) {
-          emb_load<float, PV>(p1 + (long)i * 2 * D + v * PV, x);
+      for (int i = 1; i < parts; ++i) {
+        emb_load<float, PV>(p1 + (long)i * 2 * D + v * PV, x);
 #pragma unroll
-          for (int k = 0; k < PV; ++k) y[k] += x[k];
-        }
-        emb_store<T, PV>(out + v * PV, y, scale);
+        for (int c = 0; c < PV; ++c) y[c] += x[c];
       }
-      continue;
+      emb_store<T, PV>(out + v * PV, y, scale);
     }
+  }
+  for (u64 left = todo[1]; left; left &= left - 1) {
+    const int chunk = first + __builtin_ctzll(left);
+    const int key = sorted[(chunk + 1) * EMB_CHUNK - 1].x;
+    const int parts = (start[key + 1] - 1) / EMB_CHUNK - chunk + 1;
+    const float* p0 = part + ((long)chunk * 2 + 1) * D;  // first part
+    const float* p1 = part + ((long)chunk * 2) * D;      // others: + 2 D i
+    T* out = dW + (long)key * D;
     const int lo = (int)((long)nv * blockIdx.y / EMB_JOIN);
     const int hi = (int)((long)nv * (blockIdx.y + 1) / EMB_JOIN);
-    const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
-    const int share = (parts + 7) / 8;
-    const int a = g * share, e = min(parts, a + share);
-    for (int vb = lo; vb < hi; vb += 32) {
+    // as many groups as the block's share of the columns leaves threads for
+    const int gl = 1 << glog2, ng = 256 >> glog2;
+    const int g = threadIdx.x >> glog2, l = threadIdx.x & (gl - 1);
+    const int share = (parts + ng - 1) / ng;
+    const int a = min(parts, g * share), e = min(parts, a + share);
+    for (int vb = lo; vb < hi; vb += gl) {
       const int v = vb + l;
       float y[PV] = {};
       if (v < hi) {
@@ -623,16 +636,18 @@ __global__ __launch_bounds__(256) void emb_join_kernel(
           for (int k = 0; k < PV; ++k) y[k] += x[k];
         }
       }
+      // the upper half of the groups hands its sums to the lower, and so on
+      for (int w = ng / 2; w > 0; w /= 2) {
+        if (g >= w && g < 2 * w)
 #pragma unroll
-      for (int k = 0; k < PV; ++k) sums[g][l][k] = y[k];
-      __syncthreads();
-      if (g == 0 && v < hi) {
+          for (int k = 0; k < PV; ++k) sums[threadIdx.x][k] = y[k];
+        __syncthreads();
+        if (g < w)
 #pragma unroll
-        for (int w = 1; w < 8; ++w)
-#pragma unroll
-          for (int k = 0; k < PV; ++k) y[k] += sums[w][l][k];
-        emb_store<T, PV>(out + v * PV, y, scale);
+          for (int k = 0; k < PV; ++k)
+            y[k] += sums[threadIdx.x + w * gl][k];
       }
+      if (g == 0 && v < hi) emb_store<T, PV>(out + v * PV, y, scale);
       __syncthreads();
     }
   }
@@ -688,11 +703,11 @@ int emb_chunks(long ntok) {
 // 4096 more for a block's start) times blocks beyond one for each compute
 // unit, by digits with the passes.  The whole gradient of rows of 64, in us by
 // blocks and by digits:
-//   1000 rows       16384 tokens 24 and 32,   65536 54 and 40
-//   32768 rows      32768 tokens 39 and 50,   65536 59 and 57,  262144 209, 100
-//   250000 rows     16384 tokens 44 and 56,   65536 79 and 64,  262144 221, 97
-//   2 ** 20 rows    512 tokens   64 and 59,   65536 186 and 79
-//   10 ** 7 rows    512 tokens   540 and 312, 16384 772 and 354
+//   1000 rows       16384 tokens 22 and 31,   65536 45 and 34
+//   32768 rows      32768 tokens 34 and 45,   65536 49 and 48,  262144 181, 74
+//   250000 rows     16384 tokens 43 and 55,   65536 73 and 58,  262144 208, 81
+//   2 ** 20 rows    512 tokens   65 and 60,   65536 183 and 76
+//   10 ** 7 rows    512 tokens   539 and 302, 16384 773 and 332
 struct EmbOrder {
   int rlog2;        // rows of a block, as a power of two
   unsigned blocks;
@@ -801,14 +816,20 @@ void emb_grad(int dtype, bool vec, bool idx64, const void* idx,
           nc, ns, (int)sb, zrows, zlog2);                                    \
     }                                                                        \
     constexpr int PV = (V) == 1 ? 1 : 4;                                     \
-    /* chunks of a block: few blocks start for nothing */                    \
-    const int per = max(1, min(64, nchunk / 2048));                          \
+    /* chunks of a block: few blocks start for nothing, and as many as its */ \
+    /* threads take side by side while that leaves 256 blocks              */ \
+    int jlog2 = 0;                                                           \
+    while (jlog2 < 8 && (1 << jlog2) < D / PV) ++jlog2;                      \
+    int glog2 = 0;                                                           \
+    while (glog2 < 5 && (EMB_JOIN << glog2) < D / PV) ++glog2;               \
+    const int per = max(                                                     \
+        1, min(64, max(nchunk / 2048, min(256 >> jlog2, nchunk / 256))));    \
     const int jb = (nchunk - 2 + per) / per;                                 \
     for (int j = 0; j < jb; j += EMB_LAUNCH)                                 \
       emb_join_kernel<T, PV>                                                 \
           <<<dim3(min((int)EMB_LAUNCH, jb - j), EMB_JOIN), 256, 0, s>>>(     \
               sorted, start, part, (T*)dW, vocab, D, scale, j * per, nchunk, \
-              per);                                                          \
+              per, jlog2, glog2);                                            \
   } while (0)
 #define F(T, V) \
   if (vec)      \
