@@ -16,11 +16,16 @@
 //
 // Bound by the matrix and the vector unit together, at the clock that they
 // leave (2.05 GHz).  16384 tokens in three documents, 16 heads of 128 over 8,
-// capped: dQ 930 us, 910 TFLOP/s, matrix unit 44 and vector unit 57 per cent
-// busy; dK and dV 1300 us, 815 TFLOP/s, 38 and 45 per cent (a library
-// product of 8192^3: 1166 TFLOP/s).  dS as one bf16 number took 743 and 1140.
-// Sequences of 512 in four documents, 16384 tokens, heads of 64: 77 and 93
+// capped: dQ 947 us, 893 TFLOP/s, matrix unit 45 and vector unit 58 per cent
+// busy; dK and dV 1353 us, 783 TFLOP/s, 38 and 44 per cent (a library
+// product of 8192^3 on such a card: 1116 TFLOP/s).  On one where it reached
+// 1166 they took 930 and 1300, and dS as one bf16 number 743 and 1140.
+// Sequences of 512 in four documents, 16384 tokens, heads of 64: 78 and 95
 // us, where moving the bytes takes 47 and 41.
+//
+// A query that sees nothing may hold anything, and so may the gradient of its
+// row: dQ leaves such a row out of delta, notes its 32 queries in `blind`, and
+// dK and dV stage the rows of noted tiles one by one, those as zeros.
 #include "attn_mod.h"
 
 namespace mxa {

@@ -19,13 +19,14 @@
 //
 // Bound by the vector unit, with the matrix unit behind it: per score two
 // exp2 and a reciprocal under a cap.  16384 tokens in three documents, 16
-// heads of 128 over 8, capped: 605 us, 700 TFLOP/s; vector unit 54, matrix
-// unit 32 per cent busy at 2.05 GHz.  One document, uncapped: 976 TFLOP/s,
-// where a library product of 8192^3 reaches 1166.  Two groups of four waves
-// that took turns at products and softmax, 256 queries a block, were no
-// faster (640 us; prefixes of 4095 tokens 240, not 215).  Sequences of 512 in
-// four documents, 16384 tokens, heads of 64: 53 us, where moving the bytes
-// takes 34; a block has four tiles, and its first loads and its stores weigh
+// heads of 128 over 8, capped: 623 us, 680 TFLOP/s; vector unit 58, matrix
+// unit 34 per cent busy at 2.05 GHz (605 us on a card where a library product
+// of 8192^3 reached 1166 TFLOP/s, not 1116; one document, uncapped, ran at 976
+// there).  Two groups of four waves that took turns at products and softmax,
+// 256 queries a block, were no faster (640 us there; prefixes of 4095 tokens
+// 240, not 215).  Sequences of 512 in four documents, 16384 tokens, heads of
+// 64: 54 us, where moving the bytes takes 34; a block has four tiles, and its
+// first loads and its stores weigh
 // as much.
 #include <type_traits>
 
