@@ -452,8 +452,8 @@ def _attn_ints(x, shape, what, q, lo=None, hi=None):
                          f"the queries are on {q.device}")
     if x.dtype is torch.int32 and x.is_contiguous():
         return x
-    if x.dtype is torch.int64 and lo is not None:
-        x = x.clamp(lo, hi)
+    if lo is not None and x.dtype is not torch.int32:
+        x = x.to(torch.int64).clamp(lo, hi)
     return x.to(torch.int32).contiguous()
 
 
@@ -619,8 +619,10 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
     A query that sees no key gives a row of zeros and no gradient, whatever
     it and the gradient of its row hold.  Few
     queries outside autograd.record() take the form that splits the keys
-    over the chip.  Positions count exactly up to 2**24.  These forms take
-    neither a dense mask nor dropout."""
+    over the chip.  Positions count exactly up to 2**24, and a distance bias
+    is held in 32 bits: where the nearest key that a query sees is d away,
+    its weights err by some slope * d * 2**-23.  These forms take neither a
+    dense mask nor dropout."""
     if (kv_length is not None or segment_ids is not None
             or logit_cap is not None or distance_slopes is not None
             or prefix_length is not None or query_offset is not None

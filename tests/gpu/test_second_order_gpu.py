@@ -47,3 +47,26 @@ def test_attention_twice_raises():
             with pytest.raises(RuntimeError, match="second derivative"):
                 torch.autograd.grad((y.float() ** 2).sum(), t,
                                     retain_graph=True, allow_unused=True)
+
+
+def test_transforms_raise():
+    """What the kernels cannot go through is refused, not dropped."""
+    from anand_mxnet_amd.ops.registry import RAW
+    w = torch.randn(3, 5, 8, device="cuda")
+    idx = torch.tensor([1, 3], device="cuda")
+    q = torch.randn(1, 5, 16, device="cuda").bfloat16()
+
+    def attn(t):
+        return RAW["multi_head_attention"](t, q, q, 2, num_kv_heads=2,
+                                           logit_cap=5.0)
+
+    def emb(t):
+        return RAW["Embedding"](idx, t)
+
+    with torch.enable_grad():
+        for f in (lambda: torch.func.vmap(emb)(w),
+                  lambda: torch.func.vmap(attn)(q[None]),
+                  lambda: torch.func.jvp(attn, (q,), (q,)),
+                  lambda: torch.func.grad(lambda t: emb(t).sum())(w[0])):
+            with pytest.raises(RuntimeError):
+                f()

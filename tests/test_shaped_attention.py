@@ -257,3 +257,15 @@ def test_nan_in_blind_queries(i):
     def same(x, y):
         assert torch.equal(x, y)
     check_blind(blind_cases()[i], torch.float64, nd.from_torch, same)
+
+
+def test_unsigned_lengths():
+    """Unsigned integers of 32 bits above 2**31 are lengths too."""
+    q = torch.randn(1, 4, 16)
+    a = [nd.from_torch(q)] * 3
+    want = nd.multi_head_attention(*a, 2, logit_cap=5.0)._t
+    for dt, n in ((torch.uint32, 2 ** 31 + 5), (torch.uint8, 200),
+                  (torch.int16, 4)):
+        n = nd.from_torch(torch.tensor([n], dtype=torch.int64).to(dt))
+        got = nd.multi_head_attention(*a, 2, logit_cap=5.0, kv_length=n)._t
+        assert torch.equal(got, want)
