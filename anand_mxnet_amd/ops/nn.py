@@ -567,9 +567,11 @@ def _shaped_mha_oracle(q, k, v, H, Hkv, scale, cap, causal, slopes, seg_q,
     s = torch.matmul(qh, kh.transpose(-1, -2)) * scale
     if cap:
         s = cap * torch.tanh(s / cap)
-    if slopes is not None:
-        s = s - slopes.to(ct).reshape(1, Hkv, G, 1, 1) \
-            * dist.abs()[:, None, None]
+    if slopes is not None and Tk:
+        # less the nearest key's distance, which a softmax does not see
+        far = dist.abs()
+        far = far - far.amin(-1, keepdim=True)
+        s = s - slopes.to(ct).reshape(1, Hkv, G, 1, 1) * far[:, None, None]
     s = s.masked_fill(~ok[:, None, None], float("-inf"))
     some = ok.any(-1)[:, None, None, :, None]
     p = F.softmax(s.masked_fill(~some, 0.0), dim=-1).masked_fill(~some, 0.0)
@@ -619,10 +621,12 @@ def multi_head_attention(q, k, v, num_heads, mask=None, dropout_p=0.0,
     A query that sees no key gives a row of zeros and no gradient, whatever
     it and the gradient of its row hold.  Few
     queries outside autograd.record() take the form that splits the keys
-    over the chip.  Positions count exactly up to 2**24, and a distance bias
-    is held in 32 bits: where the nearest key that a query sees is d away,
-    its weights err by some slope * d * 2**-23.  These forms take neither a
-    dense mask nor dropout."""
+    over the chip.  Distances count exactly up to 2**24 (less what lies
+    between the queries and the nearest key, where all of them are on one
+    side), and their bias is held in 32 bits: a query whose nearest key is d
+    away, in a document that begins far from it, has weights that err by
+    some slope * d * 2**-23.  These forms take neither a dense mask nor
+    dropout."""
     if (kv_length is not None or segment_ids is not None
             or logit_cap is not None or distance_slopes is not None
             or prefix_length is not None or query_offset is not None

@@ -311,6 +311,10 @@ struct RowSpan {
 // One sequence's masks, uniform over a block.
 struct SeqMask {
   int kv_len, prefix, off, causal, has_seg;
+  // what positions are moved by for the distance bias: where all queries lie
+  // behind all keys, or before them, the distances shrink by one number, which
+  // a softmax does not see and 32 bits would lose weights to
+  int shift;
 };
 
 DEVINL SeqMask attn_seq_mask(const AttnArgs& a, int b) {
@@ -322,6 +326,7 @@ DEVINL SeqMask attn_seq_mask(const AttnArgs& a, int b) {
   const long far = (1l << 30) - 1;
   const long off = (long)a.off0 + (a.q_off ? a.q_off[b] : 0);
   m.off = (int)min(max(off, -far), far);
+  m.shift = max(min(m.off, max(m.kv_len - 1, 0)), 1 - a.Tq) - m.off;
   m.causal = a.causal;
   m.has_seg = a.seg_q != nullptr;
   return m;

@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(AttnArgs a) {
                       dp);
         }
         const int j0 = cur.t * 64 + nb * 32 + 4 * half;
-        const float d0 = BIAS ? (float)(pos - j0) : 0.f;
+        const float d0 = BIAS ? (float)(pos + m.shift - j0) : 0.f;
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = attn_z<CAP>(f, s[i]);
@@ -404,7 +404,7 @@ attn_mod_dkv_kernel(AttnArgs a) {
         }
         const int r0 = nb * 32 + 4 * half;  // this lane's first tile row
         const int p0 = cur.t * 64 + r0 + m.off;
-        const float d0 = BIAS ? (float)(p0 - kj) : 0.f;
+        const float d0 = BIAS ? (float)(p0 + m.shift - kj) : 0.f;
         bf16x8 pf[2], df[2], dl[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(
       s = mfma32(attn_row_frag(sm, krow, kk, 0), qf[kk], s);
     if (more) stage_k(t + 4);
     const int j0 = t * 32 + 4 * half;
-    const float d0 = BIAS ? (float)(pos - j0) : 0.f;
+    const float d0 = BIAS ? (float)(pos + m.shift - j0) : 0.f;
     float x[16], mx = -MXA_INF;
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = attn_z<CAP>(f, s[i]);

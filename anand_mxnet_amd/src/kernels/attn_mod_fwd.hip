@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256, SHORT ? 4 : 2) void attn_mod_fwd_kernel(
     // queries: one addition for each four keys there.
     float mx = -MXA_INF, base = 0.f, step = 0.f;
     if (BIAS) {
-      const float d0 = (float)(pos - j0);
+      const float d0 = (float)(pos + m.shift - j0);
       if (cur.t * 64 + 63 <= wav.pmin) {
         base = f.slope * d0;
         step = -8.f * f.slope;

@@ -151,3 +151,44 @@ def test_nan_in_blind_queries_of_long_sequences(D, cap):
     assert not got[0][0][blind].any() and not got[0][1][blind].any()
     for x, y in zip(*got):
         assert torch.isfinite(y).all() and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("off", [10 ** 6, 2 ** 26 + 3, -10 ** 6])
+@pytest.mark.parametrize("Tq,causal,D", [(1, True, 64), (130, True, 128),
+                                         (130, False, 64), (2, False, 128)])
+def test_bias_far_from_the_keys(off, Tq, causal, D):
+    """Queries far behind all keys, or before them: the weights are those of
+    the distances' differences."""
+    from shaped_attention_ref import check, reference, visible
+    g = torch.Generator().manual_seed(12)
+    B, Tk, H = 2, 150, 2
+    q, dout = [torch.randn((B, Tq, H * D), generator=g).bfloat16()
+               for _ in range(2)]
+    k, v = [torch.randn((B, Tk, H * D), generator=g).bfloat16()
+            for _ in range(2)]
+    slopes = torch.tensor([0.5, 0.03])
+    kv_len = torch.tensor([150, 77])
+    ok, pos = visible(B, Tq, Tk, causal, kv_len=kv_len, off=off)
+    # less the nearest key's distance: the same softmax, exact in 64 bits
+    ref = reference(q, k, v, dout, H, H, ok, pos, slopes=slopes)
+    kw = dict(causal=causal, query_offset=off, kv_length=kv_len,
+              distance_slopes=slopes)
+    for train in (False, True):
+        if train:
+            import anand_mxnet_amd as mx
+            a = [mx.nd.from_torch(t.cuda()) for t in (q, k, v)]
+            for x in a:
+                x.attach_grad()
+            kd = {n: mx.nd.from_torch(x.cuda())
+                  if isinstance(x, torch.Tensor) else x
+                  for n, x in kw.items()}
+            with mx.autograd.record():
+                out = mx.nd.multi_head_attention(*a, H, num_kv_heads=H, **kd)
+            out.backward(mx.nd.from_torch(dout.cuda()))
+            got = dict(out=out._t, dq=a[0].grad._t, dk=a[1].grad._t,
+                       dv=a[2].grad._t)
+        else:
+            got = dict(out=_run([q.cuda(), k.cuda(), v.cuda()], False,
+                                **kw)[0])
+        for name, x in got.items():
+            check(name, x, ref[name])

@@ -269,3 +269,23 @@ def test_unsigned_lengths():
         n = nd.from_torch(torch.tensor([n], dtype=torch.int64).to(dt))
         got = nd.multi_head_attention(*a, 2, logit_cap=5.0, kv_length=n)._t
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("off", [10 ** 6, 2 ** 26 + 3, -10 ** 6])
+def test_bias_far_from_the_keys(off):
+    """In 32 bits too the weights are those of the distances' differences."""
+    q, k = torch.randn(1, 3, 16), torch.randn(1, 9, 16)
+    s = nd.from_torch(torch.tensor([0.5, 0.03]))
+    f = nd.multi_head_attention
+    got = f(*[nd.from_torch(t) for t in (q, k, k)], 2, distance_slopes=s,
+            query_offset=off)._t
+    want = f(*[nd.from_torch(t.double()) for t in (q, k, k)], 2,
+             distance_slopes=s, query_offset=9 if off > 0 else -3)._t
+    assert torch.allclose(got.double(), want, rtol=1e-4, atol=1e-5)
+
+
+def test_no_keys():
+    q, k = _x(1, 3, 16), _x(1, 0, 16)
+    out = nd.multi_head_attention(
+        q, k, k, 2, distance_slopes=nd.from_torch(torch.ones(2)))._t
+    assert out.shape == (1, 3, 16) and not out.any()
